@@ -2307,3 +2307,167 @@ def conv_rows(u, bias, taps, state, positions, row_seq, q_start, ctx_len, slots,
              out.stride(0), 1 if unit else 0, float(eps), float(q_scale), 1 if silu else 0, _ptr(out_bias), _ptr(copy),
              copy.stride(0) if copy is not None else 0, copy.shape[2] if copy is not None else 0, int(portions),
              ctypes.addressof(launches), _ptr(status), _stream()), f"conv_rows(channels={C}, taps={K})", kernels=launches.value)
+
+
+# ---- 8-bit and 4-bit formats: rows in e4m3 with a scale a row, weights in 8 bits a channel or 4 bits a group --------
+
+E4M3 = torch.float8_e4m3fn
+W4_SHIFTS = (0, 16, 4, 20, 8, 24, 12, 28)      # the bit of entry i of the eight that share an int32 word
+
+
+def _here(what: str, *ts) -> None:
+    """Every tensor is on the device whose stream the kernel is launched on."""
+    for t in ts:
+        if t is not None and not t.is_cuda:
+            raise KernelError("kernels take CUDA tensors only; there is no CPU path")
+    index = _device_index if _device_index is not None else torch.cuda.current_device()
+    for t in ts:
+        if t is not None and t.get_device() != index:
+            raise KernelError(f"{what}: a tensor is on device {t.get_device()}, the kernel is launched on device {index}")
+
+
+def _ld(t: torch.Tensor) -> int:
+    """Entries between the rows of a matrix (the stride of a single row says nothing)."""
+    return t.stride(0) if t.shape[0] > 1 else t.shape[1]
+
+
+def _rows_of(t, what: str) -> None:
+    _need(t.dim() == 2 and (t.stride(1) == 1 or t.shape[1] <= 1), f"{what} must be a matrix whose rows are contiguous")
+
+
+def _out_rows(t, what: str) -> None:
+    _rows_of(t, what)
+    _need(t.shape[0] <= 1 or t.stride(0) >= t.shape[1], f"{what}: its rows overlap")
+
+
+def _q8_out(out, scale, R: int, width: int, what: str) -> None:
+    _need(out.dtype == E4M3 and out.is_contiguous() and out.shape == (R, width), f"{what}: out must be contiguous float8_e4m3fn [{R}, {width}]")
+    _need(scale.dtype == torch.float32 and scale.is_contiguous() and scale.numel() == R, f"{what}: scale must be contiguous fp32 of {R} elements")
+
+
+def add_rmsnorm_q8(resid, delta, weight, eps: float, out, scale, rows=None, ahead=None, delta2=None, dst=None) -> None:
+    """``add_rmsnorm`` with its output in 8 bits: resid (fp32) += delta (+ delta2), y = weight * resid * rsqrt(mean(resid^2) + eps),
+    scale[r] = max(max |y[r]|, 2^-100) / 448 (fp32 [R]), out[r] = y[r] / scale[r] rounded to e4m3 ([R, d], contiguous).
+
+    The new stream goes into ``dst`` (fp32 like resid; default: resid, in place). With ``rows`` (int32 [R]) output row r comes from stream
+    row rows[r] and no stream is written. ``ahead``: as in ``add_rmsnorm``. delta and delta2: fp32 or bf16 alike. Sums are fp32."""
+    _here("add_rmsnorm_q8", resid, delta, weight, out, scale, rows, delta2, dst, ahead)
+    _need(resid.dim() == 2 and resid.dtype == torch.float32 and resid.is_contiguous(), "add_rmsnorm_q8: resid must be contiguous fp32 rows")
+    _i32(rows, "rows")
+    T, d = resid.shape
+    _need(weight.numel() == d and weight.is_contiguous(), "add_rmsnorm_q8: weight must be contiguous, as wide as the stream")
+    _need(delta2 is None or delta is not None, "add_rmsnorm_q8: delta2 goes beside delta")
+    for t in (delta, delta2):
+        _need(t is None or (t.is_contiguous() and t.shape == resid.shape and t.dtype == delta.dtype),
+              "add_rmsnorm_q8: delta and delta2 must be contiguous like resid, and of one dtype")
+    _need(dst is None or rows is None, "add_rmsnorm_q8: with rows no stream is written")
+    _need(dst is None or (dst.dtype == torch.float32 and dst.is_contiguous() and dst.shape == resid.shape), "add_rmsnorm_q8: dst must be contiguous fp32 like resid")
+    R = T if rows is None else rows.numel()
+    _q8_out(out, scale, R, d, "add_rmsnorm_q8")
+    xd, wd = F32 if delta is None else _dt(delta), _dt(weight)
+    if R == 0:
+        return
+    if rows is None and dst is None and delta is not None:
+        dst = resid
+    ahead_bytes = min(ahead.numel() * ahead.element_size(), AHEAD_BYTES) if ahead is not None and ahead.is_contiguous() else 0
+    f = _fn("quant_rows", "si_add_rmsnorm_q8",
+            [_c_p, _c_p, _c_p, _c_int, _c_p, _c_p, _c_int, _c_p, _c_p, _c_p, _c_int, _c_int, _c_f, _c_p, _c_ll, _c_p])
+    _check(f(_ptr(resid), _ptr(delta), _ptr(delta2), xd, _ptr(rows), _ptr(weight), wd, _ptr(dst), _ptr(out), _ptr(scale), R, d, float(eps),
+             _ptr(ahead) if ahead_bytes else None, ahead_bytes, _stream()), f"add_rmsnorm_q8(hidden={d})")
+
+
+def swiglu_q8(gu, out, scale, group=None) -> None:
+    """``swiglu`` with its output in 8 bits: y = silu(gate) * up (fp32) of the stacked projection gu [T, 2F] (fp32 or bf16, contiguous; gates
+    and ups interleaved in groups of ``group`` columns, default F), scale[t] = max(max |y[t]|, 2^-100) / 448, out[t] = y[t] / scale[t] in
+    e4m3 [T, F]."""
+    _here("swiglu_q8", gu, out, scale)
+    _need(out.dim() == 2 and gu.dim() == 2, "swiglu_q8: gu and out must be matrices")
+    T, F = out.shape
+    group = F if group is None else int(group)
+    _need(gu.shape == (T, 2 * F) and gu.is_contiguous(), "swiglu_q8: gu must be contiguous [T, 2F] for out [T, F]")
+    _q8_out(out, scale, T, F, "swiglu_q8")
+    dt = _dt(gu)
+    if T == 0:
+        return
+    _need(F > 0 and group > 0 and F % group == 0, "swiglu_q8: the group must divide F")
+    f = _fn("quant_rows", "si_swiglu_q8", [_c_p, _c_int, _c_p, _c_p, _c_int, _c_int, _c_int, _c_p])
+    _check(f(_ptr(gu), dt, _ptr(out), _ptr(scale), T, F, group, _stream()), f"swiglu_q8(F={F})")
+
+
+def quantize_q8(x, out, scale) -> None:
+    """Rows to 8 bits: scale[r] = max(max |x[r]|, 2^-100) / 448 (fp32 [R]), out[r] = x[r] / scale[r] rounded to e4m3 ([R, n], contiguous).
+    ``x``: fp32 or bf16 [R, n], its rows contiguous. For a product's rows, or a weight's, whose rows are output channels."""
+    _here("quantize_q8", x, out, scale)
+    _rows_of(x, "quantize_q8: x")
+    R, n = x.shape
+    _q8_out(out, scale, R, n, "quantize_q8")
+    dt = _dt(x)
+    if R == 0:
+        return
+    _need(n > 0, "quantize_q8: rows without entries")
+    f = _fn("quant_rows", "si_quantize_q8", [_c_p, _c_int, _c_ll, _c_p, _c_p, _c_int, _c_int, _c_p])
+    _check(f(_ptr(x), dt, _ld(x), _ptr(out), _ptr(scale), R, n, _stream()), f"quantize_q8(n={n})")
+
+
+def gemm_q8(a, a_scale, w, w_scale, out, status=None) -> None:
+    """out[m, n] = a_scale[m] * w_scale[n] * sum_k a[m, k] * w[n, k]: a [M, K] and w [N, K] in e4m3 (rows contiguous), scales fp32 [M] and
+    [N], out bf16 or fp32 [M, N]; sums fp32. ``status``: the status word that a kernel's bounded wait reports to."""
+    _here("gemm_q8", a, a_scale, w, w_scale, out, status)
+    _need(a.dtype == E4M3 and w.dtype == E4M3, "gemm_q8: a and w must be float8_e4m3fn")
+    _rows_of(a, "gemm_q8: a"); _rows_of(w, "gemm_q8: w"); _out_rows(out, "gemm_q8: out")
+    M, K = a.shape
+    N = w.shape[0]
+    _need(w.shape[1] == K and out.shape == (M, N), f"gemm_q8: a {tuple(a.shape)}, w {tuple(w.shape)} and out {tuple(out.shape)} do not fit")
+    _f32v(a_scale, "gemm_q8: a_scale", M); _f32v(w_scale, "gemm_q8: w_scale", N); _i32(status, "status")
+    od = _dt(out)
+    if M == 0 or N == 0:
+        return
+    _need(K > 0, "gemm_q8: rows without entries")
+    f = _fn("gemm_quant", "si_gemm_quant_q8", [_c_p, _c_ll, _c_p, _c_p, _c_ll, _c_p, _c_p, _c_ll, _c_int, _c_int, _c_int, _c_int, _c_p])
+    _check(f(_ptr(a), _ld(a), _ptr(a_scale), _ptr(w), _ld(w), _ptr(w_scale), _ptr(out), _ld(out), od, M, N, K, _stream()),
+           f"gemm_q8(M={M}, N={N}, K={K})")
+
+
+def gemm_w4(x, w, scales, zeros, group: int, out, status=None) -> None:
+    """out[m, n] = sum_k x[m, k] * scales[n, k / group] * (q[n, k] - zeros[n, k / group]) with weights of four bits: x bf16 [M, K] (rows
+    contiguous, K a multiple of 8), ``w`` int32 [N, K / 8], entry i of the eight in a word at bit ``W4_SHIFTS[i]`` (see ``pack_w4``); scales bf16
+    [N, ceil(K / group)], zeros uint8 like them or None (8 everywhere), ``group`` 32, 64 or a multiple of 128; out bf16 or fp32 [M, N]; sums fp32.
+    ``status``: as in ``gemm_q8``."""
+    _here("gemm_w4", x, w, scales, zeros, out, status)
+    _need(x.dtype == torch.bfloat16 and w.dtype == torch.int32, "gemm_w4: x must be bfloat16, w int32 words of eight entries")
+    _rows_of(x, "gemm_w4: x"); _rows_of(w, "gemm_w4: w"); _out_rows(out, "gemm_w4: out")
+    M, K = x.shape
+    N = w.shape[0]
+    group = int(group)
+    _need(K % 8 == 0 and w.shape[1] * 8 == K and out.shape == (M, N),
+          f"gemm_w4: x {tuple(x.shape)}, w {tuple(w.shape)} (words of eight) and out {tuple(out.shape)} do not fit")
+    _need(group in (32, 64) or (group > 0 and group % 128 == 0), f"gemm_w4: group {group} is not 32, 64 or a multiple of 128")
+    G = -(-K // group)
+    _need(scales.dtype == torch.bfloat16 and scales.is_contiguous() and scales.shape == (N, G), f"gemm_w4: scales must be contiguous bfloat16 [{N}, {G}]")
+    _need(zeros is None or (zeros.dtype == torch.uint8 and zeros.is_contiguous() and zeros.shape == (N, G)),
+          f"gemm_w4: zeros must be contiguous uint8 [{N}, {G}]")
+    _i32(status, "status")
+    od = _dt(out)
+    if M == 0 or N == 0:
+        return
+    _need(K > 0, "gemm_w4: rows without entries")
+    f = _fn("gemm_quant", "si_gemm_quant_w4", [_c_p, _c_ll, _c_p, _c_ll, _c_p, _c_p, _c_int, _c_p, _c_ll, _c_int, _c_int, _c_int, _c_int, _c_p])
+    _check(f(_ptr(x), _ld(x), _ptr(w), _ld(w), _ptr(scales), _ptr(zeros), group, _ptr(out), _ld(out), od, M, N, K, _stream()),
+           f"gemm_w4(M={M}, N={N}, K={K}, group={group})")
+
+
+def pack_w4(q) -> torch.Tensor:
+    """Entries 0 .. 15 [N, K] (any whole type, K a multiple of 8) -> int32 words [N, K / 8] as ``gemm_w4`` reads them; on q's device, in
+    plain tensor operations (weights are laid out once, at load)."""
+    _need(q.dim() == 2 and q.shape[1] % 8 == 0, "pack_w4: q must be a matrix with a multiple of 8 columns")
+    e = q.reshape(q.shape[0], -1, 8).to(torch.int32)
+    words = torch.zeros(e.shape[:2], dtype=torch.int32, device=q.device)
+    for i, s in enumerate(W4_SHIFTS):
+        words |= (e[:, :, i] & 15) << s
+    return words
+
+
+def unpack_w4(w) -> torch.Tensor:
+    """The entries 0 .. 15 [N, K] (int32) of words that ``pack_w4`` made."""
+    _need(w.dim() == 2 and w.dtype == torch.int32, "unpack_w4: w must be an int32 matrix")
+    return torch.stack([(w >> s) & 15 for s in W4_SHIFTS], 2).reshape(w.shape[0], -1)

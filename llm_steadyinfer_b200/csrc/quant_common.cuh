@@ -1,0 +1,38 @@
+// What the kernels of the 8-bit and 4-bit formats share.
+//
+// 8 bits: a row is e4m3 codes and one fp32 scale, value = code * scale, scale = max(max |x|, 2^-100) / 448, so that the row's largest
+// entry becomes e4m3's largest value. The lower bound keeps an all-zero row (and one of nothing but entries too small to matter) away
+// from a division by zero; its codes are zeros or tiny. A code is rounded to nearest (ties to even): off by at most 2^-4 of its value.
+//
+// 4 bits: entry (n, k) of a matrix is scales[n, k / group] * (q - z), q in 0 .. 15, z = zeros[n, k / group] or 8. Eight entries of a row
+// share an int32 word, entry i of the eight at bit 4 (i / 2) + 16 (i % 2): neighbours lie sixteen bits apart, so that one mask takes a
+// neighbouring pair out of a word into the two halves of a register, where the pairs of 16-bit types live.
+#pragma once
+#include "common.cuh"
+#include <cuda_fp16.h>
+#include <cuda_fp8.h>
+
+#define SI_E4M3_MAX 448.f
+#define SI_Q8_LEAST 7.888609052210118e-31f      // 2^-100
+
+__device__ __forceinline__ float q8_scale(float amax) { return fmaxf(amax, SI_Q8_LEAST) / SI_E4M3_MAX; }
+__device__ __forceinline__ float q8_factor(float amax) { return SI_E4M3_MAX / fmaxf(amax, SI_Q8_LEAST); }
+
+__device__ __forceinline__ unsigned q8_pack2(float a, float b) {      // two codes, a in the low byte
+  return (unsigned)__nv_cvt_float2_to_fp8x2(make_float2(a, b), __NV_SATFINITE, __NV_E4M3);
+}
+__device__ __forceinline__ uint2 q8_pack8(const float (&v)[8]) {
+  return make_uint2(q8_pack2(v[0], v[1]) | (q8_pack2(v[2], v[3]) << 16), q8_pack2(v[4], v[5]) | (q8_pack2(v[6], v[7]) << 16));
+}
+__device__ __forceinline__ unsigned char q8_pack1(float a) { return (unsigned char)__nv_cvt_float_to_fp8(a, __NV_SATFINITE, __NV_E4M3); }
+
+// Pair p (entries 2p, 2p + 1) of a word of eight 4-bit entries as two bf16 of value 128 + q: bf16 counts in ones from 128 to 255, so
+// the four bits go straight into the mantissa.
+__device__ __forceinline__ unsigned w4_pair_raw(unsigned word, int p) { return ((word >> (4 * p)) & 0x000f000fu) | 0x43004300u; }
+// The same less 128 + z, exact: `bias` holds 128 + z twice.
+__device__ __forceinline__ unsigned w4_pair(unsigned word, int p, __nv_bfloat162 bias) {
+  const unsigned raw = w4_pair_raw(word, p);
+  const __nv_bfloat162 v = __hsub2(*reinterpret_cast<const __nv_bfloat162*>(&raw), bias);
+  return *reinterpret_cast<const unsigned*>(&v);
+}
+__device__ __forceinline__ __nv_bfloat162 w4_bias(int z) { return __float2bfloat162_rn(128.f + (float)z); }

@@ -1,0 +1,308 @@
+// Rows to 8 bits with a scale a row, fused with what makes them: the residual add and RMS norm, the gated activation, or nothing.
+//   norm:      h = resid (+ delta (+ delta2));  dst <- h;  y = weight * h * rsqrt(mean(h^2) + eps)
+//   swiglu:    y = silu(gate) * up
+//   quantize:  y = x
+//   scale[r] = max(max_i |y[r, i]|, 2^-100) / 448;   out[r, i] = e4m3(y[r, i] / scale[r])
+// The reference has neither 8-bit type nor these kernels; the bf16 siblings are norm.cu and swiglu.cu.
+//
+// All three are one pass over memory: a block takes a row, every thread keeps its part of it (eight entries a load, up to 32) in
+// registers over the one reduction that the row needs. The norm needs no second one: max |y| = rsqrt(...) * max |weight * h|, so the sum of
+// squares and the maximum are reduced together. Arithmetic is fp32; the only rounding is the one to e4m3. Rows that are not in 16-byte
+// pieces, or wider than 16,384, take a scalar kernel that reads the row twice (the second time from cache).
+// NaN: a NaN entry becomes a NaN code and leaves the maximum to the others (fmaxf); with an infinite entry the factor is zero and the
+// entry itself becomes NaN. The norm of a row with either is NaN where the formula says so.
+#include "quant_common.cuh"
+
+typedef __nv_bfloat16 bf16;
+
+__device__ __forceinline__ void load8(const float* p, float (&v)[8]) {
+  const float4 a = reinterpret_cast<const float4*>(p)[0], b = reinterpret_cast<const float4*>(p)[1];
+  v[0] = a.x; v[1] = a.y; v[2] = a.z; v[3] = a.w; v[4] = b.x; v[5] = b.y; v[6] = b.z; v[7] = b.w;
+}
+__device__ __forceinline__ void load8(const bf16* p, float (&v)[8]) {
+  const uint4 raw = *reinterpret_cast<const uint4*>(p);
+  const __nv_bfloat162* h = reinterpret_cast<const __nv_bfloat162*>(&raw);
+#pragma unroll
+  for (int i = 0; i < 4; ++i) {
+    const float2 f = __bfloat1622float2(h[i]);
+    v[2 * i] = f.x; v[2 * i + 1] = f.y;
+  }
+}
+__device__ __forceinline__ void store8(float* p, const float (&v)[8]) {
+  reinterpret_cast<float4*>(p)[0] = make_float4(v[0], v[1], v[2], v[3]);
+  reinterpret_cast<float4*>(p)[1] = make_float4(v[4], v[5], v[6], v[7]);
+}
+
+// The block's sum of `s` and maximum of `m`, for every thread; `scratch` holds 64 floats. Called once a kernel.
+__device__ __forceinline__ float2 block_sum_max(float s, float m, float* scratch) {
+  const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5, nwarps = blockDim.x >> 5;
+  s = warp_sum(s);
+  m = warp_max(m);
+  if (nwarps == 1) return make_float2(s, m);
+  if (lane == 0) { scratch[warp] = s; scratch[32 + warp] = m; }
+  __syncthreads();
+  s = lane < nwarps ? scratch[lane] : 0.f;               // every warp adds the warps' sums up itself: no second barrier
+  m = lane < nwarps ? scratch[32 + lane] : 0.f;
+  return make_float2(warp_sum(s), warp_max(m));
+}
+
+struct NormArgs {
+  float* resid;                 // [*, width]
+  const void* delta;            // like resid, TX, or null
+  const void* delta2;           // beside delta, or null
+  float* dst;                   // where the stream goes, or null: it stays as it is
+  const int* rows;              // row r is stream row rows[r], or null
+  const void* weight;
+  float eps;
+  const void* ahead;            // what the next kernel streams, fetched into L2 by the blocks behind the rows
+  long long ahead_bytes;
+};
+
+template <typename TX, typename TW, int CHUNKS>
+__global__ void __launch_bounds__(512) norm_q8_kernel(const NormArgs a, unsigned char* __restrict__ out, float* __restrict__ scale,
+                                                      int width, int num_rows, int trigger) {
+  __shared__ float scratch[64];
+  if (trigger) pdl_trigger();
+  if ((int)blockIdx.x >= num_rows) {
+    l2_prefetch_share(a.ahead, a.ahead_bytes, blockIdx.x - num_rows, gridDim.x - num_rows);
+    return;
+  }
+  const TW* weight = (const TW*)a.weight;
+  const int nchunks = width >> 3;
+  if (trigger) {
+#pragma unroll
+    for (int c = 0; c < CHUNKS; ++c) {
+      const int ch = threadIdx.x + c * blockDim.x;
+      if (ch < nchunks) prefetch_l1(weight + ch * 8);
+    }
+  }
+  pdl_wait();
+  const int r = blockIdx.x;
+  const size_t src = (size_t)(a.rows ? a.rows[r] : r) * width;
+  const TX* d1 = (const TX*)a.delta;
+  const TX* d2 = (const TX*)a.delta2;
+  float x[CHUNKS][8], e1[CHUNKS][8], e2[CHUNKS][8];
+#pragma unroll
+  for (int c = 0; c < CHUNKS; ++c) {
+    const int ch = threadIdx.x + c * blockDim.x;
+    if (ch < nchunks) {
+      load8(a.resid + src + ch * 8, x[c]);
+      if (d1) load8(d1 + src + ch * 8, e1[c]);
+      if (d2) load8(d2 + src + ch * 8, e2[c]);
+    }
+  }
+  float ss = 0.f, top = 0.f;
+#pragma unroll
+  for (int c = 0; c < CHUNKS; ++c) {
+    const int ch = threadIdx.x + c * blockDim.x;
+    if (ch < nchunks) {
+#pragma unroll
+      for (int i = 0; i < 8; ++i) {
+        if (d1) x[c][i] += e1[c][i];
+        if (d2) x[c][i] += e2[c][i];
+      }
+      if (a.dst) store8(a.dst + src + ch * 8, x[c]);
+      float w[8];
+      load8(weight + ch * 8, w);
+#pragma unroll
+      for (int i = 0; i < 8; ++i) {
+        ss += x[c][i] * x[c][i];
+        x[c][i] *= w[i];
+        top = fmaxf(top, fabsf(x[c][i]));
+      }
+    }
+  }
+  const float2 both = block_sum_max(ss, top, scratch);
+  const float inv = rsqrtf(both.x / (float)width + a.eps);
+  const float amax = both.y * inv, f = q8_factor(amax);          // applied after inv: their product may pass fp32's range
+  if (threadIdx.x == 0) scale[r] = q8_scale(amax);
+  unsigned char* o = out + (size_t)r * width;
+#pragma unroll
+  for (int c = 0; c < CHUNKS; ++c) {
+    const int ch = threadIdx.x + c * blockDim.x;
+    if (ch < nchunks) {
+#pragma unroll
+      for (int i = 0; i < 8; ++i) x[c][i] = x[c][i] * inv * f;
+      *reinterpret_cast<uint2*>(o + ch * 8) = q8_pack8(x[c]);
+    }
+  }
+}
+
+template <typename TX, typename TW>
+__global__ void norm_q8_scalar_kernel(const NormArgs a, unsigned char* __restrict__ out, float* __restrict__ scale, int width) {
+  __shared__ float scratch[64];
+  pdl_wait();
+  const int r = blockIdx.x;
+  const size_t src = (size_t)(a.rows ? a.rows[r] : r) * width;
+  const TX* d1 = (const TX*)a.delta;
+  const TX* d2 = (const TX*)a.delta2;
+  const TW* weight = (const TW*)a.weight;
+  auto entry = [&](int i) {
+    float h = a.resid[src + i];
+    if (d1) h += to_f32<TX>(d1[src + i]);
+    if (d2) h += to_f32<TX>(d2[src + i]);
+    return h;
+  };
+  float ss = 0.f, top = 0.f;
+  for (int i = threadIdx.x; i < width; i += blockDim.x) {
+    const float h = entry(i);
+    if (a.dst) a.dst[src + i] = h;
+    ss += h * h;
+    top = fmaxf(top, fabsf(h * to_f32<TW>(weight[i])));
+  }
+  const float2 both = block_sum_max(ss, top, scratch);
+  const float inv = rsqrtf(both.x / (float)width + a.eps);
+  const float amax = both.y * inv, f = q8_factor(amax);
+  if (threadIdx.x == 0) scale[r] = q8_scale(amax);
+  for (int i = threadIdx.x; i < width; i += blockDim.x) {            // what this thread stored itself, where the stream was written
+    const float h = a.dst ? a.dst[src + i] : entry(i);
+    out[(size_t)r * width + i] = q8_pack1(h * to_f32<TW>(weight[i]) * inv * f);
+  }
+}
+
+// GATED: the row's entries are silu(gate) * up of the stacked row, gate f in column (f / group) * 2 * group + f % group.
+template <typename TX, bool GATED, int CHUNKS>
+__global__ void __launch_bounds__(512) rows_q8_kernel(const TX* __restrict__ x, long long ldx, unsigned char* __restrict__ out,
+                                                      float* __restrict__ scale, int width, int group, int trigger) {
+  __shared__ float scratch[64];
+  if (trigger) pdl_trigger();
+  pdl_wait();
+  const int r = blockIdx.x, nchunks = width >> 3;
+  const TX* row = x + (size_t)r * ldx;
+  float v[CHUNKS][8], u[CHUNKS][8];
+#pragma unroll
+  for (int c = 0; c < CHUNKS; ++c) {
+    const int ch = threadIdx.x + c * blockDim.x;
+    if (ch < nchunks) {
+      if (GATED) {
+        const int f = ch * 8, at = f / group * group + f;            // (f / group) * 2 * group + f % group
+        load8(row + at, v[c]);
+        load8(row + at + group, u[c]);
+      } else {
+        load8(row + ch * 8, v[c]);
+      }
+    }
+  }
+  float top = 0.f;
+#pragma unroll
+  for (int c = 0; c < CHUNKS; ++c)
+    if ((int)(threadIdx.x + c * blockDim.x) < nchunks) {
+#pragma unroll
+      for (int i = 0; i < 8; ++i) {
+        if (GATED) v[c][i] = silu_mul(v[c][i], u[c][i]);
+        top = fmaxf(top, fabsf(v[c][i]));
+      }
+    }
+  top = block_sum_max(0.f, top, scratch).y;
+  const float f = q8_factor(top);
+  if (threadIdx.x == 0) scale[r] = q8_scale(top);
+#pragma unroll
+  for (int c = 0; c < CHUNKS; ++c) {
+    const int ch = threadIdx.x + c * blockDim.x;
+    if (ch < nchunks) {
+#pragma unroll
+      for (int i = 0; i < 8; ++i) v[c][i] *= f;
+      *reinterpret_cast<uint2*>(out + (size_t)r * width + ch * 8) = q8_pack8(v[c]);
+    }
+  }
+}
+
+template <typename TX, bool GATED>
+__global__ void rows_q8_scalar_kernel(const TX* __restrict__ x, long long ldx, unsigned char* __restrict__ out,
+                                      float* __restrict__ scale, int width, int group) {
+  __shared__ float scratch[64];
+  pdl_wait();
+  const TX* row = x + (size_t)blockIdx.x * ldx;
+  auto entry = [&](int i) {
+    if (!GATED) return to_f32<TX>(row[i]);
+    const int at = i / group * group + i;
+    return silu_mul(to_f32<TX>(row[at]), to_f32<TX>(row[at + group]));
+  };
+  float top = 0.f;
+  for (int i = threadIdx.x; i < width; i += blockDim.x) top = fmaxf(top, fabsf(entry(i)));
+  top = block_sum_max(0.f, top, scratch).y;
+  const float f = q8_factor(top);
+  if (threadIdx.x == 0) scale[blockIdx.x] = q8_scale(top);
+  for (int i = threadIdx.x; i < width; i += blockDim.x) out[(size_t)blockIdx.x * width + i] = q8_pack1(entry(i) * f);
+}
+
+#define Q8_MAX_VEC_WIDTH (4 * 8 * 512)
+// Threads of a row's block: what covers it in one load each, up to 512; then two or four loads each.
+static int row_threads(int width) {
+  const int chunks = (width + 7) / 8;
+  return chunks >= 512 ? 512 : (chunks + 31) / 32 * 32;
+}
+
+template <typename TX, typename TW>
+static void launch_norm(const NormArgs& a, unsigned char* out, float* scale, int width, int num_rows, bool vec, cudaStream_t stream) {
+  const dim3 block(row_threads(width));
+  if (!vec) {
+    si_launch(norm_q8_scalar_kernel<TX, TW>, dim3(num_rows), block, 0, stream, a, out, scale, width);
+    return;
+  }
+  const int per = (width / 8 + block.x - 1) / block.x, sms = si_sm_count();
+  const int trigger = si_pdl_trigger_enabled() && num_rows <= 64;
+  const int extra = a.ahead ? (num_rows < sms ? 2 * sms - num_rows : sms) : 0;
+  const dim3 grid(num_rows + extra);
+#define NORM_Q8(C) si_launch(norm_q8_kernel<TX, TW, C>, grid, block, 0, stream, a, out, scale, width, num_rows, trigger)
+  if (per <= 1) NORM_Q8(1); else if (per <= 2) NORM_Q8(2); else NORM_Q8(4);
+#undef NORM_Q8
+}
+
+// resid [*, width] fp32; delta, delta2 (may be null) like it in x_dtype; weight [width] in w_dtype; dst (may be null, may be resid);
+// out [num_rows, width] e4m3, scale [num_rows] fp32. Returns 0, a CUDA error code, or -2 (size refused).
+SI_EXPORT int si_add_rmsnorm_q8(float* resid, const void* delta, const void* delta2, int x_dtype, const int* rows, const void* weight,
+                                int w_dtype, float* dst, void* out, float* scale, int num_rows, int width, float eps, const void* ahead,
+                                long long ahead_bytes, cudaStream_t stream) {
+  if (num_rows <= 0) return 0;
+  if (width <= 0 || (delta2 && !delta)) return -2;
+  NormArgs a;
+  a.resid = resid; a.delta = delta; a.delta2 = delta2; a.dst = dst; a.rows = rows; a.weight = weight; a.eps = eps;
+  a.ahead = ahead_bytes >= 4096 ? ahead : nullptr; a.ahead_bytes = ahead_bytes;
+  const bool vec = width % 8 == 0 && width <= Q8_MAX_VEC_WIDTH &&
+                   (((uintptr_t)resid | (uintptr_t)delta | (uintptr_t)delta2 | (uintptr_t)dst | (uintptr_t)weight) % 16 == 0) && (uintptr_t)out % 8 == 0;
+  unsigned char* o = (unsigned char*)out;
+  if (x_dtype == SI_BF16) {
+    if (w_dtype == SI_BF16) launch_norm<bf16, bf16>(a, o, scale, width, num_rows, vec, stream);
+    else launch_norm<bf16, float>(a, o, scale, width, num_rows, vec, stream);
+  } else {
+    if (w_dtype == SI_BF16) launch_norm<float, bf16>(a, o, scale, width, num_rows, vec, stream);
+    else launch_norm<float, float>(a, o, scale, width, num_rows, vec, stream);
+  }
+  return si_last_error();
+}
+
+template <typename TX, bool GATED>
+static void launch_rows(const void* x, long long ldx, void* out, float* scale, int num_rows, int width, int group, cudaStream_t stream) {
+  const dim3 grid(num_rows), block(row_threads(width));
+  const TX* xp = (const TX*)x;
+  unsigned char* o = (unsigned char*)out;
+  const bool vec = width % 8 == 0 && width <= Q8_MAX_VEC_WIDTH && (!GATED || group % 8 == 0) && ldx % (16 / (int)sizeof(TX)) == 0 &&
+                   (uintptr_t)x % 16 == 0 && (uintptr_t)out % 8 == 0;
+  if (!vec) {
+    si_launch(rows_q8_scalar_kernel<TX, GATED>, grid, block, 0, stream, xp, ldx, o, scale, width, group);
+    return;
+  }
+  const int per = (width / 8 + block.x - 1) / block.x, trigger = si_pdl_trigger_small(num_rows);
+#define ROWS_Q8(C) si_launch(rows_q8_kernel<TX, GATED, C>, grid, block, 0, stream, xp, ldx, o, scale, width, group, trigger)
+  if (per <= 1) ROWS_Q8(1); else if (per <= 2) ROWS_Q8(2); else ROWS_Q8(4);
+#undef ROWS_Q8
+}
+
+// x [num_rows, width], rows `ldx` entries apart -> out [num_rows, width] e4m3, scale [num_rows].
+SI_EXPORT int si_quantize_q8(const void* x, int dtype, long long ldx, void* out, float* scale, int num_rows, int width, cudaStream_t stream) {
+  if (num_rows <= 0) return 0;
+  if (width <= 0) return -2;
+  if (dtype == SI_BF16) launch_rows<bf16, false>(x, ldx, out, scale, num_rows, width, 1, stream);
+  else launch_rows<float, false>(x, ldx, out, scale, num_rows, width, 1, stream);
+  return si_last_error();
+}
+
+// gu [num_rows, 2 * inter], rows one behind the other, gates and ups interleaved in groups of `group` columns -> out [num_rows, inter].
+SI_EXPORT int si_swiglu_q8(const void* gu, int dtype, void* out, float* scale, int num_rows, int inter, int group, cudaStream_t stream) {
+  if (num_rows <= 0) return 0;
+  if (inter <= 0 || group <= 0 || inter % group || inter > 0x3fffffff) return -2;
+  if (dtype == SI_BF16) launch_rows<bf16, true>(gu, 2LL * inter, out, scale, num_rows, inter, group, stream);
+  else launch_rows<float, true>(gu, 2LL * inter, out, scale, num_rows, inter, group, stream);
+  return si_last_error();
+}

@@ -1,0 +1,426 @@
+"""The operators of the 8-bit and 4-bit formats against their definitions in 64 bits.
+
+Products are tested twice. With whole entries and scales that are powers of two every partial sum is exact in fp32, so the result must be the
+exact one, to the last bit (rounded once where the output is bf16): a wrong entry anywhere shows. With real entries the bound counts every
+rounding: each of the K additions of a sum is off by at most 2^-23 of the sum of the products' sizes (an fp32 addition rounds by 2^-24; the
+tensor cores may cut instead of rounding, which is twice that), and the output's rounding comes on top.
+"""
+import pytest
+import torch
+
+pytestmark = pytest.mark.gpu
+DEV = "cuda:0"
+E4M3 = torch.float8_e4m3fn
+BF16, F32, F64 = torch.bfloat16, torch.float32, torch.float64
+
+
+def ops():
+    from llm_steadyinfer_b200.csrc import ops as o
+    return o
+
+
+def gen(seed):
+    return torch.Generator(device=DEV).manual_seed(seed)
+
+
+def status_word():
+    return torch.zeros(1, dtype=torch.int32, device=DEV)
+
+
+# ---- rows to 8 bits ----------------------------------------------------------------------------------------------
+
+def check_rows(out, scale, y, scale_tol):
+    """``y``: the exact rows (fp64). The scale is off by ``scale_tol`` at most; a code by half a step of e4m3 (2^-4 of its value, 2^-10 below
+    the least normal one) and by what the entry and the scale are off by before they are rounded."""
+    want = y.abs().amax(1).clamp_min(2.0 ** -100) / 448
+    assert ((scale.double() - want).abs() <= scale_tol * want).all()
+    v = y / scale.double().unsqueeze(1)
+    off = (out.float().double() - v).abs()
+    assert (off <= torch.maximum(v.abs() * 2.0 ** -4, torch.tensor(2.0 ** -10, dtype=F64, device=DEV)) + 2 * scale_tol * v.abs()).all()
+
+
+def norm_exact(resid, deltas, weight, eps, rows=None):
+    h = resid.double()
+    for d in deltas:
+        h = h + d.double()
+    if rows is not None:
+        h = h[rows.long()]
+    return h, weight.double() * h / torch.sqrt((h * h).mean(1, keepdim=True) + eps)
+
+
+# width 1,336 has whole chunks of eight; 1,001 and 5 have not; 16,392 is wider than what a block holds in registers
+@pytest.mark.parametrize("xdtype,wdtype", [(BF16, BF16), (BF16, F32), (F32, F32), (F32, BF16)])
+@pytest.mark.parametrize("R,d", [(1, 4096), (3, 1336), (70, 1001), (2, 5), (1, 1), (300, 2048), (2, 16384), (2, 16392)])
+def test_add_rmsnorm_q8(xdtype, wdtype, R, d):
+    g = gen(R * d)
+    resid = torch.randn(R, d, generator=g, device=DEV) * 3
+    delta, delta2 = (torch.randn(R, d, generator=g, device=DEV).to(xdtype) for _ in range(2))
+    weight = (1 + 0.2 * torch.randn(d, generator=g, device=DEV)).to(wdtype)
+    # the sum of squares: at most 64 additions in a row (entries a thread, then threads), each off by 2^-24; the stream's own two roundings count twice in
+    # a square; the root halves all of that; then the root itself, two products, the quotient and the scale: below 64 * 2^-24 together
+    tol = 2.0 ** -18
+    for deltas in ((), (delta,), (delta, delta2)):
+        h, y = norm_exact(resid, deltas, weight, 1e-5)
+        kw = {"delta2": deltas[1]} if len(deltas) == 2 else {}
+        out, scale = torch.empty(R, d, dtype=E4M3, device=DEV), torch.full((R,), -1.0, device=DEV)
+        stream, dst = resid.clone(), torch.full_like(resid, 7.0)
+        ops().add_rmsnorm_q8(stream, deltas[0] if deltas else None, weight, 1e-5, out, scale, dst=dst, **kw)
+        assert torch.equal(stream, resid)
+        check_rows(out, scale, y, tol)
+        # each of the two additions rounds once
+        assert ((dst.double() - h).abs() <= 2 * 2.0 ** -24 * (resid.double().abs() + sum(t.double().abs() for t in deltas))).all()
+        out2, scale2 = torch.empty_like(out), torch.empty_like(scale)
+        ops().add_rmsnorm_q8(stream, deltas[0] if deltas else None, weight, 1e-5, out2, scale2, **kw)          # in place: the same, and the stream moves on
+        assert torch.equal(stream, dst if deltas else resid) and torch.equal(out2.view(torch.uint8), out.view(torch.uint8)) and torch.equal(scale2, scale)
+
+
+@pytest.mark.parametrize("d", [512, 513])
+def test_add_rmsnorm_q8_of_chosen_rows(d):
+    g = gen(5)
+    resid, delta = torch.randn(9, d, generator=g, device=DEV), torch.randn(9, d, generator=g, device=DEV).to(BF16)
+    weight = torch.ones(d, device=DEV)
+    rows = torch.tensor([8, 0, 0, 3], dtype=torch.int32, device=DEV)                     # out of order, one of them twice
+    out, scale = torch.empty(4, d, dtype=E4M3, device=DEV), torch.empty(4, device=DEV)
+    before = resid.clone()
+    ops().add_rmsnorm_q8(resid, delta, weight, 1e-5, out, scale, rows=rows)
+    assert torch.equal(resid, before)
+    check_rows(out, scale, norm_exact(resid, (delta,), weight, 1e-5, rows)[1], 2.0 ** -18)
+    ahead = torch.zeros(1 << 20, device=DEV)
+    out2, scale2 = torch.empty_like(out), torch.empty_like(scale)
+    ops().add_rmsnorm_q8(resid, delta, weight, 1e-5, out2, scale2, rows=rows, ahead=ahead)
+    assert torch.equal(out2.view(torch.uint8), out.view(torch.uint8)) and torch.equal(scale2, scale)
+
+
+@pytest.mark.parametrize("dtype", [BF16, F32])
+@pytest.mark.parametrize("R,F,group", [(1, 8192, 8), (5, 1336, 8), (3, 1336, None), (4, 90, 9), (2, 7, 1), (1, 1, None), (200, 2816, 8), (2, 14336, 8),
+                                       (2, 16392, 8), (3, 24, 12)])
+def test_swiglu_q8(dtype, R, F, group):
+    gu = (torch.randn(R, 2 * F, generator=gen(F), device=DEV) * 3).to(dtype)
+    out, scale = torch.empty(R, F, dtype=E4M3, device=DEV), torch.empty(R, device=DEV)
+    ops().swiglu_q8(gu, out, scale, group)
+    f, n = torch.arange(F, device=DEV), group or F
+    at = f // n * 2 * n + f % n
+    gate, up = gu[:, at].double(), gu[:, at + n].double()
+    # expf is off by 2^-22 at most (two units), the sum, the quotient and the product by 2^-24 each (the quotient by two units): below 2^-20
+    check_rows(out, scale, gate / (1 + torch.exp(-gate)) * up, 2.0 ** -20)
+
+
+@pytest.mark.parametrize("dtype", [BF16, F32])
+@pytest.mark.parametrize("R,n,stride", [(1, 4096, 4096), (61, 4096, 6144), (7, 1001, 1001), (3, 1000, 1003), (2, 1, 5), (700, 64, 72), (2, 16384, 16384),
+                                        (3, 20000, 20000)])
+def test_quantize_q8(dtype, R, n, stride):
+    x = (torch.randn(R, stride, generator=gen(n), device=DEV) * 5).to(dtype)[:, :n]
+    out, scale = torch.empty(R, n, dtype=E4M3, device=DEV), torch.empty(R, device=DEV)
+    ops().quantize_q8(x, out, scale)
+    check_rows(out, scale, x.double(), 2.0 ** -22)            # a quotient and a product
+    shifted = torch.empty(R * stride + 1, dtype=dtype, device=DEV)[1:].view(R, stride)[:, :n]      # a base that is not on a 16-byte boundary
+    shifted.copy_(x)
+    out2, scale2 = torch.empty_like(out), torch.empty_like(scale)
+    ops().quantize_q8(shifted, out2, scale2)
+    assert torch.equal(out2.view(torch.uint8), out.view(torch.uint8)) and torch.equal(scale2, scale)
+
+
+@pytest.mark.parametrize("n", [512, 515])
+def test_rows_of_zeros_infinities_and_nan(n):
+    """A row of zeros has zero codes and a finite scale; entries that are NaN become NaN codes and leave the others alone; with an infinite entry
+    the scale is infinite, the entry NaN and the others zero."""
+    x = torch.randn(5, n, generator=gen(1), device=DEV)
+    x[0] = 0
+    x[1, 3] = float("nan")
+    x[2, n - 1] = float("inf")
+    x[3] *= 1e-38
+    x[3, 5] = 3e38
+    out, scale = torch.empty(5, n, dtype=E4M3, device=DEV), torch.empty(5, device=DEV)
+    ops().quantize_q8(x, out, scale)
+    v = out.float()
+    assert (v[0] == 0).all() and scale[0].item() > 0
+    assert torch.isnan(v[1]).sum() == 1 and torch.isnan(v[1, 3])
+    ok = torch.arange(n, device=DEV) != 3
+    check_rows(out[1:2, ok], scale[1:2], x[1:2, ok].double(), 2.0 ** -22)
+    assert torch.isinf(scale[2]) and torch.isnan(v[2, n - 1]) and (v[2, :n - 1] == 0).all()
+    check_rows(out[3:], scale[3:], x[3:].double(), 2.0 ** -22)
+    # the norm of a row of zeros, without and with an eps that keeps its root finite
+    resid, w = torch.zeros(2, n, device=DEV), torch.ones(n, device=DEV)
+    ops().add_rmsnorm_q8(resid, None, w, 1e-30, out[:2], scale[:2])
+    assert (out[:2].float() == 0).all() and torch.isfinite(scale[:2]).all()
+
+
+def test_rows_of_no_rows():
+    out, scale = torch.empty(0, 64, dtype=E4M3, device=DEV), torch.empty(0, device=DEV)
+    ops().quantize_q8(torch.empty(0, 64, device=DEV), out, scale)
+    ops().swiglu_q8(torch.empty(0, 128, device=DEV), out, scale)
+    ops().add_rmsnorm_q8(torch.empty(0, 64, device=DEV), None, torch.ones(64, device=DEV), 1e-5, out, scale)
+
+
+# ---- products of 8-bit rows and weights --------------------------------------------------------------------------
+
+def whole_codes(g, R, n):
+    """Entries -8 .. 8, all of them e4m3 values: products up to 64, sums of up to 8,192 of them below 2^24."""
+    return torch.randint(-8, 9, (R, n), generator=g, device=DEV).float().to(E4M3)
+
+
+def powers(g, n):
+    return torch.exp2(torch.randint(-6, 7, (n,), generator=g, device=DEV).float())
+
+
+ROWS = [1, 3, 8, 9, 16, 17, 40, 64, 127, 128, 129, 200, 257, 513]
+
+
+@pytest.mark.parametrize("M", ROWS)
+@pytest.mark.parametrize("N,K", [(256, 512), (1000, 1024), (8, 16), (33, 128), (130, 2816), (1, 8), (17, 5), (64, 136), (2048, 144), (384, 4112)])
+def test_gemm_q8_whole_entries(M, N, K):
+    g = gen(M * 7 + N + K)
+    a, w, sa, sw = whole_codes(g, M, K), whole_codes(g, N, K), powers(g, M), powers(g, N)
+    want = torch.mm(a.double(), w.double().t()) * sa.double().unsqueeze(1) * sw.double()
+    for dtype in (BF16, F32):
+        out, status = torch.full((M, N), float("nan"), dtype=dtype, device=DEV), status_word()
+        ops().gemm_q8(a, sa, w, sw, out, status)
+        assert status.item() == 0
+        assert torch.equal(out, want.to(F32).to(dtype))          # the sum is exact in fp32, the scales only move its exponent
+
+
+@pytest.mark.parametrize("M,N,K", [(1, 4096, 4096), (8, 2048, 5632), (16, 6144, 4096), (61, 4096, 14336), (128, 1000, 2048), (300, 1336, 2816), (600, 2048, 1000)])
+def test_gemm_q8_real_entries(M, N, K):
+    g = gen(K)
+    a, w = torch.empty(M, K, dtype=E4M3, device=DEV), torch.empty(N, K, dtype=E4M3, device=DEV)
+    sa, sw = torch.empty(M, device=DEV), torch.empty(N, device=DEV)
+    ops().quantize_q8(torch.randn(M, K, generator=g, device=DEV), a, sa)
+    ops().quantize_q8(torch.randn(N, K, generator=g, device=DEV) * 0.02, w, sw)
+    scales = sa.double().unsqueeze(1) * sw.double()
+    want = torch.mm(a.double(), w.double().t()) * scales
+    bound = (K + 2) * 2.0 ** -23 * torch.mm(a.double().abs(), w.double().abs().t()) * scales
+    for dtype in (BF16, F32):
+        out, status = torch.empty(M, N, dtype=dtype, device=DEV), status_word()
+        ops().gemm_q8(a, sa, w, sw, out, status)
+        assert status.item() == 0
+        off = (out.double() - want).abs()
+        assert (off <= bound + (2.0 ** -8 * want.abs() if dtype == BF16 else 0)).all()
+        # The bound takes every partial sum as large as all products' sizes together. For entries of random sign a partial sum is about their root
+        # of the sum of squares, sqrt(K) where the sizes add up to 0.64 K: K roundings of 2^-24 of it add up to some 2^-23 of the sizes, and
+        # cuts (all to one side) of 2^-23 every 32 entries to sqrt(K) / 20 * 2^-23, below 6 * 2^-23 here. 2^-20 of the sizes leaves room, and a kernel
+        # that sums in fewer than 32 bits would not keep to it.
+        assert (off <= 2.0 ** -20 * bound / ((K + 2) * 2.0 ** -23) + (2.0 ** -8 * want.abs() if dtype == BF16 else 0)).all()
+
+
+@pytest.mark.parametrize("M", [1, 5, 16, 40, 128, 300])
+@pytest.mark.parametrize("K,lda,ldw,shift", [(256, 272, 288, 0), (256, 264, 257, 0), (256, 256, 256, 3), (256, 320, 256, 16)])
+def test_gemm_q8_strides_and_alignment(M, K, lda, ldw, shift):
+    g = gen(M + lda)
+    N = 200
+
+    def laid(rows, ld):
+        buf = torch.full((rows * ld + shift,), float("nan"), device=DEV).to(E4M3)          # what lies between the rows is never read into a sum
+        t = buf[shift:].view(rows, ld)[:, :K]
+        t.copy_(whole_codes(g, rows, K))
+        return t
+
+    a, w, sa, sw = laid(M, lda), laid(N, ldw), powers(g, M), powers(g, N)
+    want = (torch.mm(a.double(), w.double().t()) * sa.double().unsqueeze(1) * sw.double()).to(F32)
+    for dtype, ldo in ((BF16, 200), (BF16, 203), (F32, 208)):
+        buf = torch.full((M, ldo), 77.0, dtype=dtype, device=DEV)
+        status = status_word()
+        ops().gemm_q8(a, sa, w, sw, buf[:, :N], status)
+        assert status.item() == 0 and torch.equal(buf[:, :N], want.to(dtype)) and (buf[:, N:] == 77).all()
+
+
+@pytest.mark.parametrize("M", [2, 40, 200])
+def test_gemm_q8_nan_stays_in_its_row_and_column(M):
+    g = gen(M)
+    N, K = 160, 256
+    a, w, sa, sw = whole_codes(g, M, K), whole_codes(g, N, K), powers(g, M), powers(g, N)
+    want = torch.mm(a.double(), w.double().t()) * sa.double().unsqueeze(1) * sw.double()
+    a[1, 7] = float("nan")
+    w[33, 250] = float("nan")
+    out = torch.empty(M, N, device=DEV)
+    ops().gemm_q8(a, sa, w, sw, out, status_word())
+    want[1] = float("nan")
+    want[:, 33] = float("nan")
+    assert torch.equal(torch.nan_to_num(out, nan=-1e9), torch.nan_to_num(want.to(F32), nan=-1e9))
+
+
+# ---- products with 4-bit weights ---------------------------------------------------------------------------------
+
+def w4_weight(g, N, K, group, zeros, whole=True):
+    """(words, scales, zeros or None, the weight in fp64). ``whole``: scales are powers of two."""
+    G = -(-K // group)
+    q = torch.randint(0, 16, (N, K), generator=g, device=DEV)
+    z = torch.randint(0, 16, (N, G), generator=g, device=DEV).to(torch.uint8) if zeros else None
+    if whole:
+        s = torch.exp2(torch.randint(-1, 2, (N, G), generator=g, device=DEV).float()).to(BF16)
+    else:
+        s = (0.002 + 0.01 * torch.rand(N, G, generator=g, device=DEV)).to(BF16)
+    at = torch.arange(K, device=DEV) // group
+    w = (q.double() - (z.double()[:, at] if zeros else 8.0)) * s.double()[:, at]
+    return ops().pack_w4(q), s, z, w
+
+
+@pytest.mark.parametrize("M", ROWS)
+@pytest.mark.parametrize("N,K,group,zeros", [(256, 512, 128, False), (1000, 1024, 128, True), (16, 64, 32, True), (33, 136, 32, False), (130, 2816, 64, True),
+                                             (1, 8, 128, False), (64, 200, 64, False), (2048, 384, 256, True), (384, 4104, 128, False), (48, 520, 1024, True)])
+def test_gemm_w4_whole_entries(M, N, K, group, zeros):
+    """Entries of x -4 .. 4, weights up to 30 in halves: every sum is a multiple of a half, below 2^23."""
+    g = gen(M * 3 + N + K)
+    words, s, z, w = w4_weight(g, N, K, group, zeros)
+    x = torch.randint(-4, 5, (M, K), generator=g, device=DEV).to(BF16)
+    want = torch.mm(x.double(), w.t()).to(F32)
+    for dtype in (BF16, F32):
+        out, status = torch.full((M, N), float("nan"), dtype=dtype, device=DEV), status_word()
+        ops().gemm_w4(x, words, s, z, group, out, status)
+        assert status.item() == 0
+        assert torch.equal(out, want.to(dtype))
+
+
+@pytest.mark.parametrize("M,N,K,group,zeros", [(1, 4096, 4096, 128, False), (8, 2048, 5632, 64, True), (16, 6144, 4096, 128, True), (61, 4096, 14336, 128, False),
+                                               (128, 1000, 2048, 32, True), (300, 1336, 2816, 128, True), (600, 2048, 1000, 256, False)])
+def test_gemm_w4_real_entries(M, N, K, group, zeros):
+    g = gen(K)
+    words, s, z, w = w4_weight(g, N, K, group, zeros, whole=False)
+    x = torch.randn(M, K, generator=g, device=DEV).to(BF16)
+    want, sizes = torch.mm(x.double(), w.t()), torch.mm(x.double().abs(), w.abs().t())
+    for dtype in (BF16, F32):
+        out, status = torch.empty(M, N, dtype=dtype, device=DEV), status_word()
+        ops().gemm_w4(x, words, s, z, group, out, status)
+        assert status.item() == 0
+        # many rows round each weight to bf16 once (2^-8 of it); the sums as for 8 bits
+        assert ((out.double() - want).abs() <= (2.0 ** -8 + (K + 2) * 2.0 ** -23) * sizes + (2.0 ** -8 * want.abs() if dtype == BF16 else 0)).all()
+        # the roundings of the weights are independent: of K entries their sum is far below K times one (six standard deviations of the sum of
+        # K roundings spread over +- 2^-8 of each product)
+        spread = 6 * 2.0 ** -8 / 3 ** 0.5 * torch.sqrt(torch.mm(x.double() ** 2, (w ** 2).t()))
+        assert ((out.double() - want).abs() <= spread + (K + 2) * 2.0 ** -23 * sizes + (2.0 ** -8 * want.abs() if dtype == BF16 else 0)).all()
+
+
+@pytest.mark.parametrize("M", [1, 5, 16, 40, 128, 300])
+@pytest.mark.parametrize("ldx,ldw,shift", [(264, 36, 0), (257, 33, 0), (256, 32, 1), (272, 64, 8)])
+def test_gemm_w4_strides_and_alignment(M, ldx, ldw, shift):
+    g = gen(M + ldx)
+    N, K, group = 200, 256, 64
+    words, s, z, w = w4_weight(g, N, K, group, True)
+    wbuf = torch.full((N * ldw + shift,), -1, dtype=torch.int32, device=DEV)
+    wv = wbuf[shift:].view(N, ldw)[:, :K // 8]
+    wv.copy_(words)
+    xbuf = torch.full((M * ldx + shift,), float("nan"), dtype=BF16, device=DEV)
+    x = xbuf[shift:].view(M, ldx)[:, :K]
+    x.copy_(torch.randint(-4, 5, (M, K), generator=g, device=DEV).to(BF16))
+    want = torch.mm(x.double(), w.t()).to(F32)
+    for dtype, ldo in ((BF16, 200), (BF16, 203), (F32, 208)):
+        buf = torch.full((M, ldo), 77.0, dtype=dtype, device=DEV)
+        status = status_word()
+        ops().gemm_w4(x, wv, s, z, group, buf[:, :N], status)
+        assert status.item() == 0 and torch.equal(buf[:, :N], want.to(dtype)) and (buf[:, N:] == 77).all()
+
+
+@pytest.mark.parametrize("M", [2, 40, 200])
+def test_gemm_w4_nan_stays_in_its_row_and_column(M):
+    g = gen(M)
+    N, K, group = 160, 264, 64
+    words, s, z, w = w4_weight(g, N, K, group, False)
+    x = torch.randint(-4, 5, (M, K), generator=g, device=DEV).to(BF16)
+    want = torch.mm(x.double(), w.t()).to(F32)
+    x[1, 263] = float("nan")
+    s[33, 4] = float("inf")                                     # the last group, of which the row holds eight entries
+    want[1] = float("nan")
+    out = torch.empty(M, N, device=DEV)
+    ops().gemm_w4(x, words, s, z, group, out, status_word())
+    keep = torch.arange(N, device=DEV) != 33
+    assert torch.equal(torch.nan_to_num(out[:, keep], nan=-1e9), torch.nan_to_num(want[:, keep], nan=-1e9))
+    assert not torch.isfinite(out[:, 33]).any() or (w[33, 256:] == 0).all()
+
+
+@pytest.mark.parametrize("M", [1, 16, 33, 128, 140, 300])
+def test_products_repeat_bit_for_bit_and_rows_stand_alone(M):
+    """The same inputs give the same bits; a row's result does not change with the rows behind it as long as the kernel is the same one."""
+    g = gen(M)
+    N, K = 512, 4096
+    a, w = torch.empty(M, K, dtype=E4M3, device=DEV), torch.empty(N, K, dtype=E4M3, device=DEV)
+    sa, sw = torch.empty(M, device=DEV), torch.empty(N, device=DEV)
+    ops().quantize_q8(torch.randn(M, K, generator=g, device=DEV), a, sa)
+    ops().quantize_q8(torch.randn(N, K, generator=g, device=DEV), w, sw)
+    words, s, z, _ = w4_weight(g, N, K, 128, True, whole=False)
+    x = torch.randn(M, K, generator=g, device=DEV).to(BF16)
+    first = None
+    for _ in range(3):
+        out, out4 = torch.empty(M, N, device=DEV), torch.empty(M, N, device=DEV)
+        ops().gemm_q8(a, sa, w, sw, out, status_word())
+        ops().gemm_w4(x, words, s, z, 128, out4, status_word())
+        if first is None:
+            first = (out, out4)
+        assert torch.equal(out, first[0]) and torch.equal(out4, first[1])
+
+
+# ---- as they are used: streams, graphs, one behind the other ------------------------------------------------------
+
+def chain(o, g, M, d, F, stream_row, weights):
+    """A gated feed-forward in 8 bits on the residual stream, as a layer runs it."""
+    x, sx = torch.empty(M, d, dtype=E4M3, device=DEV), torch.empty(M, device=DEV)
+    gu, act, sact, y = (torch.empty(M, 2 * F, dtype=BF16, device=DEV), torch.empty(M, F, dtype=E4M3, device=DEV), torch.empty(M, device=DEV),
+                        torch.empty(M, d, dtype=BF16, device=DEV))
+    st = status_word()
+
+    def run():
+        o.add_rmsnorm_q8(stream_row, None, weights["norm"], 1e-5, x, sx)
+        o.gemm_q8(x, sx, weights["gu"], weights["sgu"], gu, st)
+        o.swiglu_q8(gu, act, sact, 8)
+        o.gemm_q8(act, sact, weights["down"], weights["sdown"], y, st)
+        return y
+
+    return run, st
+
+
+@pytest.mark.parametrize("M", [1, 12, 40, 200])
+def test_a_feed_forward_in_8_bits_eager_on_a_stream_and_captured(M):
+    o, g, d, F = ops(), gen(M), 512, 1408
+    w = {"norm": torch.ones(d, device=DEV)}
+    wf = {"gu": torch.randn(2 * F, d, generator=g, device=DEV) * 0.05, "down": torch.randn(d, F, generator=g, device=DEV) * 0.05}
+    for k, t in wf.items():
+        w[k], w["s" + k] = torch.empty(t.shape, dtype=E4M3, device=DEV), torch.empty(t.shape[0], device=DEV)
+        o.quantize_q8(t, w[k], w["s" + k])
+    h = torch.randn(M, d, generator=g, device=DEV)
+    run, st = chain(o, g, M, d, F, h, w)
+    want = run().clone()
+    # against fp32 weights and activations: two roundings to e4m3 a product, independent over the entries, of 2^-4 / sqrt(3) of each at most;
+    # the relative error of a product of many entries is that of one (root of the sum of squares), of the two in turn below twice 0.055
+    x = h / torch.sqrt((h * h).mean(1, keepdim=True) + 1e-5)
+    gu = (x @ wf["gu"].t()).view(M, -1, 2, 8)
+    ref = (torch.nn.functional.silu(gu[:, :, 0]) * gu[:, :, 1]).reshape(M, F) @ wf["down"].t()
+    assert (want.float() - ref).norm() <= 0.11 * ref.norm()
+    side = torch.cuda.Stream()
+    side.wait_stream(torch.cuda.current_stream())
+    with torch.cuda.stream(side):
+        got = run().clone()
+    side.synchronize()
+    assert torch.equal(got, want)
+    graph = torch.cuda.CUDAGraph()
+    with torch.cuda.stream(side):
+        with torch.cuda.graph(graph, stream=side):
+            y = run()
+    h2 = torch.randn(M, d, generator=g, device=DEV)
+    keep = h.clone()
+    h.copy_(h2)
+    torch.cuda.synchronize()
+    graph.replay()
+    torch.cuda.synchronize()
+    replayed = y.clone()
+    assert torch.equal(run(), replayed)
+    h.copy_(keep)
+    torch.cuda.synchronize()
+    graph.replay()
+    torch.cuda.synchronize()
+    assert torch.equal(y, want) and st.item() == 0
+
+
+def test_two_streams_at_once():
+    """Two products that run at the same time share nothing."""
+    o, g = ops(), gen(3)
+    M, N, K = 24, 1024, 4096
+    words, s, z, w = w4_weight(g, N, K, 128, True)
+    xs = [torch.randint(-4, 5, (M, K), generator=g, device=DEV).to(BF16) for _ in range(2)]
+    want = [torch.mm(x.double(), w.t()).to(F32) for x in xs]
+    outs = [[torch.empty(M, N, device=DEV) for _ in range(8)] for _ in range(2)]
+    streams = [torch.cuda.Stream() for _ in range(2)]
+    torch.cuda.synchronize()
+    for i in range(8):
+        for k in range(2):
+            with torch.cuda.stream(streams[k]):
+                o.gemm_w4(xs[k], words, s, z, 128, outs[k][i], None)
+    torch.cuda.synchronize()
+    assert all(torch.equal(outs[k][i], want[k]) for k in range(2) for i in range(8))

@@ -1,0 +1,162 @@
+"""The operators of the 8-bit and 4-bit formats without a GPU: what they refuse, and the packing of 4-bit weights."""
+import pytest
+import torch
+
+from llm_steadyinfer_b200.csrc import ops
+
+E4M3, BF16 = torch.float8_e4m3fn, torch.bfloat16
+
+
+def test_cpu_tensors_are_refused():
+    with pytest.raises(ops.KernelError, match="CUDA tensors only"):
+        ops.quantize_q8(torch.zeros(2, 8), torch.zeros(2, 8).to(E4M3), torch.zeros(2))
+
+
+@pytest.fixture
+def checks_alone(monkeypatch):
+    """The checks of arguments on CPU tensors: the device is not asked about, and a call that passes them would reach ``launched``."""
+    launched = []
+
+    def fn(lib, symbol, argtypes):
+        def call(*args):
+            assert len(args) == len(argtypes)
+            launched.append(symbol)
+            return 0
+        return call
+
+    monkeypatch.setattr(ops, "_here", lambda *a: None)
+    monkeypatch.setattr(ops, "_stream", lambda: 0)
+    monkeypatch.setattr(ops, "_fn", fn)
+    monkeypatch.setattr(ops, "gemm_tc05_available", lambda: True)
+    return launched
+
+
+def z(*shape, dtype=torch.float32):
+    return torch.zeros(*shape, dtype=dtype)
+
+
+def norm_args(**kw):
+    a = dict(resid=z(3, 16), delta=z(3, 16, dtype=BF16), weight=z(16), eps=1e-5, out=z(3, 16, dtype=E4M3), scale=z(3))
+    a.update(kw)
+    return a
+
+
+@pytest.mark.parametrize("kw,text", [
+    (dict(resid=z(3, 16, dtype=BF16)), "fp32"),
+    (dict(resid=z(16, 3).t()), "contiguous"),
+    (dict(weight=z(15)), "weight"),
+    (dict(delta=z(3, 15, dtype=BF16)), "delta"),
+    (dict(delta=z(3, 16, dtype=torch.float16)), "float32 or bfloat16"),
+    (dict(delta2=z(3, 16)), "one dtype"),
+    (dict(delta=None, delta2=z(3, 16)), "delta"),
+    (dict(out=z(3, 16, dtype=BF16)), "float8"),
+    (dict(out=z(2, 16, dtype=E4M3)), "float8"),
+    (dict(scale=z(4)), "scale"),
+    (dict(scale=z(6)[::2]), "scale"),
+    (dict(dst=z(3, 17)), "dst"),
+    (dict(rows=z(3, dtype=torch.int32), dst=z(3, 16)), "no stream"),
+    (dict(rows=z(3, dtype=torch.int64)), "int32"),
+])
+def test_norm_refusals(checks_alone, kw, text):
+    with pytest.raises(ops.KernelError, match=text):
+        ops.add_rmsnorm_q8(**norm_args(**kw))
+    assert not checks_alone
+
+
+def test_norm_passes(checks_alone):
+    ops.add_rmsnorm_q8(**norm_args())
+    ops.add_rmsnorm_q8(**norm_args(rows=z(3, dtype=torch.int32)))
+    assert checks_alone == ["si_add_rmsnorm_q8"] * 2
+
+
+@pytest.mark.parametrize("gu,out,scale,group", [
+    (z(2, 31), z(2, 16, dtype=E4M3), z(2), None), (z(2, 32), z(2, 16), z(2), None), (z(2, 32), z(2, 16, dtype=E4M3), z(2), 5),
+    (z(2, 32), z(2, 16, dtype=E4M3), z(2), -8), (z(2, 32), z(2, 16, dtype=E4M3), z(1), None), (z(32, 2).t(), z(2, 16, dtype=E4M3), z(2), None),
+    (z(2, 32, dtype=torch.float16), z(2, 16, dtype=E4M3), z(2), None), (z(2, 0), z(2, 0, dtype=E4M3), z(2), None)])
+def test_swiglu_refusals(checks_alone, gu, out, scale, group):
+    with pytest.raises(ops.KernelError):
+        ops.swiglu_q8(gu, out, scale, group)
+    assert not checks_alone
+
+
+@pytest.mark.parametrize("x,out,scale", [
+    (z(2, 8, dtype=torch.float16), z(2, 8, dtype=E4M3), z(2)), (z(8, 2).t(), z(2, 8, dtype=E4M3), z(2)), (z(2, 8), z(2, 9, dtype=E4M3), z(2)),
+    (z(2, 8), z(2, 8, dtype=E4M3), z(3)), (z(2, 4, 8), z(2, 8, dtype=E4M3), z(2)), (z(2, 0), z(2, 0, dtype=E4M3), z(2))])
+def test_quantize_refusals(checks_alone, x, out, scale):
+    with pytest.raises(ops.KernelError):
+        ops.quantize_q8(x, out, scale)
+    assert not checks_alone
+
+
+def q8_args(**kw):
+    a = dict(a=z(3, 32, dtype=E4M3), a_scale=z(3), w=z(5, 32, dtype=E4M3), w_scale=z(5), out=z(3, 5, dtype=BF16))
+    a.update(kw)
+    return a
+
+
+@pytest.mark.parametrize("kw", [
+    dict(a=z(3, 32, dtype=BF16)), dict(w=z(5, 32, dtype=torch.float8_e5m2)), dict(w=z(5, 31, dtype=E4M3)), dict(out=z(3, 6, dtype=BF16)),
+    dict(out=z(3, 5, dtype=torch.float16)), dict(out=z(5, 3, dtype=BF16).t()), dict(out=z(1, 5, dtype=BF16).expand(3, 5)), dict(a_scale=z(2)),
+    dict(w_scale=z(5, dtype=BF16)), dict(a=z(32, 3, dtype=E4M3).t()), dict(status=z(1)), dict(a=z(3, 0, dtype=E4M3), w=z(5, 0, dtype=E4M3)),
+    dict(a=z(32, dtype=E4M3))])
+def test_gemm_q8_refusals(checks_alone, kw):
+    with pytest.raises(ops.KernelError):
+        ops.gemm_q8(**q8_args(**kw))
+    assert not checks_alone
+
+
+def w4_args(**kw):
+    a = dict(x=z(3, 64, dtype=BF16), w=z(5, 8, dtype=torch.int32), scales=z(5, 2, dtype=BF16), zeros=z(5, 2, dtype=torch.uint8), group=32, out=z(3, 5, dtype=BF16))
+    a.update(kw)
+    return a
+
+
+@pytest.mark.parametrize("kw", [
+    dict(x=z(3, 64)), dict(w=z(5, 8)), dict(w=z(5, 7, dtype=torch.int32)), dict(group=48), dict(group=0), dict(group=-128), dict(group=96), dict(group=192),
+    dict(group=64), dict(scales=z(5, 2)), dict(scales=z(2, 5, dtype=BF16).t()), dict(zeros=z(5, 2, dtype=torch.int8)), dict(zeros=z(5, 1, dtype=torch.uint8)),
+    dict(out=z(3, 5, dtype=torch.float16)), dict(out=z(2, 5, dtype=BF16)), dict(out=z(1, 5, dtype=BF16).expand(3, 5)),
+    dict(x=z(3, 60, dtype=BF16)), dict(x=z(64, 3, dtype=BF16).t()), dict(status=z(1))])
+def test_gemm_w4_refusals(checks_alone, kw):
+    with pytest.raises(ops.KernelError):
+        ops.gemm_w4(**w4_args(**kw))
+    assert not checks_alone
+
+
+def test_products_pass_and_empty_ones_launch_nothing(checks_alone):
+    ops.gemm_q8(**q8_args())
+    ops.gemm_w4(**w4_args())
+    n = len(checks_alone)
+    assert n == 2
+    ops.gemm_q8(**q8_args(a=z(0, 32, dtype=E4M3), a_scale=z(0), out=z(0, 5, dtype=BF16)))
+    ops.gemm_w4(**w4_args(x=z(0, 64, dtype=BF16), out=z(0, 5, dtype=BF16)))
+    ops.quantize_q8(z(0, 8), z(0, 8, dtype=E4M3), z(0))
+    assert len(checks_alone) == n
+
+
+def test_a_tensor_of_another_device_is_refused(monkeypatch):
+    class Elsewhere:
+        is_cuda = True
+
+        def __init__(self, index):
+            self.index = index
+
+        def get_device(self):
+            return self.index
+
+    monkeypatch.setattr(ops, "_device_index", 1)
+    ops._here("x", Elsewhere(1), None)
+    with pytest.raises(ops.KernelError, match="device 0"):
+        ops._here("x", Elsewhere(1), Elsewhere(0))
+
+
+@pytest.mark.parametrize("N,K", [(1, 8), (5, 64), (3, 136)])
+def test_pack_and_unpack(N, K):
+    q = torch.randint(0, 16, (N, K), generator=torch.Generator().manual_seed(K))
+    words = ops.pack_w4(q)
+    assert words.shape == (N, K // 8) and words.dtype == torch.int32
+    assert torch.equal(ops.unpack_w4(words), q.to(torch.int32))
+    u = words.long() & 0xFFFFFFFF
+    for i in range(8):                                           # entry i of the eight at bit 4 (i / 2) + 16 (i % 2)
+        assert torch.equal((u >> (4 * (i // 2) + 16 * (i % 2))) & 15, q[:, i::8])
+    with pytest.raises(ops.KernelError):
+        ops.pack_w4(q[:, :7])
