@@ -2423,8 +2423,15 @@ def gemm_q8(a, a_scale, w, w_scale, out, status=None) -> None:
     if M == 0 or N == 0:
         return
     _need(K > 0, "gemm_q8: rows without entries")
+    lda, ldw = _ld(a), _ld(w)
+    if (a.data_ptr() | w.data_ptr() | lda | ldw) % 16 == 0 and lda >= K and ldw >= K and gemm_tc05_available():
+        f = _fn("gemm_q8", "si_gemm_q8", [_c_p, _c_ll, _c_p, _c_p, _c_ll, _c_p, _c_p, _c_ll, _c_int, _c_int, _c_int, _c_int, _c_p, _c_p])
+        _check(f(_ptr(a), lda, _ptr(a_scale), _ptr(w), ldw, _ptr(w_scale), _ptr(out), _ld(out), od, M, N, K, _ptr(status), _stream()),
+               f"gemm_q8(M={M}, N={N}, K={K})")
+        return
+    # rows that do not start on 16-byte boundaries
     f = _fn("gemm_quant", "si_gemm_quant_q8", [_c_p, _c_ll, _c_p, _c_p, _c_ll, _c_p, _c_p, _c_ll, _c_int, _c_int, _c_int, _c_int, _c_p])
-    _check(f(_ptr(a), _ld(a), _ptr(a_scale), _ptr(w), _ld(w), _ptr(w_scale), _ptr(out), _ld(out), od, M, N, K, _stream()),
+    _check(f(_ptr(a), lda, _ptr(a_scale), _ptr(w), ldw, _ptr(w_scale), _ptr(out), _ld(out), od, M, N, K, _stream()),
            f"gemm_q8(M={M}, N={N}, K={K})")
 
 
@@ -2451,8 +2458,16 @@ def gemm_w4(x, w, scales, zeros, group: int, out, status=None) -> None:
     if M == 0 or N == 0:
         return
     _need(K > 0, "gemm_w4: rows without entries")
+    ldx, ldw = _ld(x), _ld(w)
+    if ((x.data_ptr() | w.data_ptr()) % 16 == 0 and ldx % 8 == 0 and ldw % 4 == 0 and K % 32 == 0 and ldx >= K and ldw * 8 >= K
+            and gemm_tc05_available() and M <= 16):
+        f = _fn("gemm_w4", "si_gemm_w4", [_c_p, _c_ll, _c_p, _c_ll, _c_p, _c_p, _c_int, _c_p, _c_ll, _c_int, _c_int, _c_int, _c_int, _c_p, _c_p])
+        _check(f(_ptr(x), ldx, _ptr(w), ldw, _ptr(scales), _ptr(zeros), group, _ptr(out), _ld(out), od, M, N, K, _ptr(status), _stream()),
+               f"gemm_w4(M={M}, N={N}, K={K}, group={group})")
+        return
+    # rows that are not in 16-byte pieces
     f = _fn("gemm_quant", "si_gemm_quant_w4", [_c_p, _c_ll, _c_p, _c_ll, _c_p, _c_p, _c_int, _c_p, _c_ll, _c_int, _c_int, _c_int, _c_int, _c_p])
-    _check(f(_ptr(x), _ld(x), _ptr(w), _ld(w), _ptr(scales), _ptr(zeros), group, _ptr(out), _ld(out), od, M, N, K, _stream()),
+    _check(f(_ptr(x), ldx, _ptr(w), ldw, _ptr(scales), _ptr(zeros), group, _ptr(out), _ld(out), od, M, N, K, _stream()),
            f"gemm_w4(M={M}, N={N}, K={K}, group={group})")
 
 
