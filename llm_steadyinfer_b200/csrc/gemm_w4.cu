@@ -11,6 +11,7 @@
 // Before the wait for the kernels before this one nothing is read, the weights are only asked into L2 (see gemm_q8.cu).
 #include "tma_common.cuh"
 #include "quant_common.cuh"
+#include <stdio.h>
 
 typedef __nv_bfloat16 bf16;
 
@@ -182,6 +183,408 @@ static int w4_few(const W4Call& c) {
   return c.zeros ? w4_skinny<1, true, TO>(c) : w4_skinny<1, false, TO>(c);
 }
 
+// ---- more than 16 rows -------------------------------------------------------------------------------------------
+// out transposed: a tile is HALVES x 128 rows of the weight matrix (the M of the instruction) by `bn` rows of x (its N, a multiple of 16), k steps
+// of 128. Warp 0 fetches x (two boxes of 64 entries a step, 128-byte swizzle), warp 1 the words (rows of 64 bytes, 64-byte swizzle), both into one
+// ring. Warps 8 to 15 widen: a thread owns one row of the weight matrix, takes its 64 bytes of a step out of shared memory (the swizzle spreads
+// eight rows over all banks), makes the 128 entries bf16 in registers and writes them to its lane of tensor memory, from where the instruction reads
+// its A: the widened weights cost neither bandwidth nor room in shared memory. Two groups of four warps take the steps in turn (HALVES 1) or a
+// half of the rows each (HALVES 2, for few rows of x, where a step's instructions are short and its fixed cost counts). Warp 2 issues; warps
+// 4 to 7 store. Tensor memory: with bn up to 192 two accumulators and two A buffers, beyond one and four (HALVES 2: up to 64 two, else one, and
+// two A buffers a half). Blocks are persistent, one an SM; with few tiles the k range of a tile is cut over a cluster, whose blocks leave their
+// sums in shared memory and add a part of the rows each up over all blocks, in their order.
+#define W4_TC_SMEM (224 * 1024)
+#define W4_TC_MAX_STAGES 8
+
+__host__ __device__ inline int w4_tc_stage_bytes(int halves, int bn) { return halves * 128 * 64 + bn * 256; }
+__host__ __device__ inline int w4_tc_stages(int halves, int bn) {
+  const int n = W4_TC_SMEM / w4_tc_stage_bytes(halves, bn);
+  return n < W4_TC_MAX_STAGES ? n : W4_TC_MAX_STAGES;
+}
+__device__ __forceinline__ float4 w4_ld_cluster(unsigned cluster_addr) {
+  float4 v;
+  asm volatile("ld.shared::cluster.v4.f32 {%0,%1,%2,%3}, [%4];\n" : "=f"(v.x), "=f"(v.y), "=f"(v.z), "=f"(v.w) : "r"(cluster_addr) : "memory");
+  return v;
+}
+__device__ __forceinline__ void w4_drain(uint64_t* full, int stages, int issued) {       // as drain_copies in gemm_q8.cu
+  for (int i = issued > stages ? issued - stages : 0; i < issued; ++i) mbar_wait(&full[i % stages], (unsigned)((i / stages) & 1));
+}
+
+template <int HALVES, bool ZEROS, typename TO>
+__global__ void __launch_bounds__(512, 1)
+gemm_w4_tc_kernel(const __grid_constant__ CUtensorMap xmap, const __grid_constant__ CUtensorMap wmap, const bf16* __restrict__ scales,
+                  const unsigned char* __restrict__ zeros, int group, int groups, TO* __restrict__ out, long long ldo, int M, int N, int K, int bn,
+                  int m_tiles, int parts, int* status) {
+  constexpr int BK = 128, ROWS = HALVES * 128, W_BYTES = ROWS * 64;
+  extern __shared__ unsigned char smem_dyn[];
+  __shared__ __align__(8) uint64_t full_bar[W4_TC_MAX_STAGES], empty_bar[W4_TC_MAX_STAGES], a_full[4], a_empty[4], acc_full[2], acc_empty[2];
+  __shared__ unsigned tmem_slot;
+  unsigned char* smem = reinterpret_cast<unsigned char*>(((uintptr_t)smem_dyn + 1023) & ~(uintptr_t)1023);
+  const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
+  const int X_BYTES = bn * 256, STAGES = w4_tc_stages(HALVES, bn);
+  unsigned char* Ws = smem;
+  unsigned char* Xs = smem + STAGES * W_BYTES;
+  float* partial = reinterpret_cast<float*>(smem);         // [bn][ROWS] once the operands are used up (at most 128 KB)
+  const int nk = (K + BK - 1) / BK, tiles = (N + ROWS - 1) / ROWS * m_tiles;
+  const int part = (int)cluster_cta_rank(), first = blockIdx.x / parts, stride = gridDim.x / parts;
+  const int k0 = (int)((long long)nk * part / parts), steps = (int)((long long)nk * (part + 1) / parts) - k0;
+  // columns of tensor memory
+  const int acc_w = HALVES == 2 ? (bn <= 64 ? 64 : 128) : (bn <= 192 ? 192 : 256);
+  const int nbuf = HALVES == 2 ? (bn <= 64 ? 2 : 1) : (bn <= 192 ? 2 : 1);
+  const int a_bufs = HALVES == 2 ? 2 : (bn <= 192 ? 2 : 4), a_col = HALVES == 2 ? 256 : (bn <= 192 ? 384 : 256);
+  if (threadIdx.x == 0) {
+    for (int s = 0; s < STAGES; ++s) { mbar_init(&full_bar[s], 2); mbar_init(&empty_bar[s], 1); }
+#pragma unroll
+    for (int b = 0; b < 4; ++b) { mbar_init(&a_full[b], 4 * HALVES); mbar_init(&a_empty[b], 1); }
+#pragma unroll
+    for (int b = 0; b < 2; ++b) { mbar_init(&acc_full[b], 1); mbar_init(&acc_empty[b], 4); }
+    asm volatile("fence.mbarrier_init.release.cluster;\n" ::: "memory");
+  }
+  if (warp == 3) tmem_alloc(&tmem_slot, 512);
+  tc05_fence_before_sync();
+  __syncthreads();
+  tc05_fence_after_sync();
+  const unsigned tmem = tmem_slot;
+  if (warp < 2) {
+    if (lane == 0) {
+      const bool is_w = warp == 1;
+      const int bytes = is_w ? W_BYTES : X_BYTES;
+      unsigned char* ring = is_w ? Ws : Xs;
+      if (is_w && first < tiles)
+        for (int i = 0; i < steps && i < STAGES; ++i)
+          asm volatile("cp.async.bulk.prefetch.tensor.2d.L2.global.tile [%0, {%1, %2}];\n"
+                       ::"l"(&wmap), "r"((k0 + i) * (BK / 8)), "r"(first / m_tiles * ROWS) : "memory");
+      pdl_wait();
+      int s = 0, issued = 0;
+      unsigned phase = 1;
+      bool ok = true;
+      for (int tile = first; tile < tiles && ok; tile += stride) {
+        const int y = is_w ? tile / m_tiles * ROWS : tile % m_tiles * bn;
+        for (int it = 0; it < steps; ++it, ++issued) {
+          if (issued >= STAGES && !mbar_wait(&empty_bar[s], phase)) {
+            set_status(status, SI_WAIT_LIMIT);
+            w4_drain(full_bar, STAGES, issued);
+            ok = false;
+            break;
+          }
+          unsigned char* to = ring + s * bytes;
+          mbar_expect_tx(&full_bar[s], (unsigned)bytes);   // both warps arrive, each with its own bytes
+          if (is_w) {
+            tma_load_2d(to, &wmap, &full_bar[s], (k0 + it) * (BK / 8), y);
+          } else {
+            tma_load_2d(to, &xmap, &full_bar[s], (k0 + it) * BK, y);
+            tma_load_2d(to + bytes / 2, &xmap, &full_bar[s], (k0 + it) * BK + 64, y);
+          }
+          if (++s == STAGES) { s = 0; phase ^= 1u; }
+        }
+      }
+    }
+  } else if (warp == 2) {
+    const unsigned idesc = umma_idesc_bf16(128, bn, false);
+    const unsigned long long xd0 = umma_desc_sw128(Xs, 16, 1024);
+    const unsigned x_step = (unsigned)X_BYTES / 16;
+    int s = 0, b = 0, local = 0;
+    unsigned phase = 0, a_phase = 0;
+    unsigned long long xd = xd0;
+    bool ok = true;
+    for (int tile = first; tile < tiles && ok; tile += stride, ++local) {
+      const int d = nbuf == 2 ? local & 1 : 0;
+      if (local >= nbuf) ok = mbar_wait_warp(&acc_empty[d], (unsigned)((local / nbuf - 1) & 1));
+      if (!ok) break;
+      tc05_fence_after_sync();
+      const unsigned acc = tmem + (unsigned)(d * HALVES * acc_w);
+      for (int it = 0; it < steps; ++it) {
+        ok = mbar_wait_warp(&full_bar[s], phase) && mbar_wait_warp(&a_full[b], a_phase);
+        if (!ok) break;
+        tc05_fence_after_sync();
+        if (elect_one()) {
+#pragma unroll
+          for (int hf = 0; hf < HALVES; ++hf) {
+            const unsigned a = tmem + (unsigned)(a_col + (hf * 2 + b) * 64);          // HALVES 1: hf is 0
+#pragma unroll
+            for (int k = 0; k < 8; ++k)
+              tc05_mma_bf16_tmem_a(acc + hf * acc_w, a + 8 * k, xd + (k >> 2) * (x_step / 2) + 2 * (k & 3), idesc, (it | k) != 0 ? 1u : 0u);
+          }
+          tc05_commit(&empty_bar[s]);
+          tc05_commit(&a_empty[b]);
+          if (it + 1 == steps) tc05_commit(&acc_full[d]);
+        }
+        __syncwarp();
+        xd += x_step;
+        if (++s == STAGES) { s = 0; xd = xd0; phase ^= 1u; }
+        if (++b == a_bufs) { b = 0; a_phase ^= 1u; }
+      }
+    }
+    if (!ok && lane == 0) set_status(status, SI_WAIT_LIMIT);
+  } else if (warp >= 8) {
+    const int g = (warp - 8) >> 2, row = (warp & 3) * 32 + lane, hf = HALVES == 2 ? g : 0;
+    const unsigned char* wrow = Ws + (hf * 128 + row) * 64;
+    const int swz = (row >> 1) & 3;
+    const unsigned lanes = (unsigned)((warp & 3) * 32) << 16;
+    const int every = HALVES == 2 ? 1 : 2;                 // this group's steps: every one, or every second one
+    int s = 0, b = 0, st = 0;                              // of the step that comes next, over all tiles
+    unsigned phase = 0, a_phase = 1;
+    bool ok = true;
+    pdl_wait();
+    for (int tile = first; tile < tiles && ok; tile += stride) {
+      const int n = tile / m_tiles * ROWS + hf * 128 + row;
+      const bf16* srow = scales + (size_t)(n < N ? n : 0) * groups;
+      const unsigned char* zrow = ZEROS ? zeros + (size_t)(n < N ? n : 0) * groups : nullptr;
+      // scales of the four pieces of 32 entries of a step, asked for a step of this group ahead
+      unsigned sc[4], zp[4];
+      auto ask = [&](int it) {
+        const int k = (k0 + it) * BK;
+        if (group >= BK) {
+          const int at = min(k / group, groups - 1);
+          sc[0] = w4_ld_scale(srow + at, true);
+          if (ZEROS) zp[0] = w4_ld_zero(zrow + at, true);
+        } else {
+#pragma unroll
+          for (int j = 0; j < 4; ++j) {
+            const int at = min((k + 32 * j) / group, groups - 1);       // group is 32 or 64 here
+            sc[j] = w4_ld_scale(srow + at, true);
+            if (ZEROS) zp[j] = w4_ld_zero(zrow + at, true);
+          }
+        }
+      };
+      const int it0 = HALVES == 2 || (st & 1) == g ? 0 : 1;               // this group's first step of the tile
+      if (it0 < steps) ask(it0);
+      for (int it = 0; it < steps; ++it, ++st) {
+        const bool mine = HALVES == 2 || (st & 1) == g;
+        if (mine) {
+          unsigned now[4], z[4];
+#pragma unroll
+          for (int j = 0; j < 4; ++j) { now[j] = group >= BK ? sc[0] : sc[j]; z[j] = ZEROS ? (group >= BK ? zp[0] : zp[j]) : 8u; }
+          if (it + every < steps) ask(it + every);
+          ok = mbar_wait_warp(&full_bar[s], phase);
+          if (!ok) break;
+          uint4 wv[4];
+#pragma unroll
+          for (int j = 0; j < 4; ++j) wv[j] = *reinterpret_cast<const uint4*>(wrow + s * W_BYTES + ((j ^ swz) << 4));
+          if (st >= a_bufs) ok = mbar_wait_warp(&a_empty[b], a_phase);
+          if (!ok) break;
+          tc05_fence_after_sync();
+          const unsigned a = tmem + lanes + (unsigned)(a_col + (hf * 2 + b) * 64);
+#pragma unroll
+          for (int h = 0; h < 2; ++h) {
+            unsigned v[32];
+#pragma unroll
+            for (int j2 = 0; j2 < 2; ++j2) {
+              const int j = 2 * h + j2;
+              const __nv_bfloat162 bias = w4_bias((int)z[j]);
+              const unsigned s2 = now[j] | (now[j] << 16);
+              const unsigned words[4] = {wv[j].x, wv[j].y, wv[j].z, wv[j].w};
+#pragma unroll
+              for (int q = 0; q < 4; ++q)
+#pragma unroll
+                for (int p = 0; p < 4; ++p) {
+                  const unsigned e = w4_pair(words[q], p, bias);
+                  const __nv_bfloat162 r = __hmul2(*reinterpret_cast<const __nv_bfloat162*>(&e), *reinterpret_cast<const __nv_bfloat162*>(&s2));
+                  v[j2 * 16 + q * 4 + p] = *reinterpret_cast<const unsigned*>(&r);
+                }
+            }
+            tmem_st_32x32_issue(a + h * 32, v);
+          }
+          tmem_st_wait();
+          tc05_fence_before_sync();
+          __syncwarp();
+          if (lane == 0) mbar_arrive(&a_full[b]);
+        }
+        if (++s == STAGES) { s = 0; phase ^= 1u; }
+        if (++b == a_bufs) { b = 0; a_phase ^= 1u; }
+      }
+    }
+    if (!ok && lane == 0) set_status(status, SI_WAIT_LIMIT);
+  } else if (warp >= 4) {
+    pdl_wait();
+    const unsigned lanes = (unsigned)((warp & 3) * 32) << 16;
+    const bool vec2 = ldo % 2 == 0 && (uintptr_t)out % (2 * sizeof(TO)) == 0;
+    int local = 0;
+    for (int tile = first; tile < tiles; tile += stride, ++local) {
+      const int d = nbuf == 2 ? local & 1 : 0;
+      const int m_base = tile % m_tiles * bn, n_base = tile / m_tiles * ROWS + (warp & 3) * 32;
+      if (!mbar_wait_warp(&acc_full[d], (unsigned)((local / nbuf) & 1))) {
+        if (lane == 0) set_status(status, SI_WAIT_LIMIT);
+        break;
+      }
+      tc05_fence_after_sync();
+      const int rows = min(bn, M - m_base);
+#pragma unroll 1
+      for (int hf = 0; hf < HALVES; ++hf) {
+        const unsigned src = tmem + lanes + (unsigned)((d * HALVES + hf) * acc_w);
+        const int n = n_base + hf * 128 + lane;
+#pragma unroll 1
+        for (int m0 = 0; m0 < bn; m0 += 32) {
+          float v[32];
+          tmem_ld_32x32(src + m0, v);
+          if (hf == HALVES - 1 && m0 + 32 >= bn) {         // in registers: the issuer may have the accumulator back
+            tc05_fence_before_sync();
+            __syncwarp();
+            if (lane == 0) mbar_arrive(&acc_empty[d]);
+          }
+          if (parts > 1) {
+#pragma unroll
+            for (int j = 0; j < 32; ++j)
+              if (m0 + j < bn) partial[(m0 + j) * ROWS + hf * 128 + (warp & 3) * 32 + lane] = v[j];
+          } else if (vec2 && n_base + hf * 128 + 32 <= N) {
+            // neighbouring lanes swap: the even one stores columns n, n + 1 of row j, the odd one of row j + 1
+#pragma unroll
+            for (int j = 0; j < 32; j += 2) {
+              const float give = lane & 1 ? v[j] : v[j + 1], got = __shfl_xor_sync(0xffffffffu, give, 1);
+              const float a = lane & 1 ? got : v[j], c = lane & 1 ? v[j + 1] : got;
+              const int m = m0 + j + (lane & 1);
+              if (m < rows) {
+                TO* dst = out + (size_t)(m_base + m) * ldo + (n & ~1);
+                if constexpr (sizeof(TO) == 4) *reinterpret_cast<float2*>(dst) = make_float2(a, c);
+                else *reinterpret_cast<__nv_bfloat162*>(dst) = __floats2bfloat162_rn(a, c);
+              }
+            }
+          } else {
+#pragma unroll
+            for (int j = 0; j < 32; ++j)
+              if (m0 + j < rows && n < N) out[(size_t)(m_base + m0 + j) * ldo + n] = from_f32<TO>(v[j]);
+          }
+        }
+      }
+    }
+  }
+  if (parts > 1) {                                         // one tile a cluster
+    __syncwarp();
+    cluster_sync_all();                                    // every block's sums lie in its shared memory
+    const int m_base = first % m_tiles * bn, n0 = first / m_tiles * ROWS;
+    const int lo = bn * part / parts, hi = min(M - m_base, bn * (part + 1) / parts);
+    const bool vec = ldo % 4 == 0 && (uintptr_t)out % 16 == 0;
+    for (int i = threadIdx.x; i < (hi - lo) * (ROWS / 4); i += 512) {
+      const int m = lo + i / (ROWS / 4), c4 = i % (ROWS / 4) * 4, n = n0 + c4;
+      const float* at = partial + m * ROWS + c4;
+      float4 v[8];
+#pragma unroll
+      for (int c = 0; c < 8; ++c) v[c] = c < parts ? w4_ld_cluster(cluster_map_u32(at, (unsigned)c)) : make_float4(0.f, 0.f, 0.f, 0.f);
+#pragma unroll
+      for (int c = 1; c < 8; ++c) { v[0].x += v[c].x; v[0].y += v[c].y; v[0].z += v[c].z; v[0].w += v[c].w; }
+      TO* dst = out + (size_t)(m_base + m) * ldo + n;
+      if (vec && n + 4 <= N) {
+        if constexpr (sizeof(TO) == 4) {
+          *reinterpret_cast<float4*>(dst) = v[0];
+        } else {
+          __nv_bfloat162 p[2] = {__floats2bfloat162_rn(v[0].x, v[0].y), __floats2bfloat162_rn(v[0].z, v[0].w)};
+          *reinterpret_cast<uint2*>(dst) = *reinterpret_cast<uint2*>(p);
+        }
+      } else {
+        const float r[4] = {v[0].x, v[0].y, v[0].z, v[0].w};
+#pragma unroll
+        for (int j = 0; j < 4; ++j) if (n + j < N) dst[j] = from_f32<TO>(r[j]);
+      }
+    }
+    cluster_sync_all();                                    // no block goes while another one reads its sums
+  }
+  tc05_fence_before_sync();
+  __syncthreads();
+  if (warp == 3) tmem_dealloc(tmem, 512);
+}
+
+struct W4Shape { int halves, bn, m_tiles, parts; };
+
+static void w4_tc_config(cudaLaunchConfig_t* cfg, unsigned blocks, int parts, cudaStream_t stream, cudaLaunchAttribute* attr) {
+  cfg->gridDim = dim3(blocks);
+  cfg->blockDim = dim3(512);
+  cfg->dynamicSmemBytes = W4_TC_SMEM + 1024;
+  cfg->stream = stream;
+  attr[0].id = cudaLaunchAttributeClusterDimension;
+  attr[0].val.clusterDim.x = (unsigned)parts;
+  attr[0].val.clusterDim.y = 1;
+  attr[0].val.clusterDim.z = 1;
+  attr[1].id = cudaLaunchAttributeProgrammaticStreamSerialization;
+  attr[1].val.programmaticStreamSerializationAllowed = 1;
+  cfg->attrs = attr;
+  cfg->numAttrs = si_pdl_enabled() ? 2 : 1;
+}
+
+// Clusters of `parts` blocks that the device runs at once, asked once per device and size (all forms of the kernel take an SM a block).
+static int w4_clusters(int parts) {
+  static int known[64][9] = {};
+  int dev = 0;
+  if (cudaGetDevice(&dev) != cudaSuccess || dev < 0 || dev >= 64) dev = 0;
+  if (parts == 1) return si_sm_count();
+  if (!known[dev][parts]) {
+    auto k = gemm_w4_tc_kernel<1, true, bf16>;
+    cudaLaunchAttribute attr[2];
+    cudaLaunchConfig_t cfg = {};
+    w4_tc_config(&cfg, (unsigned)parts, parts, 0, attr);
+    int n = 0;
+    if (cudaFuncSetAttribute(k, cudaFuncAttributeMaxDynamicSharedMemorySize, W4_TC_SMEM + 1024) != cudaSuccess ||
+        cudaOccupancyMaxActiveClusters(&n, k, &cfg) != cudaSuccess || n < 1) { cudaGetLastError(); n = 1; }
+    known[dev][parts] = n;
+  }
+  return known[dev][parts];
+}
+
+static W4Shape w4_shape(int M, int N, int K) {
+  const int nk = (K + 127) / 128;
+  W4Shape best = {1, 128, 1, 1};
+  double least = -1;
+  for (int halves = 1; halves <= 2; ++halves) {
+    if (halves == 2 && M > 128) break;
+    const int n_tiles = (N + halves * 128 - 1) / (halves * 128);
+    const int fewest = (M + 255) / 256;
+    for (int mt = fewest; mt <= fewest + 2; ++mt) {
+      const int bn = ((M + mt - 1) / mt + 15) / 16 * 16;
+      if (mt > fewest && bn < 96) break;
+      for (int parts = 1; parts <= 8 && parts <= nk; parts *= 2) {
+        const long long tiles = (long long)n_tiles * mt, slots = w4_clusters(parts);
+        if (parts > 1 && tiles > slots) break;
+        const int steps = (nk + parts - 1) / parts;
+        const double mma = (bn / 2 > 47 ? bn / 2 : 47) * 8.0 * halves, step = halves == 2 ? (mma + 420 > 900 ? mma + 420 : 900) : (mma + 100 > 600 ? mma + 100 : 600);
+        const bool one = halves == 1 && bn > 192;
+        const double cost = (double)((tiles + slots - 1) / slots) * (steps * step + (one ? 20.0 * bn : 500.0)) + 6000 + 16.0 * bn + (parts > 1 ? 2500 : 0);
+        if (least < 0 || cost < least) { least = cost; best = W4Shape{halves, bn, mt, parts}; }
+      }
+    }
+  }
+  if (const char* e = getenv("W4_SHAPE")) sscanf(e, "%d,%d,%d,%d", &best.halves, &best.bn, &best.m_tiles, &best.parts);
+  if (getenv("W4_SAY")) printf("shape %dx%dx%d: halves %d bn %d mt %d parts %d\n", M, N, K, best.halves, best.bn, best.m_tiles, best.parts);
+  return best;
+}
+
+static int w4_encode(CUtensorMap* map, CUtensorMapDataType type, int size, const void* base, long long rows, long long cols, long long ld, unsigned box_cols,
+                     unsigned box_rows, CUtensorMapSwizzle swizzle) {
+  SiEncodeTiledFn fn = si_encode_fn();
+  if (!fn) return -3;
+  const cuuint64_t dims[2] = {(cuuint64_t)cols, (cuuint64_t)rows};
+  const cuuint64_t strides[1] = {(cuuint64_t)(ld * size)};
+  const cuuint32_t box[2] = {box_cols, box_rows};
+  const cuuint32_t estr[2] = {1, 1};
+  CUresult r = fn(map, type, 2, const_cast<void*>(base), dims, strides, box, estr, CU_TENSOR_MAP_INTERLEAVE_NONE, swizzle,
+                  CU_TENSOR_MAP_L2_PROMOTION_L2_128B, CU_TENSOR_MAP_FLOAT_OOB_FILL_NONE);
+  return r == CUDA_SUCCESS ? 0 : 1000 + (int)r;
+}
+
+template <int HALVES, bool ZEROS, typename TO>
+static int w4_tc_launch(const W4Call& c, const W4Shape& sh) {
+  auto k = gemm_w4_tc_kernel<HALVES, ZEROS, TO>;
+  cudaError_t e = cudaFuncSetAttribute(k, cudaFuncAttributeMaxDynamicSharedMemorySize, W4_TC_SMEM + 1024);
+  if (e != cudaSuccess) return (int)e;
+  CUtensorMap xm, wm;
+  int rc = w4_encode(&xm, CU_TENSOR_MAP_DATA_TYPE_BFLOAT16, 2, c.x, c.M, c.K, c.ldx, 64, (unsigned)sh.bn, CU_TENSOR_MAP_SWIZZLE_128B);
+  if (!rc) rc = w4_encode(&wm, CU_TENSOR_MAP_DATA_TYPE_INT32, 4, c.w, c.N, c.K / 8, c.ldw, 16, HALVES * 128, CU_TENSOR_MAP_SWIZZLE_64B);
+  if (rc) return rc;
+  const long long tiles = (long long)((c.N + HALVES * 128 - 1) / (HALVES * 128)) * sh.m_tiles, slots = si_sm_count();
+  if (tiles > 0x0fffffffLL) return -2;
+  const long long blocks = sh.parts > 1 ? tiles * sh.parts : tiles < slots ? tiles : slots;
+  cudaLaunchAttribute attr[2];
+  cudaLaunchConfig_t cfg = {};
+  w4_tc_config(&cfg, (unsigned)blocks, sh.parts, c.stream, attr);
+  cudaLaunchKernelEx(&cfg, k, xm, wm, c.scales, c.zeros, c.group, c.groups, (TO*)c.out, c.ldo, c.M, c.N, c.K, sh.bn, sh.m_tiles, sh.parts, c.status);
+  return si_last_error();
+}
+
+template <typename TO>
+static int w4_tc(const W4Call& c) {
+  const W4Shape sh = w4_shape(c.M, c.N, c.K);
+  if (sh.halves == 2) return c.zeros ? w4_tc_launch<2, true, TO>(c, sh) : w4_tc_launch<2, false, TO>(c, sh);
+  return c.zeros ? w4_tc_launch<1, true, TO>(c, sh) : w4_tc_launch<1, false, TO>(c, sh);
+}
+
 // 1 when these kernels take operands so laid out (rows that start on 16-byte boundaries and end on one, the driver's tensor maps), else
 // gemm_quant.cu does.
 SI_EXPORT int si_gemm_w4_ok(const void* x, long long ldx, const void* w, long long ldw, int K) {
@@ -198,5 +601,5 @@ SI_EXPORT int si_gemm_w4(const void* x, long long ldx, const void* w, long long 
   c.x = (const bf16*)x; c.ldx = ldx; c.w = (const unsigned*)w; c.ldw = ldw; c.scales = (const bf16*)scales; c.zeros = (const unsigned char*)zeros;
   c.group = group; c.groups = (K - 1) / group + 1; c.out = out; c.ldo = ldo; c.M = M; c.N = N; c.K = K; c.status = status; c.stream = stream;
   if (M <= 16) return out_dtype == SI_BF16 ? w4_few<bf16>(c) : w4_few<float>(c);
-  return -2;
+  return out_dtype == SI_BF16 ? w4_tc<bf16>(c) : w4_tc<float>(c);
 }

@@ -2460,7 +2460,7 @@ def gemm_w4(x, w, scales, zeros, group: int, out, status=None) -> None:
     _need(K > 0, "gemm_w4: rows without entries")
     ldx, ldw = _ld(x), _ld(w)
     if ((x.data_ptr() | w.data_ptr()) % 16 == 0 and ldx % 8 == 0 and ldw % 4 == 0 and K % 32 == 0 and ldx >= K and ldw * 8 >= K
-            and gemm_tc05_available() and M <= 16):
+            and gemm_tc05_available()):
         f = _fn("gemm_w4", "si_gemm_w4", [_c_p, _c_ll, _c_p, _c_ll, _c_p, _c_p, _c_int, _c_p, _c_ll, _c_int, _c_int, _c_int, _c_int, _c_p, _c_p])
         _check(f(_ptr(x), ldx, _ptr(w), ldw, _ptr(scales), _ptr(zeros), group, _ptr(out), _ld(out), od, M, N, K, _ptr(status), _stream()),
                f"gemm_w4(M={M}, N={N}, K={K}, group={group})")
