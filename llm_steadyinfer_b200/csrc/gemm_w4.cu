@@ -1,8 +1,8 @@
 // Product of bf16 rows with 4-bit weights: out[m, n] = sum_k x[m, k] * s[n, k / group] * (q[n, k] - z[n, k / group]), sums fp32, bf16 or fp32
 // output. q lies in int32 words of eight entries (quant_common.cuh); the weights are widened in registers on their way to the tensor cores and
 // never written anywhere in between. Two kernels by the number of rows:
-//   up to 16 rows    a stream of the weights through the fragments of mma.sync; q - z is exact in bf16 there and the scale is applied to the
-//                    fp32 sum of a group, so no weight is rounded
+//   up to 8 rows     a stream of the weights through the fragments of mma.sync; q - z is exact in bf16, and with groups of 128 and more the scale is
+//                    applied to the fp32 sum of a group, so that no weight is rounded
 //   more             tcgen05 the other way round: 128 rows of the weight matrix are the M of the instruction and come to it through tensor memory,
 //                    widened and scaled by the warps that own their lanes; a weight times its scale is rounded to bf16 once (2^-8 of it at
 //                    most: a scale has eight bits and q - z five, and the instruction takes eight)
@@ -11,7 +11,6 @@
 // Before the wait for the kernels before this one nothing is read, the weights are only asked into L2 (see gemm_q8.cu).
 #include "tma_common.cuh"
 #include "quant_common.cuh"
-#include <stdio.h>
 
 typedef __nv_bfloat16 bf16;
 
@@ -20,378 +19,591 @@ struct W4Call {
   void* out; long long ldo; int M, N, K; int* status; cudaStream_t stream;
 };
 
-// ---- up to 16 rows -----------------------------------------------------------------------------------------------
-// mma.sync m16n8k16 with 16 rows of the weight matrix as its "m" and up to 8 rows of x as its "n". Lane (g, t) takes WORDS words (8 * WORDS entries)
-// of rows n0 + g and n0 + g + 8 at k = 32 * WORDS * c + 8 * WORDS * t, and the same entries of row g of x; a word's four pairs are the k columns of two
-// instructions, alike for both operands. A chunk of 32 * WORDS entries lies in one group, so its sums are scaled by the row's number and added
-// to the running ones. A tile is 16 columns; a block's warps take the chunks in turn. U chunks of a warp are on their way at a time: as soon as
-// one is used, the one U further on, of this tile or the next, is asked for.
+// ---- up to 8 rows ------------------------------------------------------------------------------------------------
+// mma.sync m16n8k16 with 16 rows of the weight matrix (a unit) as its "m" and the rows of x as its "n". A block a SM goes through its units; sixteen
+// warps take a piece of 256 entries of the unit's rows each, 4,096 a stage, and their sums of a unit are added in shared memory. All that is not
+// arithmetic is kept away from them: one TMA load brings a stage, [16 pieces][16 rows][128 bytes] (128-byte swizzle), into a ring, four more warps bring
+// the scales (and zero points), and x lies in shared memory in the order of the lanes.
+// Lane (g, t) holds entries 32 t .. 32 t + 31 of a chunk of 128 of rows r(g) and r(g) + 8, r(g) = 4 (g mod 2) + g / 2 (neighbouring g then lie in different
+// halves of the swizzle: no bank conflict), and the same entries of row g of x. A word's four pairs are the k columns of two instructions, alike
+// for both operands. Groups of 128 and more: a chunk lies in one group, its sums are scaled by the row's number and added to the running ones, and
+// no weight is rounded. SMALL (groups of 64 and 32): a lane's entries lie in one group, and a weight times its scale is rounded to bf16 (by 2^-8 of
+// it at most), as with more rows.
+//
+// What bounds it is arithmetic: all but fp32 instructions issue every second clock, and eight weights cost three shifts, four masks and four
+// subtractions. Eight rows of 28,672 x 4,096, us: words and x by loads of the lanes, the next words on their way to registers 27.9 and, with all
+// arithmetic taken out, still 23 (a register that a load is to fill cannot be moved); words by a TMA load of every warp's own, scales by its lanes 28.3,
+// 240 instructions a chunk, 130 of them not the product's.
+//
+// Where x does not fit shared memory, or units are fewer than SMs, a cluster shares the units, each block with its slice of k; the sums of all units
+// wait in shared memory until the cluster meets, and each block adds up and stores every parts-th unit, in the order of the blocks.
+#define W4_FEW_ROWS 8
+#define W4_FEW_WARPS 16
+#define W4_FEW_BRINGERS 4
+#define W4_FEW_THREADS ((W4_FEW_WARPS + W4_FEW_BRINGERS) * 32)
+#define W4_FEW_STAGE (16 * 2048)
+#define W4_FEW_SMEM (208 * 1024)                           // beside it the warps' sums, 16 KB
 __device__ __forceinline__ void w4_mma(float (&d)[4], unsigned a0, unsigned a1, unsigned a2, unsigned a3, unsigned b0, unsigned b1) {
-  asm volatile("mma.sync.aligned.m16n8k16.row.col.f32.bf16.bf16.f32 {%0,%1,%2,%3}, {%4,%5,%6,%7}, {%8,%9}, {%0,%1,%2,%3};\n"
-               : "+f"(d[0]), "+f"(d[1]), "+f"(d[2]), "+f"(d[3]) : "r"(a0), "r"(a1), "r"(a2), "r"(a3), "r"(b0), "r"(b1));
+  asm("mma.sync.aligned.m16n8k16.row.col.f32.bf16.bf16.f32 {%0,%1,%2,%3}, {%4,%5,%6,%7}, {%8,%9}, {%0,%1,%2,%3};\n"
+      : "+f"(d[0]), "+f"(d[1]), "+f"(d[2]), "+f"(d[3]) : "r"(a0), "r"(a1), "r"(a2), "r"(a3), "r"(b0), "r"(b1));
 }
-// WORDS words without a branch: what is not taken becomes zeros. Read once: kept out of L1 where a load takes whole sectors.
-template <int WORDS> __device__ __forceinline__ void w4_ld(const unsigned* p, bool take, unsigned (&v)[WORDS]) {
-  if constexpr (WORDS == 4)
-    asm volatile("{\n\t.reg .pred q;\n\tsetp.ne.s32 q, %5, 0;\n\tmov.u32 %0, 0;\n\tmov.u32 %1, 0;\n\tmov.u32 %2, 0;\n\tmov.u32 %3, 0;\n\t"
-                 "@q ld.global.L1::no_allocate.v4.u32 {%0,%1,%2,%3}, [%4];\n\t}\n"
-                 : "=&r"(v[0]), "=&r"(v[1]), "=&r"(v[2]), "=&r"(v[3]) : "l"(p), "r"((int)take) : "memory");
-  else if constexpr (WORDS == 2)
-    asm volatile("{\n\t.reg .pred q;\n\tsetp.ne.s32 q, %3, 0;\n\tmov.u32 %0, 0;\n\tmov.u32 %1, 0;\n\t@q ld.global.v2.u32 {%0,%1}, [%2];\n\t}\n"
-                 : "=&r"(v[0]), "=&r"(v[1]) : "l"(p), "r"((int)take) : "memory");
-  else
-    asm volatile("{\n\t.reg .pred q;\n\tsetp.ne.s32 q, %2, 0;\n\tmov.u32 %0, 0;\n\t@q ld.global.u32 %0, [%1];\n\t}\n"
-                 : "=&r"(v[0]) : "l"(p), "r"((int)take) : "memory");
-}
-__device__ __forceinline__ uint4 w4_ld_x(const bf16* p, bool take) {
+// Loads of what the kernels before may have written: not by the read-only path, whose loads may be moved across the wait for them.
+__device__ __forceinline__ uint4 w4_ld_x(const bf16* p) {
   uint4 v;
-  asm volatile("{\n\t.reg .pred q;\n\tsetp.ne.s32 q, %5, 0;\n\tmov.u32 %0, 0;\n\tmov.u32 %1, 0;\n\tmov.u32 %2, 0;\n\tmov.u32 %3, 0;\n\t"
-               "@q ld.global.v4.u32 {%0,%1,%2,%3}, [%4];\n\t}\n"
-               : "=&r"(v.x), "=&r"(v.y), "=&r"(v.z), "=&r"(v.w) : "l"(p), "r"((int)take) : "memory");
+  asm volatile("ld.global.v4.u32 {%0,%1,%2,%3}, [%4];\n" : "=r"(v.x), "=r"(v.y), "=r"(v.z), "=r"(v.w) : "l"(p) : "memory");
   return v;
 }
-
-// A scale or a zero point, not by the read-only path: such a load may be moved across the wait for the kernel that writes it.
-__device__ __forceinline__ unsigned w4_ld_scale(const bf16* p, bool take) {
+__device__ __forceinline__ unsigned w4_ld_scale(const bf16* p) {
+  unsigned short v;
+  asm volatile("ld.global.u16 %0, [%1];\n" : "=h"(v) : "l"(p) : "memory");
+  return v;
+}
+__device__ __forceinline__ unsigned w4_ld_zero(const unsigned char* p) {
   unsigned v;
-  asm volatile("{\n\t.reg .pred q;\n\t.reg .u16 h;\n\tsetp.ne.s32 q, %2, 0;\n\tmov.u16 h, 0;\n\t@q ld.global.u16 h, [%1];\n\tcvt.u32.u16 %0, h;\n\t}\n"
-               : "=r"(v) : "l"(p), "r"((int)take) : "memory");
+  asm volatile("ld.global.u8 %0, [%1];\n" : "=r"(v) : "l"(p) : "memory");
   return v;
 }
-__device__ __forceinline__ unsigned w4_ld_zero(const unsigned char* p, bool take) {
-  unsigned v;
-  asm volatile("{\n\t.reg .pred q;\n\tsetp.ne.s32 q, %2, 0;\n\tmov.u32 %0, 0;\n\t@q ld.global.u8 %0, [%1];\n\t}\n" : "=&r"(v) : "l"(p), "r"((int)take) : "memory");
+__device__ __forceinline__ float w4_ld_cluster1(unsigned cluster_addr) {
+  float v;
+  asm volatile("ld.shared::cluster.f32 %0, [%1];\n" : "=f"(v) : "r"(cluster_addr) : "memory");
   return v;
 }
+// The first 1,024-byte boundary of dynamic shared memory. (Not by rounding the pointer itself, of which the compiler then no longer knows that it leads to
+// shared memory.)
+__device__ __forceinline__ unsigned char* w4_smem_base(unsigned char* smem) { return smem + ((1024u - (tma_smem_u32(smem) & 1023u)) & 1023u); }
+// A wait that all lanes of a warp make, with one answer.
+__device__ __forceinline__ bool w4_wait(uint64_t* bar, unsigned parity) { return __all_sync(0xffffffffu, mbar_wait(bar, parity)); }
 
-template <int MT, int WARPS, int U, int WORDS, bool ZEROS, typename TO>
-__global__ void __launch_bounds__(WARPS * 32, 512 / (WARPS * 32))
-gemm_w4_skinny_kernel(const bf16* __restrict__ x, long long ldx, const unsigned* __restrict__ w, long long ldw, const bf16* __restrict__ scales,
-                      const unsigned char* __restrict__ zeros, int group, int groups, TO* __restrict__ out, long long ldo, int M, int N, int K,
-                      int tiles, int trigger) {
-  constexpr int CHUNK = 32 * WORDS;
-  __shared__ float red[2][WARPS * MT * 32][4];
+// Scales a row and stage as they lie in shared memory: one a chunk of 128, or (SMALL) one a piece of 32.
+__host__ __device__ constexpr int w4_few_scales(bool small) { return small ? 128 : 32; }
+__host__ __device__ constexpr int w4_few_stages(bool small) { return small ? 3 : 4; }
+__host__ __device__ constexpr int w4_few_stage_bytes(bool zeros, bool small) { return W4_FEW_STAGE + 16 * w4_few_scales(small) * (zeros ? 3 : 2); }
+
+template <bool ZEROS, bool SMALL, typename TO>
+__global__ void __launch_bounds__(W4_FEW_THREADS, 1)
+gemm_w4_few_kernel(const __grid_constant__ CUtensorMap wmap, const bf16* __restrict__ x, long long ldx, const bf16* __restrict__ scales,
+                   const unsigned char* __restrict__ zeros, int group, int groups, TO* __restrict__ out, long long ldo, int M, int N, int K, int slice,
+                   int pieces, int parts, int units, int* status, int trigger) {
+  constexpr int STAGES = w4_few_stages(SMALL), SC = w4_few_scales(SMALL);
+  extern __shared__ unsigned char smem_dyn[];
+  __shared__ float red[2][W4_FEW_WARPS][128];
+  __shared__ __align__(8) uint64_t full_bar[STAGES], empty_bar[STAGES];
+  const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
+  unsigned char* ring = w4_smem_base(smem_dyn);
+  unsigned short* sring = reinterpret_cast<unsigned short*>(ring + STAGES * W4_FEW_STAGE);     // [stage][16 rows][SC]
+  unsigned char* zring = reinterpret_cast<unsigned char*>(sring + STAGES * 16 * SC);           // likewise
+  uint4* xs = reinterpret_cast<uint4*>(ring + STAGES * w4_few_stage_bytes(ZEROS, SMALL));       // [chunk][4][M rows][t]
+  float* sums = reinterpret_cast<float*>(xs + slice / 128 * 16 * M);                          // [unit][128], only where a cluster meets
+  const int part = (int)cluster_cta_rank(), first = blockIdx.x / parts, stride = gridDim.x / parts;
+  const int k_begin = part * slice, boxes = (min(K, k_begin + slice) - k_begin) / 256;         // K and slices are multiples of 256, none empty
+  const int mine = (units - first + stride - 1) / stride, rounds = (boxes + 15) / 16;          // units of this block (first < units), stages a unit
   if (trigger) pdl_trigger();
-  const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31, g = lane >> 2, t = lane & 3;
-  const int per_tile = ((K + CHUNK - 1) / CHUNK + WARPS - 1) / WARPS;          // chunks of a warp a tile, the last ones perhaps empty
-  const int per_group = group / CHUNK;
-  struct Slot { unsigned lo[WORDS], hi[WORDS], slo, shi, zlo, zhi; } slot[U];
-  int tile = blockIdx.x, i = 0;                                                // what is asked for next: chunk i of this warp in the tile
-  auto fetch = [&](Slot& s) {
-    const int c = warp + i * WARPS, k = c * CHUNK + t * 8 * WORDS;
-    const int n0 = tile * 16 + g < N ? tile * 16 + g : 0, n1 = tile * 16 + 8 + g < N ? tile * 16 + 8 + g : 0;   // rows beyond N stand for row 0
-    const bool take = tile < tiles && k < K;
-    w4_ld<WORDS>(w + (size_t)n0 * ldw + k / 8, take, s.lo);
-    w4_ld<WORDS>(w + (size_t)n1 * ldw + k / 8, take, s.hi);
-    const bool some = tile < tiles && c * CHUNK < K;
-    const int at = some ? c / per_group : 0;
-    const size_t a0 = (size_t)n0 * groups + at, a1 = (size_t)n1 * groups + at;
-    s.slo = w4_ld_scale(scales + a0, some);
-    s.shi = w4_ld_scale(scales + a1, some);
-    if (ZEROS) { s.zlo = w4_ld_zero(zeros + a0, some); s.zhi = w4_ld_zero(zeros + a1, some); }
-    if (++i == per_tile) { i = 0; tile += gridDim.x; }
-  };
-  for (int u = 0; u < U && u < per_tile; ++u) {                               // the first chunks' lines into L2: half a warp a lane, a row each
-    const int n = tile * 16 + (lane & 15), k = (warp + u * WARPS) * CHUNK;
-    if (lane < 16 && n < N && k < K) asm volatile("prefetch.global.L2 [%0];\n" ::"l"(w + (size_t)n * ldw + k / 8) : "memory");
+  if (threadIdx.x == 0) {
+#pragma unroll
+    for (int s = 0; s < STAGES; ++s) { mbar_init(&full_bar[s], 1 + W4_FEW_BRINGERS); mbar_init(&empty_bar[s], W4_FEW_WARPS); }
+    asm volatile("fence.mbarrier_init.release.cluster;\n" ::: "memory");
   }
-  pdl_wait();
+  __syncthreads();
+  bool ok = true;
+  if (warp >= W4_FEW_WARPS) {
+    const int b = warp - W4_FEW_WARPS;                      // brings the scales of rows 4 b .. 4 b + 3; the first of them the words as well
+    if (b == 0 && lane == 0)
+      asm volatile("cp.async.bulk.prefetch.tensor.3d.L2.global.tile [%0, {%1, %2, %3}];\n" ::"l"(&wmap), "r"(0), "r"(first * 16), "r"(k_begin / 256) : "memory");
+    pdl_wait();
+    constexpr int PER = 4 * SC / 32;                        // scales a lane and stage
+    const int row = 4 * b + lane / 8, c0 = lane % 8;         // eight lanes a row
+    int s = 0, issued = 0;
+    unsigned phase = 1;
+    for (int unit = 0; unit < mine && ok; ++unit) {
+      const int n = (first + unit * stride) * 16 + row;
+      const size_t r = (size_t)(n < N ? n : 0) * groups;       // rows beyond N: words are zeros, nothing is stored
+      for (int rd = 0; rd < rounds; ++rd, ++issued) {
+        unsigned sv[PER], zv[PER];
 #pragma unroll
-  for (int u = 0; u < U; ++u) fetch(slot[u]);
-  float acc[MT][4];
-#pragma unroll
-  for (int mt = 0; mt < MT; ++mt) acc[mt][0] = acc[mt][1] = acc[mt][2] = acc[mt][3] = 0.f;
-  int now = blockIdx.x, j = 0, par = 0;                                        // what is used next: chunk j of this warp in tile `now`
-  while (now < tiles) {
-#pragma unroll
-    for (int u = 0; u < U; ++u) {
-      if (now >= tiles) break;                                                 // alike for all warps of the block
-      const int k = (warp + j * WARPS) * CHUNK + t * 8 * WORDS;
-      Slot& s = slot[u];
-      const __nv_bfloat162 blo = ZEROS ? w4_bias((int)s.zlo) : __float2bfloat162_rn(136.f), bhi = ZEROS ? w4_bias((int)s.zhi) : __float2bfloat162_rn(136.f);
-      float part[MT][4];
-#pragma unroll
-      for (int mt = 0; mt < MT; ++mt) part[mt][0] = part[mt][1] = part[mt][2] = part[mt][3] = 0.f;
-#pragma unroll
-      for (int q = 0; q < WORDS; ++q) {
-        uint4 xv[MT];
-#pragma unroll
-        for (int mt = 0; mt < MT; ++mt) {
-          const bool in = mt * 8 + g < M;
-          xv[mt] = w4_ld_x(x + (size_t)(in ? mt * 8 + g : 0) * ldx + k + 8 * q, in && k + 8 * q < K);
+        for (int i = 0; i < PER; ++i) {                       // asked for before the stage is free
+          const int e = k_begin + rd * 4096 + (c0 + 8 * i) * (4096 / SC);
+          const int at = min(e / group, groups - 1);
+          sv[i] = w4_ld_scale(scales + r + at);
+          if (ZEROS) zv[i] = w4_ld_zero(zeros + r + at);
         }
-        unsigned a[4], b[4];
-#pragma unroll
-        for (int p = 0; p < 4; ++p) { a[p] = w4_pair(s.lo[q], p, blo); b[p] = w4_pair(s.hi[q], p, bhi); }
-#pragma unroll
-        for (int mt = 0; mt < MT; ++mt) {
-          w4_mma(part[mt], a[0], b[0], a[1], b[1], xv[mt].x, xv[mt].y);
-          w4_mma(part[mt], a[2], b[2], a[3], b[3], xv[mt].z, xv[mt].w);
+        if (issued >= STAGES) ok = w4_wait(&empty_bar[s], phase);
+        if (!ok) {
+          if (lane == 0) set_status(status, SI_WAIT_LIMIT);
+          break;
         }
-      }
-      const float slo = __uint_as_float(s.slo << 16), shi = __uint_as_float(s.shi << 16);
-#pragma unroll
-      for (int mt = 0; mt < MT; ++mt) {
-        acc[mt][0] += slo * part[mt][0]; acc[mt][1] += slo * part[mt][1];
-        acc[mt][2] += shi * part[mt][2]; acc[mt][3] += shi * part[mt][3];
-      }
-      fetch(s);
-      if (++j == per_tile) {                                                   // the tile is through: the warps' sums, added in warp order
-        j = 0;
-#pragma unroll
-        for (int mt = 0; mt < MT; ++mt) {
-          *reinterpret_cast<float4*>(red[par][(warp * MT + mt) * 32 + lane]) = make_float4(acc[mt][0], acc[mt][1], acc[mt][2], acc[mt][3]);
-          acc[mt][0] = acc[mt][1] = acc[mt][2] = acc[mt][3] = 0.f;
+        if (b == 0 && lane == 0) {
+          mbar_expect_tx(&full_bar[s], (unsigned)pieces * 2048u);
+          tma_load_3d(ring + s * W4_FEW_STAGE, &wmap, &full_bar[s], 0, (first + unit * stride) * 16, k_begin / 256 + rd * 16);
         }
-        __syncthreads();                       // one barrier a tile: a buffer is written again two tiles later, behind the next tile's barrier
-        for (int idx = threadIdx.x; idx < MT * 128; idx += WARPS * 32) {
-          const int mt = idx / 128, ln = (idx >> 2) & 31, e = idx & 3;
-          float sum = 0.f;
 #pragma unroll
-          for (int v = 0; v < WARPS; ++v) sum += red[par][(v * MT + mt) * 32 + ln][e];
-          const int n = now * 16 + (ln >> 2) + ((e >> 1) ? 8 : 0), m = mt * 8 + (ln & 3) * 2 + (e & 1);
-          if (n < N && m < M) out[(size_t)m * ldo + n] = from_f32<TO>(sum);
+        for (int i = 0; i < PER; ++i) {
+          sring[(s * 16 + row) * SC + c0 + 8 * i] = (unsigned short)sv[i];
+          if (ZEROS) zring[(s * 16 + row) * SC + c0 + 8 * i] = (unsigned char)zv[i];
         }
-        par ^= 1;
-        now += gridDim.x;
+        __syncwarp();
+        if (lane == 0) mbar_arrive(&full_bar[s]);
+        if (++s == STAGES) { s = 0; phase ^= 1u; }
       }
     }
+    if (!ok && b == 0 && lane == 0)                           // the copies still under way, with a limit again
+      for (int i = issued > STAGES ? issued - STAGES : 0; i < issued; ++i) mbar_wait(&full_bar[i % STAGES], (unsigned)((i / STAGES) & 1));
+  } else {
+    const int g = lane >> 2, t = lane & 3, row = (g & 1) * 4 + (g >> 1);
+    pdl_wait();
+    for (int i = threadIdx.x; i < boxes * 8 * M; i += W4_FEW_WARPS * 32) {    // x: a thread takes a lane's 32 entries of a chunk
+      const int tt = i & 3, m = (i >> 2) % M, ch = (i >> 2) / M;
+      const bf16* from = x + (size_t)m * ldx + k_begin + ch * 128 + tt * 32;
+#pragma unroll
+      for (int q = 0; q < 4; ++q) xs[((ch * 4 + q) * M + m) * 4 + tt] = w4_ld_x(from + 8 * q);
+    }
+    asm volatile("bar.sync 1, %0;\n" ::"n"(W4_FEW_WARPS * 32) : "memory");
+    const uint4* xl = xs + (g < M ? g : 0) * 4 + t;           // a lane of a row of x that is not there takes row 0's: nothing of it is stored
+    const int x_step = 4 * M;                                 // from a word's entries to the next word's
+    const unsigned char* wl = ring + warp * 2048 + row * 128;
+    const int off[2] = {(t ^ row) << 4, ((4 + t) ^ row) << 4};
+    const int se = row * SC + (SMALL ? warp * 8 + t : warp * 2);      // this lane's scales of a stage: chunk h's 4 h (SMALL) or h further
+    float acc[4] = {0.f, 0.f, 0.f, 0.f};
+    int s = 0, par = 0;
+    unsigned phase = 0;
+#pragma unroll 1
+    for (int unit = 0; unit < mine; ++unit) {
+#pragma unroll 1
+      for (int rd = 0; rd < rounds; ++rd) {
+        if (ok) ok = w4_wait(&full_bar[s], phase);
+        const int bx = rd * 16 + warp;
+        if (bx < boxes) {                                     // alike for the warp
+          const unsigned char* box = wl + s * W4_FEW_STAGE;
+          const uint4* xb = xl + bx * 8 * x_step;
+          const unsigned short* sp = sring + s * 16 * SC + se;
+          const unsigned char* zp = zring + s * 16 * SC + se;
+#pragma unroll
+          for (int h = 0; h < 2; ++h) {
+            const int sh = SMALL ? 4 * h : h;
+            const uint4 lo = *reinterpret_cast<const uint4*>(box + off[h]), hi = *reinterpret_cast<const uint4*>(box + 1024 + off[h]);
+            const unsigned slo = sp[sh], shi = sp[8 * SC + sh];
+            const __nv_bfloat162 blo = ZEROS ? w4_bias((int)zp[sh]) : __float2bfloat162_rn(136.f);
+            const __nv_bfloat162 bhi = ZEROS ? w4_bias((int)zp[8 * SC + sh]) : __float2bfloat162_rn(136.f);
+            const unsigned lw[4] = {lo.x, lo.y, lo.z, lo.w}, hw[4] = {hi.x, hi.y, hi.z, hi.w};
+            const unsigned s0w = slo | (slo << 16), s1w = shi | (shi << 16);
+            float part0[4] = {0.f, 0.f, 0.f, 0.f};
+#pragma unroll
+            for (int q = 0; q < 4; ++q) {
+              const uint4 xv = xb[(h * 4 + q) * x_step];
+              unsigned a[4], c[4];
+#pragma unroll
+              for (int p = 0; p < 4; ++p) {
+                a[p] = w4_pair(lw[q], p, blo);
+                c[p] = w4_pair(hw[q], p, bhi);
+                if (SMALL) {
+                  const __nv_bfloat162 ra = __hmul2(*reinterpret_cast<__nv_bfloat162*>(&a[p]), *reinterpret_cast<const __nv_bfloat162*>(&s0w));
+                  const __nv_bfloat162 rc = __hmul2(*reinterpret_cast<__nv_bfloat162*>(&c[p]), *reinterpret_cast<const __nv_bfloat162*>(&s1w));
+                  a[p] = *reinterpret_cast<const unsigned*>(&ra);
+                  c[p] = *reinterpret_cast<const unsigned*>(&rc);
+                }
+              }
+              float (&to)[4] = SMALL ? acc : part0;
+              w4_mma(to, a[0], c[0], a[1], c[1], xv.x, xv.y);
+              w4_mma(to, a[2], c[2], a[3], c[3], xv.z, xv.w);
+            }
+            if (!SMALL) {
+              const float s0 = __uint_as_float(slo << 16), s1 = __uint_as_float(shi << 16);
+              acc[0] += s0 * part0[0]; acc[1] += s0 * part0[1];
+              acc[2] += s1 * part0[2]; acc[3] += s1 * part0[3];
+            }
+          }
+        }
+        __syncwarp();                                         // all lanes have read the stage
+        if (lane == 0) mbar_arrive(&empty_bar[s]);
+        if (++s == STAGES) { s = 0; phase ^= 1u; }
+      }
+      *reinterpret_cast<float4*>(&red[par][warp][lane * 4]) = make_float4(acc[0], acc[1], acc[2], acc[3]);
+      acc[0] = acc[1] = acc[2] = acc[3] = 0.f;
+      // one barrier (of these warps) a unit: a buffer is written again two units later, behind the next unit's barrier
+      asm volatile("bar.sync 1, %0;\n" ::"n"(W4_FEW_WARPS * 32) : "memory");
+      // four lanes an output, each a quarter of the warps in order
+      const int e = threadIdx.x >> 2, v0 = (threadIdx.x & 3) * (W4_FEW_WARPS / 4);
+      float sum = 0.f;
+#pragma unroll
+      for (int v = 0; v < W4_FEW_WARPS / 4; ++v) sum += red[par][v0 + v][e];
+      sum += __shfl_xor_sync(0xffffffffu, sum, 1);
+      sum += __shfl_xor_sync(0xffffffffu, sum, 2);
+      if ((threadIdx.x & 3) == 0) {
+        if (parts > 1) {
+          sums[unit * 128 + e] = sum;
+        } else {
+          const int ln = e >> 2, gg = ln >> 2, m = (ln & 3) * 2 + (e & 1), n = (first + unit * stride) * 16 + (gg & 1) * 4 + (gg >> 1) + ((e >> 1) & 1) * 8;
+          if (n < N && m < M && ok) out[(size_t)m * ldo + n] = from_f32<TO>(sum);
+        }
+      }
+      par ^= 1;
+    }
+    if (!ok && lane == 0) set_status(status, SI_WAIT_LIMIT);
+  }
+  __syncwarp();
+  if (parts > 1) {
+    cluster_sync_all();                                       // every block's sums of its slice lie in its shared memory
+    for (int u = part; u < mine; u += parts)
+      if (threadIdx.x < 128) {
+        const int e = threadIdx.x;
+        float v[8];
+#pragma unroll
+        for (int p = 0; p < 8; ++p) v[p] = p < parts ? w4_ld_cluster1(cluster_map_u32(sums + u * 128 + e, (unsigned)p)) : 0.f;
+#pragma unroll
+        for (int p = 1; p < 8; ++p) v[0] += v[p];
+        const int ln = e >> 2, gg = ln >> 2, m = (ln & 3) * 2 + (e & 1), n = (first + u * stride) * 16 + (gg & 1) * 4 + (gg >> 1) + ((e >> 1) & 1) * 8;
+        if (n < N && m < M && ok) out[(size_t)m * ldo + n] = from_f32<TO>(v[0]);
+      }
+    cluster_sync_all();                                       // no block goes while another one reads its sums
   }
 }
 
-template <int WORDS, bool ZEROS, typename TO>
-static int w4_skinny(const W4Call& c) {
-  const long long sms = si_sm_count(), tiles = (c.N + 15) / 16;
-  int warps = 8;
-  if (const char* e = getenv("W4_WARPS")) warps = atoi(e);
-  const long long slots = 512 / (warps * 32) * sms;
-  const dim3 grid((unsigned)(tiles > slots ? slots : tiles)), block(warps * 32);
-  const int trig = si_pdl_trigger_mode(grid.x, slots);
-  constexpr int U1 = WORDS == 4 ? 4 : 8, U2 = WORDS == 4 ? 3 : 6;
-#define W4_SK(MT, WARPS, U) si_launch(gemm_w4_skinny_kernel<MT, WARPS, U, WORDS, ZEROS, TO>, grid, block, 0, c.stream, c.x, c.ldx, c.w, c.ldw, c.scales, \
-                                      c.zeros, c.group, c.groups, (TO*)c.out, c.ldo, c.M, c.N, c.K, (int)tiles, trig)
-  if (c.M > 8) { if (warps == 4) W4_SK(2, 4, U2); else W4_SK(2, 8, U2); }
-  else if (warps == 4) W4_SK(1, 4, U1); else W4_SK(1, 8, U1);
-#undef W4_SK
+// How k is cut for `units` units: blocks of a cluster, a block's slice, clusters, dynamic shared memory. False where it does not fit.
+static int w4_clusters(int size);
+struct W4Few { int parts, slice, clusters; size_t smem; };
+static bool w4_few_shape(int M, int N, int K, bool zeros, bool small, W4Few* f) {
+  if (M > W4_FEW_ROWS || K % 256) return false;
+  const int units = (N + 15) / 16, boxes = K / 256;
+  for (int parts = 1; parts <= 8; parts *= 2) {
+    const int per = (boxes + parts - 1) / parts;
+    if ((long long)per * (parts - 1) >= boxes) return false;                                  // a block without a piece
+    const int slots = w4_clusters(parts);
+    f->parts = parts;
+    f->slice = per * 256;
+    f->clusters = units < slots ? units : slots;
+    const size_t sum_bytes = parts > 1 ? (size_t)((units + f->clusters - 1) / f->clusters) * 512 : 0;
+    f->smem = (size_t)w4_few_stages(small) * w4_few_stage_bytes(zeros, small) + (size_t)per * 512 * M + sum_bytes + 1024;
+    const bool more = 2 * units * parts <= si_sm_count() && per >= 2 * W4_FEW_WARPS;          // half of the SMs idle, and pieces enough to share
+    if (f->smem <= W4_FEW_SMEM && !(more && parts < 8)) return true;
+  }
+  return false;
+}
+
+static int w4_encode(CUtensorMap* map, CUtensorMapDataType type, int size, const void* base, long long rows, long long cols, long long ld, unsigned box_cols,
+                     unsigned box_rows, CUtensorMapSwizzle swizzle) {
+  SiEncodeTiledFn fn = si_encode_fn();
+  if (!fn) return -3;
+  const cuuint64_t dims[2] = {(cuuint64_t)cols, (cuuint64_t)rows};
+  const cuuint64_t strides[1] = {(cuuint64_t)(ld * size)};
+  const cuuint32_t box[2] = {box_cols, box_rows};
+  const cuuint32_t estr[2] = {1, 1};
+  CUresult r = fn(map, type, 2, const_cast<void*>(base), dims, strides, box, estr, CU_TENSOR_MAP_INTERLEAVE_NONE, swizzle,
+                  CU_TENSOR_MAP_L2_PROMOTION_L2_128B, CU_TENSOR_MAP_FLOAT_OOB_FILL_NONE);
+  return r == CUDA_SUCCESS ? 0 : 1000 + (int)r;
+}
+// The words [rows, pieces of 128 bytes] as (word of a piece, row, piece), boxes of [box_pieces, 16 rows, 128 bytes].
+static int w4_encode_pieces(CUtensorMap* map, const void* base, long long rows, int pieces, long long ld, int box_pieces) {
+  SiEncodeTiledFn fn = si_encode_fn();
+  if (!fn) return -3;
+  const cuuint64_t dims[3] = {32, (cuuint64_t)rows, (cuuint64_t)pieces};
+  const cuuint64_t strides[2] = {(cuuint64_t)(ld * 4), 128};
+  const cuuint32_t box[3] = {32, 16, (cuuint32_t)box_pieces};
+  const cuuint32_t estr[3] = {1, 1, 1};
+  CUresult r = fn(map, CU_TENSOR_MAP_DATA_TYPE_INT32, 3, const_cast<void*>(base), dims, strides, box, estr, CU_TENSOR_MAP_INTERLEAVE_NONE,
+                  CU_TENSOR_MAP_SWIZZLE_128B, CU_TENSOR_MAP_L2_PROMOTION_L2_128B, CU_TENSOR_MAP_FLOAT_OOB_FILL_NONE);
+  return r == CUDA_SUCCESS ? 0 : 1000 + (int)r;
+}
+
+template <bool ZEROS, bool SMALL, typename TO>
+static int w4_few_launch(const W4Call& c, const W4Few& f) {
+  auto k = gemm_w4_few_kernel<ZEROS, SMALL, TO>;
+  cudaError_t e = cudaFuncSetAttribute(k, cudaFuncAttributeMaxDynamicSharedMemorySize, W4_FEW_SMEM);
+  if (e != cudaSuccess) return (int)e;
+  const int pieces = f.slice / 256 < 16 ? f.slice / 256 : 16;
+  CUtensorMap wm;
+  const int rc = w4_encode_pieces(&wm, c.w, c.N, c.K / 256, c.ldw, pieces);
+  if (rc) return rc;
+  const int blocks = f.clusters * f.parts;
+  cudaLaunchConfig_t cfg = {};
+  cfg.gridDim = dim3((unsigned)blocks);
+  cfg.blockDim = dim3(W4_FEW_THREADS);
+  cfg.dynamicSmemBytes = f.smem;
+  cfg.stream = c.stream;
+  cudaLaunchAttribute attr[2];
+  attr[0].id = cudaLaunchAttributeClusterDimension;
+  attr[0].val.clusterDim.x = (unsigned)f.parts;
+  attr[0].val.clusterDim.y = 1;
+  attr[0].val.clusterDim.z = 1;
+  attr[1].id = cudaLaunchAttributeProgrammaticStreamSerialization;
+  attr[1].val.programmaticStreamSerializationAllowed = 1;
+  cfg.attrs = attr;
+  cfg.numAttrs = si_pdl_enabled() ? 2 : 1;
+  cudaLaunchKernelEx(&cfg, k, wm, c.x, c.ldx, c.scales, c.zeros, c.group, c.groups, (TO*)c.out, c.ldo, c.M, c.N, c.K, f.slice, pieces, f.parts,
+                     (c.N + 15) / 16, c.status, si_pdl_trigger_mode(blocks, si_sm_count()));
   return si_last_error();
 }
 
 template <typename TO>
-static int w4_few(const W4Call& c) {
-  if (c.group % 128 == 0) return c.zeros ? w4_skinny<4, true, TO>(c) : w4_skinny<4, false, TO>(c);
-  if (c.group == 64) return c.zeros ? w4_skinny<2, true, TO>(c) : w4_skinny<2, false, TO>(c);
-  return c.zeros ? w4_skinny<1, true, TO>(c) : w4_skinny<1, false, TO>(c);
+static int w4_few(const W4Call& c, const W4Few& f) {
+  if (c.group < 128) return c.zeros ? w4_few_launch<true, true, TO>(c, f) : w4_few_launch<false, true, TO>(c, f);
+  return c.zeros ? w4_few_launch<true, false, TO>(c, f) : w4_few_launch<false, false, TO>(c, f);
 }
 
-// ---- more than 16 rows -------------------------------------------------------------------------------------------
-// out transposed: a tile is HALVES x 128 rows of the weight matrix (the M of the instruction) by `bn` rows of x (its N, a multiple of 16), k steps
-// of 128. Warp 0 fetches x (two boxes of 64 entries a step, 128-byte swizzle), warp 1 the words (rows of 64 bytes, 64-byte swizzle), both into one
-// ring. Warps 8 to 15 widen: a thread owns one row of the weight matrix, takes its 64 bytes of a step out of shared memory (the swizzle spreads
-// eight rows over all banks), makes the 128 entries bf16 in registers and writes them to its lane of tensor memory, from where the instruction reads
-// its A: the widened weights cost neither bandwidth nor room in shared memory. Two groups of four warps take the steps in turn (HALVES 1) or a
-// half of the rows each (HALVES 2, for few rows of x, where a step's instructions are short and its fixed cost counts). Warp 2 issues; warps
-// 4 to 7 store. Tensor memory: with bn up to 192 two accumulators and two A buffers, beyond one and four (HALVES 2: up to 64 two, else one, and
-// two A buffers a half). Blocks are persistent, one an SM; with few tiles the k range of a tile is cut over a cluster, whose blocks leave their
-// sums in shared memory and add a part of the rows each up over all blocks, in their order.
-#define W4_TC_SMEM (224 * 1024)
-#define W4_TC_MAX_STAGES 8
+// ---- more than 8 rows --------------------------------------------------------------------------------------------
+// out transposed: a tile is 128 rows of the weight matrix a CTA (the M of the instruction) by `bn` rows of x (its N, a multiple of 16), k steps of 128.
+// Four slots go round; to a slot belong 8 KB of words, the step's part of x, and 64 columns of tensor memory for the widened weights. Warp 0 fetches
+// x (two boxes of 64 entries, 128-byte swizzle), warp 1 the words (rows of 64 bytes, 64-byte swizzle). Warps 8 to 23 widen, four a slot, so that four
+// steps are in the making at once (all but fp32 arithmetic issues every second clock, and one warp a scheduler left more than half of those empty:
+// with eight warps a step took 1,000 clocks): a thread owns one row of the weight matrix, takes its 64 bytes out of shared memory (the swizzle spreads eight rows over all
+// banks), makes the 128 entries bf16 in registers and writes them to its lane of tensor memory, where the instruction reads its A: the widened weights
+// cost neither bandwidth nor room in shared memory. Warp 2 issues, eight instructions a step; warps 4 to 7 store. Up to 128 rows of x there are two
+// accumulators of 128 columns, beyond one of 256.
+//
+// PAIR: two CTAs (a cluster) on a tile of 256 rows of the weight matrix, each with its 128 in its own tensor memory and half of the tile's rows of x; the
+// leader's instructions (cta_group::2) read both. With many rows x is what bounds a CTA alone: it takes in bn * 256 bytes of it for every 8 KB of
+// words, and an SM was seen to take in 50 to 80 GB/s (937 x 4,096 x 14,336: 97 us alone).
+//
+// A wait costs the issuing warp 100 to 350 clocks even where there is nothing to wait for, and a commit not less than that, so there is one of each
+// a step: `ready` of a slot counts the bytes of x and the warps that widened (the leader's counts both CTAs'), and the one commit on `empty` gives back
+// all that belongs to the slot. The words' own barrier comes only after that, so the widening warps wait for it alone.
+//
+// Blocks are persistent, one an SM. Without PAIR the k range of a tile may be cut over a cluster, whose blocks leave their sums in shared memory and
+// add a part of the rows each up over all blocks, in their order.
+#define W4_SLOTS 4
+#define W4_THREADS ((8 + 4 * W4_SLOTS) * 32)
+#define W4_TC_SMEM (W4_SLOTS * (128 * 64 + 128 * 256))      // with 128 rows of x a CTA at most
 
-__host__ __device__ inline int w4_tc_stage_bytes(int halves, int bn) { return halves * 128 * 64 + bn * 256; }
-__host__ __device__ inline int w4_tc_stages(int halves, int bn) {
-  const int n = W4_TC_SMEM / w4_tc_stage_bytes(halves, bn);
-  return n < W4_TC_MAX_STAGES ? n : W4_TC_MAX_STAGES;
-}
 __device__ __forceinline__ float4 w4_ld_cluster(unsigned cluster_addr) {
   float4 v;
   asm volatile("ld.shared::cluster.v4.f32 {%0,%1,%2,%3}, [%4];\n" : "=f"(v.x), "=f"(v.y), "=f"(v.z), "=f"(v.w) : "r"(cluster_addr) : "memory");
   return v;
 }
-__device__ __forceinline__ void w4_drain(uint64_t* full, int stages, int issued) {       // as drain_copies in gemm_q8.cu
-  for (int i = issued > stages ? issued - stages : 0; i < issued; ++i) mbar_wait(&full[i % stages], (unsigned)((i / stages) & 1));
+__device__ __forceinline__ void w4_mma_pair_tmem_a(unsigned d, unsigned a, unsigned long long b_desc, unsigned idesc, unsigned accumulate) {
+  asm volatile("{\n.reg .pred p;\nsetp.ne.b32 p, %4, 0;\ntcgen05.mma.cta_group::2.kind::f16 [%0], [%1], %2, %3, p;\n}\n"
+               ::"r"(d), "r"(a), "l"(b_desc), "r"(idesc), "r"(accumulate) : "memory");
+}
+// An arrival at the leader's barrier. What it orders lies in tensor memory, which the tcgen05 fences on both sides see to, so it is a relaxed one: a
+// release to the cluster waits for everything the warp has under way (the scales asked for ahead among it) and took 1,000 to 1,700 clocks a step.
+__device__ __forceinline__ void w4_arrive_leader(uint64_t* bar) {
+  asm volatile("mbarrier.arrive.relaxed.cluster.shared::cluster.b64 _, [%0];\n" ::"r"(cluster_map_u32(bar, 0)) : "memory");
+}
+// After a wait that ran out: the copies still under way are waited for, with a limit again, before the block's shared memory goes.
+__device__ __forceinline__ void w4_drain(uint64_t* full, int issued) {
+  for (int i = issued > W4_SLOTS ? issued - W4_SLOTS : 0; i < issued; ++i) mbar_wait(&full[i % W4_SLOTS], (unsigned)((i / W4_SLOTS) & 1));
 }
 
-template <int HALVES, bool ZEROS, typename TO>
-__global__ void __launch_bounds__(512, 1)
+// The scales and zero points of one row of the weight matrix along its steps of 128 entries: those of a step are asked for ahead, when the
+// caller's step before it is done with. Groups of 128 and more: one of each a step, the group counted along; SMALL (64 and 32): one a piece of 32 entries.
+template <bool ZEROS, bool SMALL> struct W4Scales {
+  static constexpr int N = SMALL ? 4 : 1;
+  const bf16* s; const unsigned char* z;
+  int last, span, at, rem;              // last group; SMALL: groups a step, else steps a group; group of the next step, and its place in it
+  unsigned sv[N], zv[N];
+  __device__ __forceinline__ void start(const bf16* scales, const unsigned char* zeros, long long row, int group, int groups, int step) {
+    last = groups - 1;
+    s = scales + row * groups;
+    z = ZEROS ? zeros + row * groups : nullptr;
+    span = SMALL ? 128 / group : group / 128;
+    at = SMALL ? step * span : step / span;
+    rem = SMALL ? 0 : step % span;
+  }
+  // `by`: steps until the caller's next one
+  __device__ __forceinline__ void ask(int by) {
+#pragma unroll
+    for (int j = 0; j < N; ++j) {
+      const int i = min(SMALL ? at + (span == 4 ? j : j >> 1) : at, last);
+      sv[j] = w4_ld_scale(s + i);
+      if (ZEROS) zv[j] = w4_ld_zero(z + i);
+    }
+    if (SMALL) {
+      at += by * span;
+    } else {
+      rem += by;
+      while (rem >= span) { rem -= span; ++at; }
+    }
+  }
+};
+
+// A thread's row of a step, 128 entries, out of shared memory (64 bytes in the 64-byte swizzle: `swz` is the row's) ...
+__device__ __forceinline__ void w4_take_row(const unsigned char* row, int swz, uint4 (&wv)[4]) {
+#pragma unroll
+  for (int j = 0; j < 4; ++j) wv[j] = *reinterpret_cast<const uint4*>(row + ((j ^ swz) << 4));
+}
+// ... as bf16 into 64 columns of its lane of tensor memory, a piece of 32 entries (16 columns) at a time.
+template <bool ZEROS, bool SMALL>
+__device__ __forceinline__ void w4_widen_row(const uint4 (&wv)[4], const unsigned* scale, const unsigned* zero, unsigned a) {
+#pragma unroll
+  for (int j = 0; j < 4; ++j) {
+    const int i = SMALL ? j : 0;
+    const __nv_bfloat162 bias = ZEROS ? w4_bias((int)zero[i]) : __float2bfloat162_rn(136.f);
+    const unsigned s2 = scale[i] | (scale[i] << 16);
+    const unsigned words[4] = {wv[j].x, wv[j].y, wv[j].z, wv[j].w};
+    unsigned v[16];
+#pragma unroll
+    for (int q = 0; q < 4; ++q)
+#pragma unroll
+      for (int p = 0; p < 4; ++p) {
+        const unsigned e = w4_pair(words[q], p, bias);
+        const __nv_bfloat162 r = __hmul2(*reinterpret_cast<const __nv_bfloat162*>(&e), *reinterpret_cast<const __nv_bfloat162*>(&s2));
+        v[q * 4 + p] = *reinterpret_cast<const unsigned*>(&r);
+      }
+    asm volatile("tcgen05.st.sync.aligned.32x32b.x16.b32 [%0], {%1,%2,%3,%4,%5,%6,%7,%8,%9,%10,%11,%12,%13,%14,%15,%16};\n"
+                 ::"r"(a + j * 16), "r"(v[0]), "r"(v[1]), "r"(v[2]), "r"(v[3]), "r"(v[4]), "r"(v[5]), "r"(v[6]), "r"(v[7]), "r"(v[8]), "r"(v[9]), "r"(v[10]),
+                   "r"(v[11]), "r"(v[12]), "r"(v[13]), "r"(v[14]), "r"(v[15]) : "memory");
+  }
+  tmem_st_wait();
+}
+
+// 32 rows of x (from m0 on, `rows` of the tile in all) of this thread's column n of the output; `whole`: the warp's 32 columns lie inside. Neighbouring
+// lanes swap, so that the even one stores columns n and n + 1 of one row and the odd one of the next.
+template <typename TO>
+__device__ __forceinline__ void w4_store(TO* __restrict__ out, long long ldo, const float (&v)[32], long long m_base, int m0, int rows, int n, int N, int lane,
+                                         bool whole) {
+  if (whole) {
+#pragma unroll
+    for (int j = 0; j < 32; j += 2) {
+      const float give = lane & 1 ? v[j] : v[j + 1], got = __shfl_xor_sync(0xffffffffu, give, 1);
+      const float a = lane & 1 ? got : v[j], c = lane & 1 ? v[j + 1] : got;
+      const int m = m0 + j + (lane & 1);
+      if (m < rows) {
+        TO* dst = out + (m_base + m) * ldo + (n & ~1);
+        if constexpr (sizeof(TO) == 4) *reinterpret_cast<float2*>(dst) = make_float2(a, c);
+        else *reinterpret_cast<__nv_bfloat162*>(dst) = __floats2bfloat162_rn(a, c);
+      }
+    }
+  } else {
+#pragma unroll
+    for (int j = 0; j < 32; ++j)
+      if (m0 + j < rows && n < N) out[(m_base + m0 + j) * ldo + n] = from_f32<TO>(v[j]);
+  }
+}
+
+template <bool PAIR, bool ZEROS, bool SMALL, typename TO>
+__global__ void __launch_bounds__(W4_THREADS, 1)
 gemm_w4_tc_kernel(const __grid_constant__ CUtensorMap xmap, const __grid_constant__ CUtensorMap wmap, const bf16* __restrict__ scales,
                   const unsigned char* __restrict__ zeros, int group, int groups, TO* __restrict__ out, long long ldo, int M, int N, int K, int bn,
-                  int m_tiles, int parts, int* status) {
-  constexpr int BK = 128, ROWS = HALVES * 128, W_BYTES = ROWS * 64;
+                  int m_tiles, int parts, int* status, int trigger) {
+  constexpr int BK = 128, W_BYTES = 128 * 64, CTAS = PAIR ? 2 : 1, ROWS = 128 * CTAS, A_COL = 256;
   extern __shared__ unsigned char smem_dyn[];
-  __shared__ __align__(8) uint64_t full_bar[W4_TC_MAX_STAGES], empty_bar[W4_TC_MAX_STAGES], a_full[4], a_empty[4], acc_full[2], acc_empty[2];
+  __shared__ __align__(8) uint64_t w_full[W4_SLOTS], ready[W4_SLOTS], empty_bar[W4_SLOTS], acc_full[2], acc_empty[2];
   __shared__ unsigned tmem_slot;
-  unsigned char* smem = reinterpret_cast<unsigned char*>(((uintptr_t)smem_dyn + 1023) & ~(uintptr_t)1023);
+  unsigned char* Ws = w4_smem_base(smem_dyn);
+  unsigned char* Xs = Ws + W4_SLOTS * W_BYTES;
+  float* partial = reinterpret_cast<float*>(Ws);           // [bn][128] once the operands are used up (at most 128 KB)
   const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
-  const int X_BYTES = bn * 256, STAGES = w4_tc_stages(HALVES, bn);
-  unsigned char* Ws = smem;
-  unsigned char* Xs = smem + STAGES * W_BYTES;
-  float* partial = reinterpret_cast<float*>(smem);         // [bn][ROWS] once the operands are used up (at most 128 KB)
+  const int rank = PAIR ? (int)cluster_cta_rank() : 0, part = PAIR ? 0 : (int)cluster_cta_rank(), sharers = PAIR ? 2 : parts;
+  const int X_BYTES = bn / CTAS * 256;
   const int nk = (K + BK - 1) / BK, tiles = (N + ROWS - 1) / ROWS * m_tiles;
-  const int part = (int)cluster_cta_rank(), first = blockIdx.x / parts, stride = gridDim.x / parts;
   const int k0 = (int)((long long)nk * part / parts), steps = (int)((long long)nk * (part + 1) / parts) - k0;
-  // columns of tensor memory
-  const int acc_w = HALVES == 2 ? (bn <= 64 ? 64 : 128) : (bn <= 192 ? 192 : 256);
-  const int nbuf = HALVES == 2 ? (bn <= 64 ? 2 : 1) : (bn <= 192 ? 2 : 1);
-  const int a_bufs = HALVES == 2 ? 2 : (bn <= 192 ? 2 : 4), a_col = HALVES == 2 ? 256 : (bn <= 192 ? 384 : 256);
+  const int first = blockIdx.x / sharers, stride = gridDim.x / sharers;
+  const int nbuf = bn <= 128 ? 2 : 1;
+  if (trigger) pdl_trigger();
   if (threadIdx.x == 0) {
-    for (int s = 0; s < STAGES; ++s) { mbar_init(&full_bar[s], 2); mbar_init(&empty_bar[s], 1); }
 #pragma unroll
-    for (int b = 0; b < 4; ++b) { mbar_init(&a_full[b], 4 * HALVES); mbar_init(&a_empty[b], 1); }
+    for (int s = 0; s < W4_SLOTS; ++s) { mbar_init(&w_full[s], 1); mbar_init(&ready[s], 1 + 4 * CTAS); mbar_init(&empty_bar[s], 1); }
 #pragma unroll
-    for (int b = 0; b < 2; ++b) { mbar_init(&acc_full[b], 1); mbar_init(&acc_empty[b], 4); }
+    for (int b = 0; b < 2; ++b) { mbar_init(&acc_full[b], 1); mbar_init(&acc_empty[b], 4 * CTAS); }
     asm volatile("fence.mbarrier_init.release.cluster;\n" ::: "memory");
   }
-  if (warp == 3) tmem_alloc(&tmem_slot, 512);
+  if (warp == 3) { if (PAIR) tmem_alloc_pair(&tmem_slot, 512); else tmem_alloc(&tmem_slot, 512); }
   tc05_fence_before_sync();
-  __syncthreads();
+  if (PAIR) cluster_sync_all(); else __syncthreads();       // both CTAs' barriers and tensor memory are ready
   tc05_fence_after_sync();
   const unsigned tmem = tmem_slot;
   if (warp < 2) {
     if (lane == 0) {
       const bool is_w = warp == 1;
-      const int bytes = is_w ? W_BYTES : X_BYTES;
-      unsigned char* ring = is_w ? Ws : Xs;
       if (is_w && first < tiles)
-        for (int i = 0; i < steps && i < STAGES; ++i)
+        for (int i = 0; i < steps && i < W4_SLOTS; ++i)
           asm volatile("cp.async.bulk.prefetch.tensor.2d.L2.global.tile [%0, {%1, %2}];\n"
-                       ::"l"(&wmap), "r"((k0 + i) * (BK / 8)), "r"(first / m_tiles * ROWS) : "memory");
+                       ::"l"(&wmap), "r"((k0 + i) * (BK / 8)), "r"(first / m_tiles * ROWS + rank * 128) : "memory");
       pdl_wait();
       int s = 0, issued = 0;
       unsigned phase = 1;
       bool ok = true;
       for (int tile = first; tile < tiles && ok; tile += stride) {
-        const int y = is_w ? tile / m_tiles * ROWS : tile % m_tiles * bn;
+        const int y = is_w ? tile / m_tiles * ROWS + rank * 128 : tile % m_tiles * bn + rank * (bn / 2);
         for (int it = 0; it < steps; ++it, ++issued) {
-          if (issued >= STAGES && !mbar_wait(&empty_bar[s], phase)) {
+          if (issued >= W4_SLOTS && !mbar_wait(&empty_bar[s], phase)) {
             set_status(status, SI_WAIT_LIMIT);
-            w4_drain(full_bar, STAGES, issued);
+            if (is_w) w4_drain(w_full, issued);
+            else if (rank == 0) w4_drain(ready, issued);
             ok = false;
             break;
           }
-          unsigned char* to = ring + s * bytes;
-          mbar_expect_tx(&full_bar[s], (unsigned)bytes);   // both warps arrive, each with its own bytes
           if (is_w) {
-            tma_load_2d(to, &wmap, &full_bar[s], (k0 + it) * (BK / 8), y);
+            mbar_expect_tx(&w_full[s], W_BYTES);
+            tma_load_2d(Ws + s * W_BYTES, &wmap, &w_full[s], (k0 + it) * (BK / 8), y);
           } else {
-            tma_load_2d(to, &xmap, &full_bar[s], (k0 + it) * BK, y);
-            tma_load_2d(to + bytes / 2, &xmap, &full_bar[s], (k0 + it) * BK + 64, y);
+            unsigned char* to = Xs + s * X_BYTES;
+            if (rank == 0) mbar_expect_tx(&ready[s], (unsigned)(CTAS * X_BYTES));
+            if (PAIR) {
+              const unsigned bar = cluster_map_u32(&ready[s], 0);
+              tma_load_2d_pair(to, &xmap, bar, it * BK, y);
+              tma_load_2d_pair(to + X_BYTES / 2, &xmap, bar, it * BK + 64, y);
+            } else {
+              tma_load_2d(to, &xmap, &ready[s], (k0 + it) * BK, y);
+              tma_load_2d(to + X_BYTES / 2, &xmap, &ready[s], (k0 + it) * BK + 64, y);
+            }
           }
-          if (++s == STAGES) { s = 0; phase ^= 1u; }
+          if (++s == W4_SLOTS) { s = 0; phase ^= 1u; }
         }
       }
     }
   } else if (warp == 2) {
-    const unsigned idesc = umma_idesc_bf16(128, bn, false);
-    const unsigned long long xd0 = umma_desc_sw128(Xs, 16, 1024);
-    const unsigned x_step = (unsigned)X_BYTES / 16;
-    int s = 0, b = 0, local = 0;
-    unsigned phase = 0, a_phase = 0;
-    unsigned long long xd = xd0;
-    bool ok = true;
-    for (int tile = first; tile < tiles && ok; tile += stride, ++local) {
-      const int d = nbuf == 2 ? local & 1 : 0;
-      if (local >= nbuf) ok = mbar_wait_warp(&acc_empty[d], (unsigned)((local / nbuf - 1) & 1));
-      if (!ok) break;
-      tc05_fence_after_sync();
-      const unsigned acc = tmem + (unsigned)(d * HALVES * acc_w);
-      for (int it = 0; it < steps; ++it) {
-        ok = mbar_wait_warp(&full_bar[s], phase) && mbar_wait_warp(&a_full[b], a_phase);
+    if (rank == 0) {
+      const unsigned idesc = umma_idesc_bf16(ROWS, bn, false);
+      const unsigned long long xd0 = umma_desc_sw128(Xs, 16, 1024);
+      const unsigned x_step = (unsigned)X_BYTES / 16;
+      int s = 0, local = 0;
+      unsigned phase = 0;
+      unsigned long long xd = xd0;
+      bool ok = true;
+      for (int tile = first; tile < tiles && ok; tile += stride, ++local) {
+        const int d = nbuf == 2 ? local & 1 : 0;
+        if (local >= nbuf) ok = w4_wait(&acc_empty[d], (unsigned)((local / nbuf - 1) & 1));
         if (!ok) break;
         tc05_fence_after_sync();
-        if (elect_one()) {
-#pragma unroll
-          for (int hf = 0; hf < HALVES; ++hf) {
-            const unsigned a = tmem + (unsigned)(a_col + (hf * 2 + b) * 64);          // HALVES 1: hf is 0
-#pragma unroll
-            for (int k = 0; k < 8; ++k)
-              tc05_mma_bf16_tmem_a(acc + hf * acc_w, a + 8 * k, xd + (k >> 2) * (x_step / 2) + 2 * (k & 3), idesc, (it | k) != 0 ? 1u : 0u);
-          }
-          tc05_commit(&empty_bar[s]);
-          tc05_commit(&a_empty[b]);
-          if (it + 1 == steps) tc05_commit(&acc_full[d]);
-        }
-        __syncwarp();
-        xd += x_step;
-        if (++s == STAGES) { s = 0; xd = xd0; phase ^= 1u; }
-        if (++b == a_bufs) { b = 0; a_phase ^= 1u; }
-      }
-    }
-    if (!ok && lane == 0) set_status(status, SI_WAIT_LIMIT);
-  } else if (warp >= 8) {
-    const int g = (warp - 8) >> 2, row = (warp & 3) * 32 + lane, hf = HALVES == 2 ? g : 0;
-    const unsigned char* wrow = Ws + (hf * 128 + row) * 64;
-    const int swz = (row >> 1) & 3;
-    const unsigned lanes = (unsigned)((warp & 3) * 32) << 16;
-    const int every = HALVES == 2 ? 1 : 2;                 // this group's steps: every one, or every second one
-    int s = 0, b = 0, st = 0;                              // of the step that comes next, over all tiles
-    unsigned phase = 0, a_phase = 1;
-    bool ok = true;
-    pdl_wait();
-    for (int tile = first; tile < tiles && ok; tile += stride) {
-      const int n = tile / m_tiles * ROWS + hf * 128 + row;
-      const bf16* srow = scales + (size_t)(n < N ? n : 0) * groups;
-      const unsigned char* zrow = ZEROS ? zeros + (size_t)(n < N ? n : 0) * groups : nullptr;
-      // scales of the four pieces of 32 entries of a step, asked for a step of this group ahead
-      unsigned sc[4], zp[4];
-      auto ask = [&](int it) {
-        const int k = (k0 + it) * BK;
-        if (group >= BK) {
-          const int at = min(k / group, groups - 1);
-          sc[0] = w4_ld_scale(srow + at, true);
-          if (ZEROS) zp[0] = w4_ld_zero(zrow + at, true);
-        } else {
-#pragma unroll
-          for (int j = 0; j < 4; ++j) {
-            const int at = min((k + 32 * j) / group, groups - 1);       // group is 32 or 64 here
-            sc[j] = w4_ld_scale(srow + at, true);
-            if (ZEROS) zp[j] = w4_ld_zero(zrow + at, true);
-          }
-        }
-      };
-      const int it0 = HALVES == 2 || (st & 1) == g ? 0 : 1;               // this group's first step of the tile
-      if (it0 < steps) ask(it0);
-      for (int it = 0; it < steps; ++it, ++st) {
-        const bool mine = HALVES == 2 || (st & 1) == g;
-        if (mine) {
-          unsigned now[4], z[4];
-#pragma unroll
-          for (int j = 0; j < 4; ++j) { now[j] = group >= BK ? sc[0] : sc[j]; z[j] = ZEROS ? (group >= BK ? zp[0] : zp[j]) : 8u; }
-          if (it + every < steps) ask(it + every);
-          ok = mbar_wait_warp(&full_bar[s], phase);
-          if (!ok) break;
-          uint4 wv[4];
-#pragma unroll
-          for (int j = 0; j < 4; ++j) wv[j] = *reinterpret_cast<const uint4*>(wrow + s * W_BYTES + ((j ^ swz) << 4));
-          if (st >= a_bufs) ok = mbar_wait_warp(&a_empty[b], a_phase);
+        const unsigned acc = tmem + (unsigned)(d * 128);
+        for (int it = 0; it < steps; ++it) {
+          ok = w4_wait(&ready[s], phase);
           if (!ok) break;
           tc05_fence_after_sync();
-          const unsigned a = tmem + lanes + (unsigned)(a_col + (hf * 2 + b) * 64);
+          if (elect_one()) {
+            const unsigned a = tmem + (unsigned)(A_COL + s * 64);
 #pragma unroll
-          for (int h = 0; h < 2; ++h) {
-            unsigned v[32];
-#pragma unroll
-            for (int j2 = 0; j2 < 2; ++j2) {
-              const int j = 2 * h + j2;
-              const __nv_bfloat162 bias = w4_bias((int)z[j]);
-              const unsigned s2 = now[j] | (now[j] << 16);
-              const unsigned words[4] = {wv[j].x, wv[j].y, wv[j].z, wv[j].w};
-#pragma unroll
-              for (int q = 0; q < 4; ++q)
-#pragma unroll
-                for (int p = 0; p < 4; ++p) {
-                  const unsigned e = w4_pair(words[q], p, bias);
-                  const __nv_bfloat162 r = __hmul2(*reinterpret_cast<const __nv_bfloat162*>(&e), *reinterpret_cast<const __nv_bfloat162*>(&s2));
-                  v[j2 * 16 + q * 4 + p] = *reinterpret_cast<const unsigned*>(&r);
-                }
+            for (int k = 0; k < 8; ++k) {
+              const unsigned long long b = xd + (k >> 2) * (x_step / 2) + 2 * (k & 3);
+              if (PAIR) w4_mma_pair_tmem_a(acc, a + 8 * k, b, idesc, (it | k) != 0 ? 1u : 0u);
+              else tc05_mma_bf16_tmem_a(acc, a + 8 * k, b, idesc, (it | k) != 0 ? 1u : 0u);
             }
-            tmem_st_32x32_issue(a + h * 32, v);
+            if (PAIR) tc05_commit_pair(&empty_bar[s], 3); else tc05_commit(&empty_bar[s]);
+            if (it + 1 == steps) { if (PAIR) tc05_commit_pair(&acc_full[d], 3); else tc05_commit(&acc_full[d]); }
           }
-          tmem_st_wait();
-          tc05_fence_before_sync();
           __syncwarp();
-          if (lane == 0) mbar_arrive(&a_full[b]);
+          xd += x_step;
+          if (++s == W4_SLOTS) { s = 0; xd = xd0; phase ^= 1u; }
         }
-        if (++s == STAGES) { s = 0; phase ^= 1u; }
-        if (++b == a_bufs) { b = 0; a_phase ^= 1u; }
+      }
+      if (!ok && lane == 0) set_status(status, SI_WAIT_LIMIT);
+    }
+  } else if (warp >= 8) {
+    const int slot = (warp - 8) >> 2, row = (warp & 3) * 32 + lane;      // four warps a slot: every fourth step is theirs
+    const unsigned char* wrow = Ws + slot * W_BYTES + row * 64;
+    const int swz = (row >> 1) & 3;
+    const unsigned mine = tmem + ((unsigned)((warp & 3) * 32) << 16) + (unsigned)(A_COL + slot * 64);
+    int at = slot;                                         // this group's next step, counted from the tile's first
+    unsigned phase = 0;
+    bool ok = true;
+    pdl_wait();
+    for (int tile = first; tile < tiles && ok; tile += stride, at -= steps) {
+      const int n = tile / m_tiles * ROWS + rank * 128 + row;
+      W4Scales<ZEROS, SMALL> sc;
+      sc.start(scales, zeros, n < N ? n : 0, group, groups, k0 + at);
+      if (at < steps) sc.ask(W4_SLOTS);
+      for (; at < steps; at += W4_SLOTS, phase ^= 1u) {
+        unsigned now[W4Scales<ZEROS, SMALL>::N], z[W4Scales<ZEROS, SMALL>::N];
+#pragma unroll
+        for (int j = 0; j < W4Scales<ZEROS, SMALL>::N; ++j) { now[j] = sc.sv[j]; if (ZEROS) z[j] = sc.zv[j]; }
+        if (at + W4_SLOTS < steps) sc.ask(W4_SLOTS);
+        ok = w4_wait(&w_full[slot], phase);                // the slot's columns are free as well: see above
+        if (!ok) break;
+        tc05_fence_after_sync();
+        uint4 wv[4];
+        w4_take_row(wrow, swz, wv);
+        w4_widen_row<ZEROS, SMALL>(wv, now, z, mine);
+        tc05_fence_before_sync();
+        __syncwarp();
+        if (lane == 0) { if (PAIR) w4_arrive_leader(&ready[slot]); else mbar_arrive(&ready[slot]); }
       }
     }
     if (!ok && lane == 0) set_status(status, SI_WAIT_LIMIT);
@@ -402,7 +614,7 @@ gemm_w4_tc_kernel(const __grid_constant__ CUtensorMap xmap, const __grid_constan
     int local = 0;
     for (int tile = first; tile < tiles; tile += stride, ++local) {
       const int d = nbuf == 2 ? local & 1 : 0;
-      const int m_base = tile % m_tiles * bn, n_base = tile / m_tiles * ROWS + (warp & 3) * 32;
+      const int m_base = tile % m_tiles * bn, n_base = tile / m_tiles * ROWS + rank * 128 + (warp & 3) * 32;
       if (!mbar_wait_warp(&acc_full[d], (unsigned)((local / nbuf) & 1))) {
         if (lane == 0) set_status(status, SI_WAIT_LIMIT);
         break;
@@ -410,53 +622,33 @@ gemm_w4_tc_kernel(const __grid_constant__ CUtensorMap xmap, const __grid_constan
       tc05_fence_after_sync();
       const int rows = min(bn, M - m_base);
 #pragma unroll 1
-      for (int hf = 0; hf < HALVES; ++hf) {
-        const unsigned src = tmem + lanes + (unsigned)((d * HALVES + hf) * acc_w);
-        const int n = n_base + hf * 128 + lane;
-#pragma unroll 1
-        for (int m0 = 0; m0 < bn; m0 += 32) {
-          float v[32];
-          tmem_ld_32x32(src + m0, v);
-          if (hf == HALVES - 1 && m0 + 32 >= bn) {         // in registers: the issuer may have the accumulator back
-            tc05_fence_before_sync();
-            __syncwarp();
-            if (lane == 0) mbar_arrive(&acc_empty[d]);
-          }
-          if (parts > 1) {
+      for (int m0 = 0; m0 < bn; m0 += 32) {
+        float v[32];
+        tmem_ld_32x32(tmem + lanes + (unsigned)(d * 128 + m0), v);
+        if (m0 + 32 >= bn) {                               // in registers: the issuer may have the accumulator back
+          tc05_fence_before_sync();
+          __syncwarp();
+          if (lane == 0) { if (PAIR) w4_arrive_leader(&acc_empty[d]); else mbar_arrive(&acc_empty[d]); }
+        }
+        if (!PAIR && parts > 1) {
 #pragma unroll
-            for (int j = 0; j < 32; ++j)
-              if (m0 + j < bn) partial[(m0 + j) * ROWS + hf * 128 + (warp & 3) * 32 + lane] = v[j];
-          } else if (vec2 && n_base + hf * 128 + 32 <= N) {
-            // neighbouring lanes swap: the even one stores columns n, n + 1 of row j, the odd one of row j + 1
-#pragma unroll
-            for (int j = 0; j < 32; j += 2) {
-              const float give = lane & 1 ? v[j] : v[j + 1], got = __shfl_xor_sync(0xffffffffu, give, 1);
-              const float a = lane & 1 ? got : v[j], c = lane & 1 ? v[j + 1] : got;
-              const int m = m0 + j + (lane & 1);
-              if (m < rows) {
-                TO* dst = out + (size_t)(m_base + m) * ldo + (n & ~1);
-                if constexpr (sizeof(TO) == 4) *reinterpret_cast<float2*>(dst) = make_float2(a, c);
-                else *reinterpret_cast<__nv_bfloat162*>(dst) = __floats2bfloat162_rn(a, c);
-              }
-            }
-          } else {
-#pragma unroll
-            for (int j = 0; j < 32; ++j)
-              if (m0 + j < rows && n < N) out[(size_t)(m_base + m0 + j) * ldo + n] = from_f32<TO>(v[j]);
-          }
+          for (int j = 0; j < 32; ++j)
+            if (m0 + j < bn) partial[(m0 + j) * 128 + (warp & 3) * 32 + lane] = v[j];
+        } else {
+          w4_store<TO>(out, ldo, v, m_base, m0, rows, n_base + lane, N, lane, vec2 && n_base + 32 <= N);
         }
       }
     }
   }
-  if (parts > 1) {                                         // one tile a cluster
+  if (!PAIR && parts > 1) {                                // one tile a cluster
     __syncwarp();
     cluster_sync_all();                                    // every block's sums lie in its shared memory
-    const int m_base = first % m_tiles * bn, n0 = first / m_tiles * ROWS;
+    const int m_base = first % m_tiles * bn, n0 = first / m_tiles * 128;
     const int lo = bn * part / parts, hi = min(M - m_base, bn * (part + 1) / parts);
     const bool vec = ldo % 4 == 0 && (uintptr_t)out % 16 == 0;
-    for (int i = threadIdx.x; i < (hi - lo) * (ROWS / 4); i += 512) {
-      const int m = lo + i / (ROWS / 4), c4 = i % (ROWS / 4) * 4, n = n0 + c4;
-      const float* at = partial + m * ROWS + c4;
+    for (int i = threadIdx.x; i < (hi - lo) * 32; i += W4_THREADS) {
+      const int m = lo + (i >> 5), c4 = (i & 31) * 4, n = n0 + c4;
+      const float* at = partial + m * 128 + c4;
       float4 v[8];
 #pragma unroll
       for (int c = 0; c < 8; ++c) v[c] = c < parts ? w4_ld_cluster(cluster_map_u32(at, (unsigned)c)) : make_float4(0.f, 0.f, 0.f, 0.f);
@@ -479,19 +671,19 @@ gemm_w4_tc_kernel(const __grid_constant__ CUtensorMap xmap, const __grid_constan
     cluster_sync_all();                                    // no block goes while another one reads its sums
   }
   tc05_fence_before_sync();
-  __syncthreads();
-  if (warp == 3) tmem_dealloc(tmem, 512);
+  if (PAIR) cluster_sync_all(); else __syncthreads();       // no CTA frees tensor memory the other one's instructions use
+  if (warp == 3) { if (PAIR) tmem_dealloc_pair(tmem, 512); else tmem_dealloc(tmem, 512); }
 }
 
-struct W4Shape { int halves, bn, m_tiles, parts; };
+struct W4Shape { bool pair; int bn, m_tiles, parts; };
 
-static void w4_tc_config(cudaLaunchConfig_t* cfg, unsigned blocks, int parts, cudaStream_t stream, cudaLaunchAttribute* attr) {
+static void w4_tc_config(cudaLaunchConfig_t* cfg, unsigned blocks, int cluster, cudaStream_t stream, cudaLaunchAttribute* attr) {
   cfg->gridDim = dim3(blocks);
-  cfg->blockDim = dim3(512);
+  cfg->blockDim = dim3(W4_THREADS);
   cfg->dynamicSmemBytes = W4_TC_SMEM + 1024;
   cfg->stream = stream;
   attr[0].id = cudaLaunchAttributeClusterDimension;
-  attr[0].val.clusterDim.x = (unsigned)parts;
+  attr[0].val.clusterDim.x = (unsigned)cluster;
   attr[0].val.clusterDim.y = 1;
   attr[0].val.clusterDim.z = 1;
   attr[1].id = cudaLaunchAttributeProgrammaticStreamSerialization;
@@ -500,89 +692,82 @@ static void w4_tc_config(cudaLaunchConfig_t* cfg, unsigned blocks, int parts, cu
   cfg->numAttrs = si_pdl_enabled() ? 2 : 1;
 }
 
-// Clusters of `parts` blocks that the device runs at once, asked once per device and size (all forms of the kernel take an SM a block).
-static int w4_clusters(int parts) {
+// Clusters of `size` blocks that the device runs at once (the SMs of a cluster lie together, so not every one finds its place), asked once per device
+// and size; all forms of the kernel take an SM a block.
+static int w4_clusters(int size) {
   static int known[64][9] = {};
   int dev = 0;
   if (cudaGetDevice(&dev) != cudaSuccess || dev < 0 || dev >= 64) dev = 0;
-  if (parts == 1) return si_sm_count();
-  if (!known[dev][parts]) {
-    auto k = gemm_w4_tc_kernel<1, true, bf16>;
+  if (size == 1) return si_sm_count();
+  if (!known[dev][size]) {
+    auto k = gemm_w4_tc_kernel<false, true, true, bf16>;
     cudaLaunchAttribute attr[2];
     cudaLaunchConfig_t cfg = {};
-    w4_tc_config(&cfg, (unsigned)parts, parts, 0, attr);
+    w4_tc_config(&cfg, (unsigned)size, size, 0, attr);
     int n = 0;
     if (cudaFuncSetAttribute(k, cudaFuncAttributeMaxDynamicSharedMemorySize, W4_TC_SMEM + 1024) != cudaSuccess ||
         cudaOccupancyMaxActiveClusters(&n, k, &cfg) != cudaSuccess || n < 1) { cudaGetLastError(); n = 1; }
-    known[dev][parts] = n;
+    known[dev][size] = n;
   }
-  return known[dev][parts];
+  return known[dev][size];
 }
 
+// The shape for which the busiest SM is done first, in clocks: a step is bn * 4 of the tensor cores (4,096 products a clock and SM) and 150 beside them, 800 at
+// least (instructions, a wait, a commit), and for a CTA alone what taking in its bn rows of x lasts (60 bytes a clock). Where there is one accumulator its
+// stores come on top. More and narrower tiles have to save a sixteenth: they cost more power, at whose cap long products run. us, 2,048 x 28,672 x 4,096:
+// 8 tiles of 256 361, 9 of 240 376, 11 of 192 386, 16 of 128 396; 512 x 4,096 x 14,336: 2 of 256 77, 3 of 176 69, 4 of 128 65.
 static W4Shape w4_shape(int M, int N, int K) {
-  const int nk = (K + 127) / 128;
-  W4Shape best = {1, 128, 1, 1};
-  double least = -1;
-  for (int halves = 1; halves <= 2; ++halves) {
-    if (halves == 2 && M > 128) break;
-    const int n_tiles = (N + halves * 128 - 1) / (halves * 128);
-    const int fewest = (M + 255) / 256;
-    for (int mt = fewest; mt <= fewest + 2; ++mt) {
-      const int bn = ((M + mt - 1) / mt + 15) / 16 * 16;
-      if (mt > fewest && bn < 96) break;
-      for (int parts = 1; parts <= 8 && parts <= nk; parts *= 2) {
-        const long long tiles = (long long)n_tiles * mt, slots = w4_clusters(parts);
-        if (parts > 1 && tiles > slots) break;
-        const int steps = (nk + parts - 1) / parts;
-        const double mma = (bn / 2 > 47 ? bn / 2 : 47) * 8.0 * halves, step = halves == 2 ? (mma + 420 > 900 ? mma + 420 : 900) : (mma + 100 > 600 ? mma + 100 : 600);
-        const bool one = halves == 1 && bn > 192;
-        const double cost = (double)((tiles + slots - 1) / slots) * (steps * step + (one ? 20.0 * bn : 500.0)) + 6000 + 16.0 * bn + (parts > 1 ? 2500 : 0);
-        if (least < 0 || cost < least) { least = cost; best = W4Shape{halves, bn, mt, parts}; }
-      }
-    }
+  const int nk = (K + 127) / 128, fewest = (M + 255) / 256;
+  W4Shape best = {false, 128, 1, 1};
+  long long least = -1;
+  auto consider = [&](bool pair, int bn, int mt, int parts) {
+    const long long tiles = (long long)((N + (pair ? 255 : 127)) / (pair ? 256 : 128)) * mt, slots = w4_clusters(pair ? 2 : parts);
+    if (parts > 1 && tiles > slots) return;
+    const int steps = (nk + parts - 1) / parts;
+    long long step = bn * 4 + 150;
+    if (step < 800) step = 800;
+    if (!pair && step < (8192 + bn * 256) / 60) step = (8192 + bn * 256) / 60;
+    const long long cost = (tiles + slots - 1) / slots * (steps * step + (bn > 128 ? 8 * bn : 300)) + 12 * bn + (parts > 1 ? 2500 : 0);
+    if (least < 0 || cost * 16 < least * 15) { least = cost; best = W4Shape{pair, bn, mt, parts}; }
+  };
+  for (int mt = fewest; mt <= fewest + 8; ++mt) {
+    const int bn = ((M + mt - 1) / mt + 15) / 16 * 16;
+    if (mt > fewest && bn < 64) break;
+    if (M > 64) consider(true, bn, mt, 1);
+    if (bn <= 128)                                         // a CTA alone holds 128 rows of x a slot
+      for (int parts = 1; parts <= 8 && parts <= nk; parts *= 2) consider(false, bn, mt, parts);
   }
-  if (const char* e = getenv("W4_SHAPE")) sscanf(e, "%d,%d,%d,%d", &best.halves, &best.bn, &best.m_tiles, &best.parts);
-  if (getenv("W4_SAY")) printf("shape %dx%dx%d: halves %d bn %d mt %d parts %d\n", M, N, K, best.halves, best.bn, best.m_tiles, best.parts);
   return best;
 }
 
-static int w4_encode(CUtensorMap* map, CUtensorMapDataType type, int size, const void* base, long long rows, long long cols, long long ld, unsigned box_cols,
-                     unsigned box_rows, CUtensorMapSwizzle swizzle) {
-  SiEncodeTiledFn fn = si_encode_fn();
-  if (!fn) return -3;
-  const cuuint64_t dims[2] = {(cuuint64_t)cols, (cuuint64_t)rows};
-  const cuuint64_t strides[1] = {(cuuint64_t)(ld * size)};
-  const cuuint32_t box[2] = {box_cols, box_rows};
-  const cuuint32_t estr[2] = {1, 1};
-  CUresult r = fn(map, type, 2, const_cast<void*>(base), dims, strides, box, estr, CU_TENSOR_MAP_INTERLEAVE_NONE, swizzle,
-                  CU_TENSOR_MAP_L2_PROMOTION_L2_128B, CU_TENSOR_MAP_FLOAT_OOB_FILL_NONE);
-  return r == CUDA_SUCCESS ? 0 : 1000 + (int)r;
-}
-
-template <int HALVES, bool ZEROS, typename TO>
+template <bool PAIR, bool ZEROS, bool SMALL, typename TO>
 static int w4_tc_launch(const W4Call& c, const W4Shape& sh) {
-  auto k = gemm_w4_tc_kernel<HALVES, ZEROS, TO>;
+  auto k = gemm_w4_tc_kernel<PAIR, ZEROS, SMALL, TO>;
   cudaError_t e = cudaFuncSetAttribute(k, cudaFuncAttributeMaxDynamicSharedMemorySize, W4_TC_SMEM + 1024);
   if (e != cudaSuccess) return (int)e;
   CUtensorMap xm, wm;
-  int rc = w4_encode(&xm, CU_TENSOR_MAP_DATA_TYPE_BFLOAT16, 2, c.x, c.M, c.K, c.ldx, 64, (unsigned)sh.bn, CU_TENSOR_MAP_SWIZZLE_128B);
-  if (!rc) rc = w4_encode(&wm, CU_TENSOR_MAP_DATA_TYPE_INT32, 4, c.w, c.N, c.K / 8, c.ldw, 16, HALVES * 128, CU_TENSOR_MAP_SWIZZLE_64B);
+  int rc = w4_encode(&xm, CU_TENSOR_MAP_DATA_TYPE_BFLOAT16, 2, c.x, c.M, c.K, c.ldx, 64, (unsigned)(PAIR ? sh.bn / 2 : sh.bn), CU_TENSOR_MAP_SWIZZLE_128B);
+  if (!rc) rc = w4_encode(&wm, CU_TENSOR_MAP_DATA_TYPE_INT32, 4, c.w, c.N, c.K / 8, c.ldw, 16, 128, CU_TENSOR_MAP_SWIZZLE_64B);
   if (rc) return rc;
-  const long long tiles = (long long)((c.N + HALVES * 128 - 1) / (HALVES * 128)) * sh.m_tiles, slots = si_sm_count();
+  const int cluster = PAIR ? 2 : sh.parts;
+  const long long tiles = (long long)((c.N + (PAIR ? 255 : 127)) / (PAIR ? 256 : 128)) * sh.m_tiles, slots = w4_clusters(cluster);
   if (tiles > 0x0fffffffLL) return -2;
-  const long long blocks = sh.parts > 1 ? tiles * sh.parts : tiles < slots ? tiles : slots;
+  const long long blocks = (tiles < slots || cluster == sh.parts && cluster > 1 ? tiles : slots) * cluster;      // a tile cut over a cluster is its only one
   cudaLaunchAttribute attr[2];
   cudaLaunchConfig_t cfg = {};
-  w4_tc_config(&cfg, (unsigned)blocks, sh.parts, c.stream, attr);
-  cudaLaunchKernelEx(&cfg, k, xm, wm, c.scales, c.zeros, c.group, c.groups, (TO*)c.out, c.ldo, c.M, c.N, c.K, sh.bn, sh.m_tiles, sh.parts, c.status);
+  w4_tc_config(&cfg, (unsigned)blocks, cluster, c.stream, attr);
+  cudaLaunchKernelEx(&cfg, k, xm, wm, c.scales, c.zeros, c.group, c.groups, (TO*)c.out, c.ldo, c.M, c.N, c.K, sh.bn, sh.m_tiles, sh.parts, c.status,
+                     si_pdl_trigger_mode(blocks, si_sm_count()));
   return si_last_error();
 }
 
 template <typename TO>
 static int w4_tc(const W4Call& c) {
   const W4Shape sh = w4_shape(c.M, c.N, c.K);
-  if (sh.halves == 2) return c.zeros ? w4_tc_launch<2, true, TO>(c, sh) : w4_tc_launch<2, false, TO>(c, sh);
-  return c.zeros ? w4_tc_launch<1, true, TO>(c, sh) : w4_tc_launch<1, false, TO>(c, sh);
+#define W4_TC(PAIR, ZEROS) (c.group < 128 ? w4_tc_launch<PAIR, ZEROS, true, TO>(c, sh) : w4_tc_launch<PAIR, ZEROS, false, TO>(c, sh))
+  if (sh.pair) return c.zeros ? W4_TC(true, true) : W4_TC(true, false);
+  return c.zeros ? W4_TC(false, true) : W4_TC(false, false);
+#undef W4_TC
 }
 
 // 1 when these kernels take operands so laid out (rows that start on 16-byte boundaries and end on one, the driver's tensor maps), else
@@ -600,6 +785,7 @@ SI_EXPORT int si_gemm_w4(const void* x, long long ldx, const void* w, long long 
   W4Call c;
   c.x = (const bf16*)x; c.ldx = ldx; c.w = (const unsigned*)w; c.ldw = ldw; c.scales = (const bf16*)scales; c.zeros = (const unsigned char*)zeros;
   c.group = group; c.groups = (K - 1) / group + 1; c.out = out; c.ldo = ldo; c.M = M; c.N = N; c.K = K; c.status = status; c.stream = stream;
-  if (M <= 16) return out_dtype == SI_BF16 ? w4_few<bf16>(c) : w4_few<float>(c);
+  W4Few f;
+  if (w4_few_shape(M, N, K, zeros != nullptr, group < 128, &f)) return out_dtype == SI_BF16 ? w4_few<bf16>(c, f) : w4_few<float>(c, f);
   return out_dtype == SI_BF16 ? w4_tc<bf16>(c) : w4_tc<float>(c);
 }

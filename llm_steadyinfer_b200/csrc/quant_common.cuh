@@ -28,7 +28,12 @@ __device__ __forceinline__ unsigned char q8_pack1(float a) { return (unsigned ch
 
 // Pair p (entries 2p, 2p + 1) of a word of eight 4-bit entries as two bf16 of value 128 + q: bf16 counts in ones from 128 to 255, so
 // the four bits go straight into the mantissa.
-__device__ __forceinline__ unsigned w4_pair_raw(unsigned word, int p) { return ((word >> (4 * p)) & 0x000f000fu) | 0x43004300u; }
+// (Written as one instruction: the compiler makes two of the mask and the or, and such instructions are what bounds the kernels that widen.)
+__device__ __forceinline__ unsigned w4_pair_raw(unsigned word, int p) {
+  unsigned v;
+  asm("lop3.b32 %0, %1, %2, %3, 0xea;\n" : "=r"(v) : "r"(word >> (4 * p)), "r"(0x000f000fu), "r"(0x43004300u));
+  return v;
+}
 // The same less 128 + z, exact: `bias` holds 128 + z twice.
 __device__ __forceinline__ unsigned w4_pair(unsigned word, int p, __nv_bfloat162 bias) {
   const unsigned raw = w4_pair_raw(word, p);
