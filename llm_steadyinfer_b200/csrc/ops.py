@@ -2315,34 +2315,55 @@ E4M3 = torch.float8_e4m3fn
 W4_SHIFTS = (0, 16, 4, 20, 8, 24, 12, 28)      # the bit of entry i of the eight that share an int32 word
 
 
-def _here(what: str, *ts) -> None:
-    """Every tensor is on the device whose stream the kernel is launched on."""
+# These calls check their arguments without building a message before one is needed: a decode step makes many of them, and each lasts a few
+# microseconds on the GPU.
+_ROWS_Q8_ARGS = [_c_p, _c_int, _c_ll, _c_p, _c_p, _c_int, _c_int, _c_p]
+_SWIGLU_Q8_ARGS = [_c_p, _c_int, _c_p, _c_p, _c_int, _c_int, _c_int, _c_p]
+_NORM_Q8_ARGS = [_c_p, _c_p, _c_p, _c_int, _c_p, _c_p, _c_int, _c_p, _c_p, _c_p, _c_int, _c_int, _c_f, _c_p, _c_ll, _c_p]
+_GEMM_Q8_ARGS = [_c_p, _c_ll, _c_p, _c_p, _c_ll, _c_p, _c_p, _c_ll, _c_int, _c_int, _c_int, _c_int, _c_p, _c_p]
+_GEMM_W4_ARGS = [_c_p, _c_ll, _c_p, _c_ll, _c_p, _c_p, _c_int, _c_p, _c_ll, _c_int, _c_int, _c_int, _c_int, _c_p, _c_p]
+
+
+def _here(what: str, *ts) -> int:
+    """The handle of the stream that the kernel is launched on; every tensor has to be on that stream's device."""
+    index = ts[0].get_device()
+    for t in ts:
+        if t is not None and t.get_device() != index:
+            index = -1
+            break
+    if index >= 0:
+        at = _device_index if _device_index is not None else torch.cuda.current_device()
+        if index == at:
+            return _raw_stream(at) if _raw_stream is not None else torch.cuda.current_stream().cuda_stream
+        raise KernelError(f"{what}: the tensors are on device {index}, the kernel is launched on device {at}")
     for t in ts:
         if t is not None and not t.is_cuda:
             raise KernelError("kernels take CUDA tensors only; there is no CPU path")
-    index = _device_index if _device_index is not None else torch.cuda.current_device()
-    for t in ts:
-        if t is not None and t.get_device() != index:
-            raise KernelError(f"{what}: a tensor is on device {t.get_device()}, the kernel is launched on device {index}")
+    raise KernelError(f"{what}: the tensors are on different devices ({', '.join(str(t.get_device()) for t in ts if t is not None)})")
 
 
-def _ld(t: torch.Tensor) -> int:
-    """Entries between the rows of a matrix (the stride of a single row says nothing)."""
-    return t.stride(0) if t.shape[0] > 1 else t.shape[1]
+def _matrix(t, what: str):
+    """(rows, columns, entries between rows) of a matrix whose rows are contiguous; the stride of a single row says nothing."""
+    shape, strides = t.shape, t.stride()
+    if len(shape) != 2 or (strides[1] != 1 and shape[1] > 1):
+        raise KernelError(f"{what} must be a matrix whose rows are contiguous")
+    rows, cols = shape
+    return rows, cols, strides[0] if rows > 1 else cols
 
 
-def _rows_of(t, what: str) -> None:
-    _need(t.dim() == 2 and (t.stride(1) == 1 or t.shape[1] <= 1), f"{what} must be a matrix whose rows are contiguous")
+def _f32_of(t, n: int, what: str) -> None:
+    if t.dtype is not _F32 or t.numel() != n or not t.is_contiguous():
+        raise KernelError(f"{what} must be contiguous fp32 of {n} elements")
 
 
-def _out_rows(t, what: str) -> None:
-    _rows_of(t, what)
-    _need(t.shape[0] <= 1 or t.stride(0) >= t.shape[1], f"{what}: its rows overlap")
+_F32, _BF16 = torch.float32, torch.bfloat16
 
 
 def _q8_out(out, scale, R: int, width: int, what: str) -> None:
-    _need(out.dtype == E4M3 and out.is_contiguous() and out.shape == (R, width), f"{what}: out must be contiguous float8_e4m3fn [{R}, {width}]")
-    _need(scale.dtype == torch.float32 and scale.is_contiguous() and scale.numel() == R, f"{what}: scale must be contiguous fp32 of {R} elements")
+    if out.dtype is not E4M3 or out.shape != (R, width) or not out.is_contiguous():
+        raise KernelError(f"{what}: out must be contiguous float8_e4m3fn [{R}, {width}]")
+    if scale.dtype is not _F32 or scale.numel() != R or not scale.is_contiguous():
+        raise KernelError(f"{what}: scale must be contiguous fp32 of {R} elements")
 
 
 def add_rmsnorm_q8(resid, delta, weight, eps: float, out, scale, rows=None, ahead=None, delta2=None, dst=None) -> None:
@@ -2350,125 +2371,147 @@ def add_rmsnorm_q8(resid, delta, weight, eps: float, out, scale, rows=None, ahea
     scale[r] = max(max |y[r]|, 2^-100) / 448 (fp32 [R]), out[r] = y[r] / scale[r] rounded to e4m3 ([R, d], contiguous).
 
     The new stream goes into ``dst`` (fp32 like resid; default: resid, in place). With ``rows`` (int32 [R]) output row r comes from stream
-    row rows[r] and no stream is written. ``ahead``: as in ``add_rmsnorm``. delta and delta2: fp32 or bf16 alike. Sums are fp32."""
-    _here("add_rmsnorm_q8", resid, delta, weight, out, scale, rows, delta2, dst, ahead)
-    _need(resid.dim() == 2 and resid.dtype == torch.float32 and resid.is_contiguous(), "add_rmsnorm_q8: resid must be contiguous fp32 rows")
-    _i32(rows, "rows")
-    T, d = resid.shape
-    _need(weight.numel() == d and weight.is_contiguous(), "add_rmsnorm_q8: weight must be contiguous, as wide as the stream")
-    _need(delta2 is None or delta is not None, "add_rmsnorm_q8: delta2 goes beside delta")
+    row rows[r] and no stream is written. ``ahead``: as in ``add_rmsnorm``. delta and delta2: fp32 or bf16 alike. Sums are fp32. A row with an
+    entry that is not finite comes out as the formula says: NaN, or zero where a finite entry meets an infinite norm."""
+    stream = _here("add_rmsnorm_q8", resid, delta, weight, out, scale, rows, delta2, dst, ahead)
+    shape = resid.shape
+    if len(shape) != 2 or resid.dtype is not _F32 or not resid.is_contiguous():
+        raise KernelError("add_rmsnorm_q8: resid must be contiguous fp32 rows")
+    T, d = shape
+    if weight.numel() != d or not weight.is_contiguous():
+        raise KernelError("add_rmsnorm_q8: weight must be contiguous, as wide as the stream")
+    if delta2 is not None and delta is None:
+        raise KernelError("add_rmsnorm_q8: delta2 goes beside delta")
     for t in (delta, delta2):
-        _need(t is None or (t.is_contiguous() and t.shape == resid.shape and t.dtype == delta.dtype),
-              "add_rmsnorm_q8: delta and delta2 must be contiguous like resid, and of one dtype")
-    _need(dst is None or rows is None, "add_rmsnorm_q8: with rows no stream is written")
-    _need(dst is None or (dst.dtype == torch.float32 and dst.is_contiguous() and dst.shape == resid.shape), "add_rmsnorm_q8: dst must be contiguous fp32 like resid")
-    R = T if rows is None else rows.numel()
+        if t is not None and (t.shape != shape or t.dtype is not delta.dtype or not t.is_contiguous()):
+            raise KernelError("add_rmsnorm_q8: delta and delta2 must be contiguous like resid, and of one dtype")
+    if dst is not None:
+        if rows is not None:
+            raise KernelError("add_rmsnorm_q8: with rows no stream is written")
+        if dst.dtype is not _F32 or dst.shape != shape or not dst.is_contiguous():
+            raise KernelError("add_rmsnorm_q8: dst must be contiguous fp32 like resid")
+    if rows is None:
+        R = T
+        if dst is None and delta is not None:
+            dst = resid
+    else:
+        _i32(rows, "rows")
+        R = rows.numel()
     _q8_out(out, scale, R, d, "add_rmsnorm_q8")
     xd, wd = F32 if delta is None else _dt(delta), _dt(weight)
     if R == 0:
         return
-    if rows is None and dst is None and delta is not None:
-        dst = resid
     ahead_bytes = min(ahead.numel() * ahead.element_size(), AHEAD_BYTES) if ahead is not None and ahead.is_contiguous() else 0
-    f = _fn("quant_rows", "si_add_rmsnorm_q8",
-            [_c_p, _c_p, _c_p, _c_int, _c_p, _c_p, _c_int, _c_p, _c_p, _c_p, _c_int, _c_int, _c_f, _c_p, _c_ll, _c_p])
-    _check(f(_ptr(resid), _ptr(delta), _ptr(delta2), xd, _ptr(rows), _ptr(weight), wd, _ptr(dst), _ptr(out), _ptr(scale), R, d, float(eps),
-             _ptr(ahead) if ahead_bytes else None, ahead_bytes, _stream()), f"add_rmsnorm_q8(hidden={d})")
+    rc = _fn("quant_rows", "si_add_rmsnorm_q8", _NORM_Q8_ARGS)(
+        resid.data_ptr(), _ptr(delta), _ptr(delta2), xd, _ptr(rows), weight.data_ptr(), wd, _ptr(dst), out.data_ptr(), scale.data_ptr(), R, d, eps,
+        ahead.data_ptr() if ahead_bytes else None, ahead_bytes, stream)
+    _check(rc, "add_rmsnorm_q8" if rc == 0 else f"add_rmsnorm_q8(hidden={d})")
 
 
 def swiglu_q8(gu, out, scale, group=None) -> None:
     """``swiglu`` with its output in 8 bits: y = silu(gate) * up (fp32) of the stacked projection gu [T, 2F] (fp32 or bf16, contiguous; gates
     and ups interleaved in groups of ``group`` columns, default F), scale[t] = max(max |y[t]|, 2^-100) / 448, out[t] = y[t] / scale[t] in
     e4m3 [T, F]."""
-    _here("swiglu_q8", gu, out, scale)
-    _need(out.dim() == 2 and gu.dim() == 2, "swiglu_q8: gu and out must be matrices")
-    T, F = out.shape
+    stream = _here("swiglu_q8", gu, out, scale)
+    shape = out.shape
+    if len(shape) != 2:
+        raise KernelError("swiglu_q8: gu and out must be matrices")
+    T, F = shape
     group = F if group is None else int(group)
-    _need(gu.shape == (T, 2 * F) and gu.is_contiguous(), "swiglu_q8: gu must be contiguous [T, 2F] for out [T, F]")
+    if gu.shape != (T, 2 * F) or not gu.is_contiguous():
+        raise KernelError("swiglu_q8: gu must be contiguous [T, 2F] for out [T, F]")
     _q8_out(out, scale, T, F, "swiglu_q8")
     dt = _dt(gu)
     if T == 0:
         return
-    _need(F > 0 and group > 0 and F % group == 0, "swiglu_q8: the group must divide F")
-    f = _fn("quant_rows", "si_swiglu_q8", [_c_p, _c_int, _c_p, _c_p, _c_int, _c_int, _c_int, _c_p])
-    _check(f(_ptr(gu), dt, _ptr(out), _ptr(scale), T, F, group, _stream()), f"swiglu_q8(F={F})")
+    if F <= 0 or group <= 0 or F % group:
+        raise KernelError("swiglu_q8: the group must divide F")
+    rc = _fn("quant_rows", "si_swiglu_q8", _SWIGLU_Q8_ARGS)(gu.data_ptr(), dt, out.data_ptr(), scale.data_ptr(), T, F, group, stream)
+    _check(rc, "swiglu_q8" if rc == 0 else f"swiglu_q8(F={F})")
 
 
 def quantize_q8(x, out, scale) -> None:
     """Rows to 8 bits: scale[r] = max(max |x[r]|, 2^-100) / 448 (fp32 [R]), out[r] = x[r] / scale[r] rounded to e4m3 ([R, n], contiguous).
-    ``x``: fp32 or bf16 [R, n], its rows contiguous. For a product's rows, or a weight's, whose rows are output channels."""
-    _here("quantize_q8", x, out, scale)
-    _rows_of(x, "quantize_q8: x")
-    R, n = x.shape
+    ``x``: fp32 or bf16 [R, n], its rows contiguous. For a product's rows, or a weight's, whose rows are output channels. A NaN entry becomes a
+    NaN code and leaves the others alone; with an infinite entry the scale is infinite, the entry NaN and the others zero."""
+    stream = _here("quantize_q8", x, out, scale)
+    R, n, ldx = _matrix(x, "quantize_q8: x")
     _q8_out(out, scale, R, n, "quantize_q8")
     dt = _dt(x)
     if R == 0:
         return
-    _need(n > 0, "quantize_q8: rows without entries")
-    f = _fn("quant_rows", "si_quantize_q8", [_c_p, _c_int, _c_ll, _c_p, _c_p, _c_int, _c_int, _c_p])
-    _check(f(_ptr(x), dt, _ld(x), _ptr(out), _ptr(scale), R, n, _stream()), f"quantize_q8(n={n})")
+    if n <= 0:
+        raise KernelError("quantize_q8: rows without entries")
+    rc = _fn("quant_rows", "si_quantize_q8", _ROWS_Q8_ARGS)(x.data_ptr(), dt, ldx, out.data_ptr(), scale.data_ptr(), R, n, stream)
+    _check(rc, "quantize_q8" if rc == 0 else f"quantize_q8(n={n})")
 
 
 def gemm_q8(a, a_scale, w, w_scale, out, status=None) -> None:
     """out[m, n] = a_scale[m] * w_scale[n] * sum_k a[m, k] * w[n, k]: a [M, K] and w [N, K] in e4m3 (rows contiguous), scales fp32 [M] and
     [N], out bf16 or fp32 [M, N]; sums fp32. ``status``: the status word that a kernel's bounded wait reports to."""
-    _here("gemm_q8", a, a_scale, w, w_scale, out, status)
-    _need(a.dtype == E4M3 and w.dtype == E4M3, "gemm_q8: a and w must be float8_e4m3fn")
-    _rows_of(a, "gemm_q8: a"); _rows_of(w, "gemm_q8: w"); _out_rows(out, "gemm_q8: out")
-    M, K = a.shape
-    N = w.shape[0]
-    _need(w.shape[1] == K and out.shape == (M, N), f"gemm_q8: a {tuple(a.shape)}, w {tuple(w.shape)} and out {tuple(out.shape)} do not fit")
-    _f32v(a_scale, "gemm_q8: a_scale", M); _f32v(w_scale, "gemm_q8: w_scale", N); _i32(status, "status")
+    stream = _here("gemm_q8", a, a_scale, w, w_scale, out, status)
+    if a.dtype is not E4M3 or w.dtype is not E4M3:
+        raise KernelError("gemm_q8: a and w must be float8_e4m3fn")
+    (M, K, lda), (N, kw, ldw), (mo, no, ldo) = _matrix(a, "gemm_q8: a"), _matrix(w, "gemm_q8: w"), _matrix(out, "gemm_q8: out")
+    if kw != K or mo != M or no != N:
+        raise KernelError(f"gemm_q8: a {tuple(a.shape)}, w {tuple(w.shape)} and out {tuple(out.shape)} do not fit")
+    if ldo < N:
+        raise KernelError("gemm_q8: out's rows overlap")
+    _f32_of(a_scale, M, "gemm_q8: a_scale"); _f32_of(w_scale, N, "gemm_q8: w_scale")
+    if status is not None:
+        _i32(status, "status")
     od = _dt(out)
     if M == 0 or N == 0:
         return
-    _need(K > 0, "gemm_q8: rows without entries")
-    lda, ldw = _ld(a), _ld(w)
-    if (a.data_ptr() | w.data_ptr() | lda | ldw) % 16 == 0 and lda >= K and ldw >= K and gemm_tc05_available():
-        f = _fn("gemm_q8", "si_gemm_q8", [_c_p, _c_ll, _c_p, _c_p, _c_ll, _c_p, _c_p, _c_ll, _c_int, _c_int, _c_int, _c_int, _c_p, _c_p])
-        _check(f(_ptr(a), lda, _ptr(a_scale), _ptr(w), ldw, _ptr(w_scale), _ptr(out), _ld(out), od, M, N, K, _ptr(status), _stream()),
-               f"gemm_q8(M={M}, N={N}, K={K})")
-        return
-    # rows that do not start on 16-byte boundaries
-    f = _fn("gemm_quant", "si_gemm_quant_q8", [_c_p, _c_ll, _c_p, _c_p, _c_ll, _c_p, _c_p, _c_ll, _c_int, _c_int, _c_int, _c_int, _c_p])
-    _check(f(_ptr(a), lda, _ptr(a_scale), _ptr(w), ldw, _ptr(w_scale), _ptr(out), _ld(out), od, M, N, K, _stream()),
-           f"gemm_q8(M={M}, N={N}, K={K})")
+    if K <= 0:
+        raise KernelError("gemm_q8: rows without entries")
+    pa, pw = a.data_ptr(), w.data_ptr()
+    if (pa | pw | lda | ldw) % 16 == 0 and lda >= K and ldw >= K and gemm_tc05_available():
+        rc = _fn("gemm_q8", "si_gemm_q8", _GEMM_Q8_ARGS)(pa, lda, a_scale.data_ptr(), pw, ldw, w_scale.data_ptr(), out.data_ptr(), ldo, od, M, N, K,
+                                                         _ptr(status), stream)
+    else:                                                        # rows that do not start on 16-byte boundaries
+        rc = _fn("gemm_quant", "si_gemm_quant_q8", _GEMM_Q8_ARGS[:-1])(pa, lda, a_scale.data_ptr(), pw, ldw, w_scale.data_ptr(), out.data_ptr(), ldo, od,
+                                                                       M, N, K, stream)
+    _check(rc, "gemm_q8" if rc == 0 else f"gemm_q8(M={M}, N={N}, K={K})")
 
 
 def gemm_w4(x, w, scales, zeros, group: int, out, status=None) -> None:
     """out[m, n] = sum_k x[m, k] * scales[n, k / group] * (q[n, k] - zeros[n, k / group]) with weights of four bits: x bf16 [M, K] (rows
     contiguous, K a multiple of 8), ``w`` int32 [N, K / 8], entry i of the eight in a word at bit ``W4_SHIFTS[i]`` (see ``pack_w4``); scales bf16
     [N, ceil(K / group)], zeros uint8 like them or None (8 everywhere), ``group`` 32, 64 or a multiple of 128; out bf16 or fp32 [M, N]; sums fp32.
-    ``status``: as in ``gemm_q8``."""
-    _here("gemm_w4", x, w, scales, zeros, out, status)
-    _need(x.dtype == torch.bfloat16 and w.dtype == torch.int32, "gemm_w4: x must be bfloat16, w int32 words of eight entries")
-    _rows_of(x, "gemm_w4: x"); _rows_of(w, "gemm_w4: w"); _out_rows(out, "gemm_w4: out")
-    M, K = x.shape
-    N = w.shape[0]
+    A weight times its scale is rounded to bf16 before it is multiplied, except up to eight rows with groups of 128 and more. ``status``: as in
+    ``gemm_q8``."""
+    stream = _here("gemm_w4", x, w, scales, zeros, out, status)
+    if x.dtype is not _BF16 or w.dtype is not torch.int32:
+        raise KernelError("gemm_w4: x must be bfloat16, w int32 words of eight entries")
+    (M, K, ldx), (N, words, ldw), (mo, no, ldo) = _matrix(x, "gemm_w4: x"), _matrix(w, "gemm_w4: w"), _matrix(out, "gemm_w4: out")
     group = int(group)
-    _need(K % 8 == 0 and w.shape[1] * 8 == K and out.shape == (M, N),
-          f"gemm_w4: x {tuple(x.shape)}, w {tuple(w.shape)} (words of eight) and out {tuple(out.shape)} do not fit")
-    _need(group in (32, 64) or (group > 0 and group % 128 == 0), f"gemm_w4: group {group} is not 32, 64 or a multiple of 128")
+    if words * 8 != K or mo != M or no != N:
+        raise KernelError(f"gemm_w4: x {tuple(x.shape)}, w {tuple(w.shape)} (words of eight) and out {tuple(out.shape)} do not fit")
+    if ldo < N:
+        raise KernelError("gemm_w4: out's rows overlap")
+    if group not in (32, 64) and (group <= 0 or group % 128):
+        raise KernelError(f"gemm_w4: group {group} is not 32, 64 or a multiple of 128")
     G = -(-K // group)
-    _need(scales.dtype == torch.bfloat16 and scales.is_contiguous() and scales.shape == (N, G), f"gemm_w4: scales must be contiguous bfloat16 [{N}, {G}]")
-    _need(zeros is None or (zeros.dtype == torch.uint8 and zeros.is_contiguous() and zeros.shape == (N, G)),
-          f"gemm_w4: zeros must be contiguous uint8 [{N}, {G}]")
-    _i32(status, "status")
+    if scales.dtype is not _BF16 or scales.shape != (N, G) or not scales.is_contiguous():
+        raise KernelError(f"gemm_w4: scales must be contiguous bfloat16 [{N}, {G}]")
+    if zeros is not None and (zeros.dtype is not torch.uint8 or zeros.shape != (N, G) or not zeros.is_contiguous()):
+        raise KernelError(f"gemm_w4: zeros must be contiguous uint8 [{N}, {G}]")
+    if status is not None:
+        _i32(status, "status")
     od = _dt(out)
     if M == 0 or N == 0:
         return
-    _need(K > 0, "gemm_w4: rows without entries")
-    ldx, ldw = _ld(x), _ld(w)
-    if ((x.data_ptr() | w.data_ptr()) % 16 == 0 and ldx % 8 == 0 and ldw % 4 == 0 and K % 32 == 0 and ldx >= K and ldw * 8 >= K
-            and gemm_tc05_available()):
-        f = _fn("gemm_w4", "si_gemm_w4", [_c_p, _c_ll, _c_p, _c_ll, _c_p, _c_p, _c_int, _c_p, _c_ll, _c_int, _c_int, _c_int, _c_int, _c_p, _c_p])
-        _check(f(_ptr(x), ldx, _ptr(w), ldw, _ptr(scales), _ptr(zeros), group, _ptr(out), _ld(out), od, M, N, K, _ptr(status), _stream()),
-               f"gemm_w4(M={M}, N={N}, K={K}, group={group})")
-        return
-    # rows that are not in 16-byte pieces
-    f = _fn("gemm_quant", "si_gemm_quant_w4", [_c_p, _c_ll, _c_p, _c_ll, _c_p, _c_p, _c_int, _c_p, _c_ll, _c_int, _c_int, _c_int, _c_int, _c_p])
-    _check(f(_ptr(x), ldx, _ptr(w), ldw, _ptr(scales), _ptr(zeros), group, _ptr(out), _ld(out), od, M, N, K, _stream()),
-           f"gemm_w4(M={M}, N={N}, K={K}, group={group})")
+    if K <= 0:
+        raise KernelError("gemm_w4: rows without entries")
+    px, pw = x.data_ptr(), w.data_ptr()
+    if (px | pw) % 16 == 0 and ldx % 8 == 0 and ldw % 4 == 0 and K % 32 == 0 and ldx >= K and ldw * 8 >= K and gemm_tc05_available():
+        rc = _fn("gemm_w4", "si_gemm_w4", _GEMM_W4_ARGS)(px, ldx, pw, ldw, scales.data_ptr(), _ptr(zeros), group, out.data_ptr(), ldo, od, M, N, K,
+                                                         _ptr(status), stream)
+    else:                                                        # rows that are not in 16-byte pieces
+        rc = _fn("gemm_quant", "si_gemm_quant_w4", _GEMM_W4_ARGS[:-1])(px, ldx, pw, ldw, scales.data_ptr(), _ptr(zeros), group, out.data_ptr(), ldo, od,
+                                                                       M, N, K, stream)
+    _check(rc, "gemm_w4" if rc == 0 else f"gemm_w4(M={M}, N={N}, K={K}, group={group})")
 
 
 def pack_w4(q) -> torch.Tensor:

@@ -28,6 +28,27 @@ __device__ __forceinline__ void load8(const bf16* p, float (&v)[8]) {
     v[2 * i] = f.x; v[2 * i + 1] = f.y;
   }
 }
+// Eight entries as they were loaded: bf16 take half the registers of what they are widened to.
+template <typename T> struct Raw8;
+template <> struct Raw8<bf16> {
+  uint4 r;
+  __device__ __forceinline__ void load(const bf16* p) { r = *reinterpret_cast<const uint4*>(p); }
+  __device__ __forceinline__ void get(float (&v)[8]) const {
+    const __nv_bfloat162* h = reinterpret_cast<const __nv_bfloat162*>(&r);
+#pragma unroll
+    for (int i = 0; i < 4; ++i) {
+      const float2 f = __bfloat1622float2(h[i]);
+      v[2 * i] = f.x; v[2 * i + 1] = f.y;
+    }
+  }
+};
+template <> struct Raw8<float> {
+  float4 a, b;
+  __device__ __forceinline__ void load(const float* p) { a = reinterpret_cast<const float4*>(p)[0]; b = reinterpret_cast<const float4*>(p)[1]; }
+  __device__ __forceinline__ void get(float (&v)[8]) const {
+    v[0] = a.x; v[1] = a.y; v[2] = a.z; v[3] = a.w; v[4] = b.x; v[5] = b.y; v[6] = b.z; v[7] = b.w;
+  }
+};
 __device__ __forceinline__ void store8(float* p, const float (&v)[8]) {
   reinterpret_cast<float4*>(p)[0] = make_float4(v[0], v[1], v[2], v[3]);
   reinterpret_cast<float4*>(p)[1] = make_float4(v[4], v[5], v[6], v[7]);
@@ -81,14 +102,15 @@ __global__ void __launch_bounds__(512) norm_q8_kernel(const NormArgs a, unsigned
   const size_t src = (size_t)(a.rows ? a.rows[r] : r) * width;
   const TX* d1 = (const TX*)a.delta;
   const TX* d2 = (const TX*)a.delta2;
-  float x[CHUNKS][8], e1[CHUNKS][8], e2[CHUNKS][8];
+  float x[CHUNKS][8];
+  Raw8<TX> e1[CHUNKS], e2[CHUNKS];
 #pragma unroll
   for (int c = 0; c < CHUNKS; ++c) {
     const int ch = threadIdx.x + c * blockDim.x;
     if (ch < nchunks) {
       load8(a.resid + src + ch * 8, x[c]);
-      if (d1) load8(d1 + src + ch * 8, e1[c]);
-      if (d2) load8(d2 + src + ch * 8, e2[c]);
+      if (d1) e1[c].load(d1 + src + ch * 8);
+      if (d2) e2[c].load(d2 + src + ch * 8);
     }
   }
   float ss = 0.f, top = 0.f;
@@ -96,10 +118,16 @@ __global__ void __launch_bounds__(512) norm_q8_kernel(const NormArgs a, unsigned
   for (int c = 0; c < CHUNKS; ++c) {
     const int ch = threadIdx.x + c * blockDim.x;
     if (ch < nchunks) {
+      float e[8];
+      if (d1) {
+        e1[c].get(e);
 #pragma unroll
-      for (int i = 0; i < 8; ++i) {
-        if (d1) x[c][i] += e1[c][i];
-        if (d2) x[c][i] += e2[c][i];
+        for (int i = 0; i < 8; ++i) x[c][i] += e[i];
+      }
+      if (d2) {
+        e2[c].get(e);
+#pragma unroll
+        for (int i = 0; i < 8; ++i) x[c][i] += e[i];
       }
       if (a.dst) store8(a.dst + src + ch * 8, x[c]);
       float w[8];
@@ -160,36 +188,88 @@ __global__ void norm_q8_scalar_kernel(const NormArgs a, unsigned char* __restric
   }
 }
 
-// GATED: the row's entries are silu(gate) * up of the stacked row, gate f in column (f / group) * 2 * group + f % group.
-template <typename TX, bool GATED, int CHUNKS>
-__global__ void __launch_bounds__(512) rows_q8_kernel(const TX* __restrict__ x, long long ldx, unsigned char* __restrict__ out,
-                                                      float* __restrict__ scale, int width, int group, int trigger) {
+// silu(g) * u with the quick exponential and quotient: off by 2 + 1.2 |g| units where g is negative (and exp(-g) large), by four where it is positive; zero only
+// where exp(-g) is beyond 2^126, and so g exp(g) below any code. The accurate ones took 84 us for 2,048 x 14,336 (the accurate quotient alone 50 of
+// them): at forty instructions an entry arithmetic was what bounded the kernel.
+__device__ __forceinline__ float silu_mul_q8(float g, float u) { return __fdividef(g, 1.f + __expf(-g)) * u; }
+
+// x as it is: the loaded entries stay packed in registers and are widened twice, before and after the reduction. A block goes through rows, and asks for
+// its next one before it reduces this one.
+template <typename TX, int CHUNKS>
+__global__ void __launch_bounds__(512, sizeof(TX) == 2 || CHUNKS < 4 ? 2 : 1)
+rows_q8_kernel(const TX* __restrict__ x, long long ldx, unsigned char* __restrict__ out, float* __restrict__ scale, int width, int num_rows, int trigger) {
+  __shared__ float scratch[2][64];
+  if (trigger) pdl_trigger();
+  pdl_wait();
+  const int nchunks = width >> 3;
+  Raw8<TX> raw[CHUNKS], next[CHUNKS];
+  auto load = [&](int r, Raw8<TX> (&to)[CHUNKS]) {
+    const TX* row = x + (size_t)r * ldx;
+#pragma unroll
+    for (int c = 0; c < CHUNKS; ++c) {
+      const int ch = threadIdx.x + c * blockDim.x;
+      if (ch < nchunks) to[c].load(row + ch * 8);
+    }
+  };
+  load(blockIdx.x, next);
+  int par = 0;
+  for (int r = blockIdx.x; r < num_rows; r += gridDim.x, par ^= 1) {
+#pragma unroll
+    for (int c = 0; c < CHUNKS; ++c) raw[c] = next[c];
+    if (r + (int)gridDim.x < num_rows) load(r + gridDim.x, next);
+    float top = 0.f, v[8];
+#pragma unroll
+    for (int c = 0; c < CHUNKS; ++c)
+      if ((int)(threadIdx.x + c * blockDim.x) < nchunks) {
+        raw[c].get(v);
+#pragma unroll
+        for (int i = 0; i < 8; ++i) top = fmaxf(top, fabsf(v[i]));
+      }
+    top = block_sum_max(0.f, top, scratch[par]).y;      // a buffer is written again two rows later, behind the next row's barrier
+    const float f = q8_factor(top);
+    if (threadIdx.x == 0) scale[r] = q8_scale(top);
+#pragma unroll
+    for (int c = 0; c < CHUNKS; ++c) {
+      const int ch = threadIdx.x + c * blockDim.x;
+      if (ch < nchunks) {
+        raw[c].get(v);
+#pragma unroll
+        for (int i = 0; i < 8; ++i) v[i] *= f;
+        *reinterpret_cast<uint2*>(out + (size_t)r * width + ch * 8) = q8_pack8(v);
+      }
+    }
+  }
+}
+
+// The gated activation: gate f in column (f / group) * 2 * group + f % group, its up `group` columns further.
+template <typename TX, int CHUNKS>
+__global__ void __launch_bounds__(512, 2) gated_q8_kernel(const TX* __restrict__ gu, unsigned char* __restrict__ out, float* __restrict__ scale, int width,
+                                                          int group, int trigger) {
   __shared__ float scratch[64];
   if (trigger) pdl_trigger();
   pdl_wait();
   const int r = blockIdx.x, nchunks = width >> 3;
-  const TX* row = x + (size_t)r * ldx;
-  float v[CHUNKS][8], u[CHUNKS][8];
+  const TX* row = gu + (size_t)r * 2 * width;
+  Raw8<TX> gate[CHUNKS], up[CHUNKS];
 #pragma unroll
   for (int c = 0; c < CHUNKS; ++c) {
     const int ch = threadIdx.x + c * blockDim.x;
     if (ch < nchunks) {
-      if (GATED) {
-        const int f = ch * 8, at = f / group * group + f;            // (f / group) * 2 * group + f % group
-        load8(row + at, v[c]);
-        load8(row + at + group, u[c]);
-      } else {
-        load8(row + ch * 8, v[c]);
-      }
+      const int f = ch * 8, at = f / group * group + f;              // (f / group) * 2 * group + f % group
+      gate[c].load(row + at);
+      up[c].load(row + at + group);
     }
   }
-  float top = 0.f;
+  float top = 0.f, v[CHUNKS][8];
 #pragma unroll
   for (int c = 0; c < CHUNKS; ++c)
     if ((int)(threadIdx.x + c * blockDim.x) < nchunks) {
+      float u[8];
+      gate[c].get(v[c]);
+      up[c].get(u);
 #pragma unroll
       for (int i = 0; i < 8; ++i) {
-        if (GATED) v[c][i] = silu_mul(v[c][i], u[c][i]);
+        v[c][i] = silu_mul_q8(v[c][i], u[i]);
         top = fmaxf(top, fabsf(v[c][i]));
       }
     }
@@ -216,7 +296,7 @@ __global__ void rows_q8_scalar_kernel(const TX* __restrict__ x, long long ldx, u
   auto entry = [&](int i) {
     if (!GATED) return to_f32<TX>(row[i]);
     const int at = i / group * group + i;
-    return silu_mul(to_f32<TX>(row[at]), to_f32<TX>(row[at + group]));
+    return silu_mul_q8(to_f32<TX>(row[at]), to_f32<TX>(row[at + group]));
   };
   float top = 0.f;
   for (int i = threadIdx.x; i < width; i += blockDim.x) top = fmaxf(top, fabsf(entry(i)));
@@ -228,14 +308,15 @@ __global__ void rows_q8_scalar_kernel(const TX* __restrict__ x, long long ldx, u
 
 #define Q8_MAX_VEC_WIDTH (4 * 8 * 512)
 // Threads of a row's block: what covers it in one load each, up to 512; then two or four loads each.
-static int row_threads(int width) {
+// Many rows of a norm go by half as many threads with twice the loads each, so that more blocks, in different phases, share an SM.
+static int row_threads(int width, int most = 512) {
   const int chunks = (width + 7) / 8;
-  return chunks >= 512 ? 512 : (chunks + 31) / 32 * 32;
+  return chunks >= most ? most : (chunks + 31) / 32 * 32;
 }
 
 template <typename TX, typename TW>
 static void launch_norm(const NormArgs& a, unsigned char* out, float* scale, int width, int num_rows, bool vec, cudaStream_t stream) {
-  const dim3 block(row_threads(width));
+  const dim3 block(row_threads(width, vec && num_rows >= 1024 && width <= Q8_MAX_VEC_WIDTH / 2 ? 256 : 512));
   if (!vec) {
     si_launch(norm_q8_scalar_kernel<TX, TW>, dim3(num_rows), block, 0, stream, a, out, scale, width);
     return;
@@ -274,7 +355,8 @@ SI_EXPORT int si_add_rmsnorm_q8(float* resid, const void* delta, const void* del
 
 template <typename TX, bool GATED>
 static void launch_rows(const void* x, long long ldx, void* out, float* scale, int num_rows, int width, int group, cudaStream_t stream) {
-  const dim3 grid(num_rows), block(row_threads(width));
+  const dim3 block(row_threads(width));
+  dim3 grid(num_rows);
   const TX* xp = (const TX*)x;
   unsigned char* o = (unsigned char*)out;
   const bool vec = width % 8 == 0 && width <= Q8_MAX_VEC_WIDTH && (!GATED || group % 8 == 0) && ldx % (16 / (int)sizeof(TX)) == 0 &&
@@ -284,7 +366,10 @@ static void launch_rows(const void* x, long long ldx, void* out, float* scale, i
     return;
   }
   const int per = (width / 8 + block.x - 1) / block.x, trigger = si_pdl_trigger_small(num_rows);
-#define ROWS_Q8(C) si_launch(rows_q8_kernel<TX, GATED, C>, grid, block, 0, stream, xp, ldx, o, scale, width, group, trigger)
+  const int most = si_sm_count() * (int)(1024 / block.x);          // blocks that run at once
+  if (!GATED && num_rows > most) grid.x = most;
+#define ROWS_Q8(C) do { if constexpr (GATED) si_launch(gated_q8_kernel<TX, C>, grid, block, 0, stream, xp, o, scale, width, group, trigger); \
+                        else si_launch(rows_q8_kernel<TX, C>, grid, block, 0, stream, xp, ldx, o, scale, width, num_rows, trigger); } while (0)
   if (per <= 1) ROWS_Q8(1); else if (per <= 2) ROWS_Q8(2); else ROWS_Q8(4);
 #undef ROWS_Q8
 }

@@ -24,8 +24,7 @@ def checks_alone(monkeypatch):
             return 0
         return call
 
-    monkeypatch.setattr(ops, "_here", lambda *a: None)
-    monkeypatch.setattr(ops, "_stream", lambda: 0)
+    monkeypatch.setattr(ops, "_here", lambda *a: 0)
     monkeypatch.setattr(ops, "_fn", fn)
     monkeypatch.setattr(ops, "gemm_tc05_available", lambda: True)
     return launched
@@ -144,9 +143,11 @@ def test_a_tensor_of_another_device_is_refused(monkeypatch):
             return self.index
 
     monkeypatch.setattr(ops, "_device_index", 1)
-    ops._here("x", Elsewhere(1), None)
-    with pytest.raises(ops.KernelError, match="device 0"):
-        ops._here("x", Elsewhere(1), Elsewhere(0))
+    monkeypatch.setattr(ops, "_raw_stream", lambda index: 1000 + index)
+    assert ops._here("x", Elsewhere(1), None) == 1001              # the stream of the device that kernels are launched on
+    for ts in ((Elsewhere(1), Elsewhere(0)), (Elsewhere(0), Elsewhere(0)), (Elsewhere(0), None)):
+        with pytest.raises(ops.KernelError, match="device"):
+            ops._here("x", *ts)
 
 
 @pytest.mark.parametrize("N,K", [(1, 8), (5, 64), (3, 136)])
