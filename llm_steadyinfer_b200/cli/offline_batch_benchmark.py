@@ -45,6 +45,8 @@ def parse_args(argv: Optional[List[str]] = None) -> argparse.Namespace:
     ap.add_argument("--seed", type=int, default=42)
     # what the reference takes from the environment or fixes in code
     ap.add_argument("--dtype", default="bfloat16", choices=["bfloat16", "float32"])
+    ap.add_argument("--weight-format", default=None, choices=["q8", "w4"],
+                    help="keep the layers' matrices in 8 bits (activations too) or in 4 bits by groups of 128; default: the dtype's")
     ap.add_argument("--max-model-len", type=int, default=None, help="default: longest prompt + max-gen")
     ap.add_argument("--kv-block-size", type=int, default=None, help="default 8/16/32 by mean prompt length (scheduler.cpp:11-15)")
     ap.add_argument("--num-kv-blocks", type=int, default=None)
@@ -241,11 +243,11 @@ def main(argv: Optional[List[str]] = None) -> int:
     rng = random.Random(args.seed)
     dtype = torch.bfloat16 if args.dtype == "bfloat16" else torch.float32
     if args.checkpoint:
-        model = load_model(args.checkpoint, dtype, "cuda:0")
+        model = load_model(args.checkpoint, dtype, "cuda:0", args.weight_format)
     else:
         from llm_steadyinfer_b200.config import config_from_dict
         with open(args.model_config) as f:
-            model = Model(config_from_dict(json.load(f)), dtype, "cuda:0")
+            model = Model(config_from_dict(json.load(f)), dtype, "cuda:0", args.weight_format)
         init_random(model, args.seed)
     vocab = model.spec.vocab_size
     prompts, out_lens = load_prompts(args, vocab, rng)

@@ -54,7 +54,7 @@ static int encode_u8_2d(CUtensorMap* map, const void* base, long long rows, long
 template <int STAGES, typename TO, int BN>
 __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(192)
 gemm_q8_pair_kernel(const __grid_constant__ CUtensorMap amap, const __grid_constant__ CUtensorMap bmap, const float* __restrict__ sa,
-                    const float* __restrict__ sw, TO* __restrict__ out, long long ldo, int M, int N, int K, int* status) {
+                    const float* __restrict__ sw, TO* __restrict__ out, long long ldo, int M, int N, int K, int* status, int trigger) {
   constexpr int BM = 128, BK = 128;
   constexpr int CW = BN < 128 ? BN : 128;                // columns that an epilogue thread holds at once
   constexpr int A_BYTES = BM * BK, B_BYTES = (BN / 2) * BK;
@@ -68,7 +68,7 @@ gemm_q8_pair_kernel(const __grid_constant__ CUtensorMap amap, const __grid_const
   const int pair = blockIdx.x >> 1, pairs = gridDim.x >> 1;
   const int m_tiles = (M + 2 * BM - 1) / (2 * BM), n_tiles = (N + BN - 1) / BN;
   const int tiles = m_tiles * n_tiles, nk = (K + BK - 1) / BK;
-  pdl_trigger();
+  if (trigger) pdl_trigger();                             // one block an SM: the next kernel's blocks take no block's place
   if (threadIdx.x == 0) {
 #pragma unroll
     for (int s = 0; s < STAGES; ++s) { mbar_init(&full_bar[s], 1); mbar_init(&empty_bar[s], 1); }
@@ -229,7 +229,9 @@ static int q8_pair(const Q8Call& c) {
   if (rc) return rc;
   const long long tiles = (long long)((c.M + 255) / 256) * ((c.N + BN - 1) / BN), slots = si_sm_count() / 2;
   if (tiles > 0x3fffffffLL || slots < 1) return -2;
-  si_launch(k, dim3((unsigned)(2 * (tiles < slots ? tiles : slots))), dim3(192), smem, c.stream, am, bm, c.sa, c.sw, (TO*)c.out, c.ldo, c.M, c.N, c.K, c.status);
+  const long long blocks = 2 * (tiles < slots ? tiles : slots);
+  si_launch(k, dim3((unsigned)blocks), dim3(192), smem, c.stream, am, bm, c.sa, c.sw, (TO*)c.out, c.ldo, c.M, c.N, c.K, c.status,
+            si_pdl_trigger_mode(blocks, si_sm_count()));
   return si_last_error();
 }
 

@@ -47,7 +47,7 @@ class LLM:
                  max_gen_len: int = 256, block_size: int = 16, num_blocks: Optional[int] = None,
                  max_num_batched_tokens: Union[int, str] = "adaptive", enable_prefix_cache: bool = True,
                  use_cuda_graph: bool = True, async_decode: bool = True, device: str = "cuda:0",
-                 reserve: str = "prompt"):
+                 reserve: str = "prompt", weight_format: Optional[str] = None):
         """``model``: a model folder or a built ``Model``. ``max_batch``: most requests running at
         once. ``max_seq_len``: most tokens (prompt + generated) of one request, by default the
         model's ``max_position``. ``num_blocks``: pages of the cache pool, by default
@@ -57,9 +57,13 @@ class LLM:
         step runs, the next one is already decided and launched (the tokens it draws pass to the
         next step on the device), so the host's work per step hides behind the GPU's. ``reserve``: pages
         a request must get to be admitted, its whole prompt's ("prompt", as the reference) or its first
-        portion's ("portion": more requests run than the pool holds prompts of, and later portions preempt)."""
+        portion's ("portion": more requests run than the pool holds prompts of, and later portions preempt).
+        ``weight_format``: "q8" or "w4" quantises the layers' matrices when the folder is loaded, to 8 bits (rows of activations
+        too) or to 4 bits in groups of 128 (bfloat16 Llama models; a built model has its own format)."""
         self.dtype = _dtype_of(dtype)
-        self.model = load_model(model, self.dtype, device) if isinstance(model, (str, bytes)) else model
+        if weight_format is not None and not isinstance(model, (str, bytes)):
+            raise ValueError("weight_format is for a model folder; a built model has the format it was built with")
+        self.model = load_model(model, self.dtype, device, weight_format) if isinstance(model, (str, bytes)) else model
         spec = self.model.spec
         self.max_seq_len = int(max_seq_len or spec.max_position)
         if self.max_seq_len <= 0:

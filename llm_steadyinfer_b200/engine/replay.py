@@ -14,10 +14,10 @@ from .step import ModelRunner, StepEntry
 
 class Replayer:
     def __init__(self, model_dir: str, dtype: torch.dtype, max_tokens: int, page_size: int = 16,
-                 max_requests: int = 8, device: str = "cuda:0"):
+                 max_requests: int = 8, device: str = "cuda:0", weight_format: Optional[str] = None):
         if 64 % page_size:
             raise ValueError(f"page size {page_size} must divide 64, the unit --max-tokens is counted in")
-        model = load_model(model_dir, dtype, device)
+        model = load_model(model_dir, dtype, device, weight_format)
         num_pages = max(1, -(-max_tokens // page_size))
         self.runner = ModelRunner(model, page_size=page_size, num_pages=num_pages,
                                   max_requests=max_requests, max_step_tokens=max(max_tokens, 64))

@@ -8,6 +8,7 @@ logits for every row of a mixed step and drops the prompt rows, scheduler.cpp:61
 """
 from __future__ import annotations
 
+from dataclasses import replace
 from typing import Dict, List, Optional, Tuple
 
 import torch
@@ -17,15 +18,20 @@ from ..csrc import ops
 from ..parts import Block, NormedDelta, StreamConnections, StreamDelta, SublayerGate, SummedDelta, TokenSideInput, embedder_class, feed_forward_class, mixer_class, norm_class, position_class
 from ..parts.linear import configure_library_gemm, linear
 from ..parts.norm import RMSNorm, add_to_stream
+from ..parts.quantized import quantized_layer
 from ..engine import tracing
 
 
 class Model:
-    def __init__(self, config: ModelConfig, dtype: torch.dtype, device):
+    def __init__(self, config: ModelConfig, dtype: torch.dtype, device, weight_format: Optional[str] = None):
+        """``weight_format``: "q8" or "w4" keeps the layers' matrices in 8 or 4 bits (see ``parts/quantized.py``); None: in the compute dtype."""
         if dtype not in (torch.float32, torch.bfloat16):
             raise ValueError(f"compute dtype must be float32 or bfloat16, found {dtype}")
         self.config = config
         self.spec: ModelSpec = config.model_spec()
+        self.weight_format = weight_format
+        if weight_format is not None:
+            self.spec = replace(self.spec, layers=[quantized_layer(ls, weight_format) for ls in self.spec.layers])
         self.dtype = dtype
         self.device = torch.device(device)
         configure_library_gemm()

@@ -6,3 +6,4 @@ from . import (attention, delta_rule, diff_attention, embedding, gated_recurrenc
 from .streams import StreamConnections
 from .token_side import TokenSideInput
 from .block import Block, SublayerGate, arrangement, register_arrangement
+from . import quantized  # noqa: F401

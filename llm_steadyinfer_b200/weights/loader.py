@@ -88,10 +88,10 @@ def load_weights_into(model, model_dir: str) -> None:
     model.load_weights(tensors)
 
 
-def load_model(model_dir: str, dtype: torch.dtype, device="cuda:0"):
-    """config.json picks the architecture; returns the model with its weights on the device."""
+def load_model(model_dir: str, dtype: torch.dtype, device="cuda:0", weight_format=None):
+    """config.json picks the architecture; returns the model with its weights on the device. ``weight_format``: see ``Model``."""
     from ..models import Model
     config: ModelConfig = load_config(model_dir)
-    model = Model(config, dtype, device)
+    model = Model(config, dtype, device, weight_format)
     load_weights_into(model, model_dir)
     return model

@@ -161,3 +161,39 @@ def test_pack_and_unpack(N, K):
         assert torch.equal((u >> (4 * (i // 2) + 16 * (i % 2))) & 15, q[:, i::8])
     with pytest.raises(ops.KernelError):
         ops.pack_w4(q[:, :7])
+
+
+def test_weight_formats_of_models():
+    """The layers' specs in a format, and what has none."""
+    from llm_steadyinfer_b200.config import config_from_dict
+    from llm_steadyinfer_b200.models import Model
+    from nufasun_configs import CONFIGS as OTHERS
+    from tiny_configs import TINY_A
+    for fmt, arrangement, files in (("q8", "pre_norm_q8", {"quant_rows", "gemm_q8", "gemm_quant"}), ("w4", "pre_norm", {"gemm_w4", "gemm_quant", "swiglu"})):
+        m = Model(config_from_dict(TINY_A), torch.bfloat16, "cpu", fmt)
+        assert m.weight_format == fmt and m.capturable()
+        assert {b.arrangement for b in m.blocks} == {arrangement}
+        assert {ls.mixer.kind for ls in m.spec.layers} == {"quantized_attention"}
+        assert files <= set(m.kernel_files(16))
+        assert m.weight_shapes() == Model(config_from_dict(TINY_A), torch.bfloat16, "cpu").weight_shapes()
+        with pytest.raises(ValueError, match="bfloat16"):
+            Model(config_from_dict(TINY_A), torch.float32, "cpu", fmt)
+    with pytest.raises(ValueError, match="weight_format"):
+        Model(config_from_dict(TINY_A), torch.bfloat16, "cpu", "q4")
+    other = next(iter(OTHERS.values()))
+    with pytest.raises(ValueError, match="has no form for it|goes with the arrangement"):
+        Model(config_from_dict(other[0] if isinstance(other, tuple) else other), torch.bfloat16, "cpu", "w4")
+
+
+def test_quantize_w4_on_the_cpu():
+    from llm_steadyinfer_b200.parts.quantized import quantize, quantize_w4
+    g = torch.Generator().manual_seed(1)
+    w = torch.randn(7, 200, generator=g).to(BF16) * 0.05
+    for group in (32, 64, 128, 256):
+        q = quantize_w4(w, group)
+        G = -(-200 // group)
+        assert q.scales.shape == q.zeros.shape == (7, G) and q.words.shape == (7, 25)
+        step = q.scales.double().repeat_interleave(group, 1)[:, :200]
+        assert ((q.dense().double() - w.double()).abs() <= step * (1 + 15 * 2.0 ** -8)).all()
+    with pytest.raises(ValueError, match="multiple of 8"):
+        quantize(w[:, :100].contiguous()[:, :99], "w4")
