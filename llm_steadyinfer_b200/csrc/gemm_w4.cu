@@ -21,9 +21,9 @@ struct W4Call {
 
 // ---- up to 8 rows ------------------------------------------------------------------------------------------------
 // mma.sync m16n8k16 with 16 rows of the weight matrix (a unit) as its "m" and the rows of x as its "n". A block a SM goes through its units; sixteen
-// warps take a piece of 256 entries of the unit's rows each, 4,096 a stage, and their sums of a unit are added in shared memory. All that is not
-// arithmetic is kept away from them: one TMA load brings a stage, [16 pieces][16 rows][128 bytes] (128-byte swizzle), into a ring, four more warps bring
-// the scales (and zero points), and x lies in shared memory in the order of the lanes.
+// warps take a piece of 256 entries of the unit's rows each, always the same one of the block's at most 4,096, so that a warp's part of x stays in its
+// registers. All that is not arithmetic is kept away from them: one TMA load brings a unit, [16 pieces][16 rows][128 bytes] (128-byte swizzle), into a
+// ring of stages, four more warps bring the scales (and zero points), and four add the sixteen warps' sums of a unit up and store them.
 // Lane (g, t) holds entries 32 t .. 32 t + 31 of a chunk of 128 of rows r(g) and r(g) + 8, r(g) = 4 (g mod 2) + g / 2 (neighbouring g then lie in different
 // halves of the swizzle: no bank conflict), and the same entries of row g of x. A word's four pairs are the k columns of two instructions, alike
 // for both operands. Groups of 128 and more: a chunk lies in one group, its sums are scaled by the row's number and added to the running ones, and
@@ -33,14 +33,16 @@ struct W4Call {
 // What bounds it is arithmetic: all but fp32 instructions issue every second clock, and eight weights cost three shifts, four masks and four
 // subtractions. Eight rows of 28,672 x 4,096, us: words and x by loads of the lanes, the next words on their way to registers 27.9 and, with all
 // arithmetic taken out, still 23 (a register that a load is to fill cannot be moved); words by a TMA load of every warp's own, scales by its lanes 28.3,
-// 240 instructions a chunk, 130 of them not the product's.
+// 240 instructions a chunk, 130 of them not the product's; by one TMA load a unit and warps for the scales, x in shared memory, the sums added by the same
+// warps behind a barrier 21.9, 203 instructions.
 //
-// Where x does not fit shared memory, or units are fewer than SMs, a cluster shares the units, each block with its slice of k; the sums of all units
-// wait in shared memory until the cluster meets, and each block adds up and stores every parts-th unit, in the order of the blocks.
+// More than 4,096 entries a row, or fewer units than SMs: a cluster shares the units, each block with its slice of k; the sums of all units wait in
+// shared memory until the cluster meets, and each block adds up and stores every parts-th unit, in the order of the blocks.
 #define W4_FEW_ROWS 8
 #define W4_FEW_WARPS 16
-#define W4_FEW_BRINGERS 4
-#define W4_FEW_THREADS ((W4_FEW_WARPS + W4_FEW_BRINGERS) * 32)
+#define W4_FEW_HELPERS 4                                    // warps that bring scales, and as many that add sums up
+#define W4_FEW_THREADS ((W4_FEW_WARPS + 2 * W4_FEW_HELPERS) * 32)
+#define W4_FEW_SLICE 4096
 #define W4_FEW_STAGE (16 * 2048)
 #define W4_FEW_SMEM (208 * 1024)                           // beside it the warps' sums, 16 KB
 __device__ __forceinline__ void w4_mma(float (&d)[4], unsigned a0, unsigned a1, unsigned a2, unsigned a3, unsigned b0, unsigned b1) {
@@ -76,188 +78,192 @@ __device__ __forceinline__ bool w4_wait(uint64_t* bar, unsigned parity) { return
 
 // Scales a row and stage as they lie in shared memory: one a chunk of 128, or (SMALL) one a piece of 32.
 __host__ __device__ constexpr int w4_few_scales(bool small) { return small ? 128 : 32; }
-__host__ __device__ constexpr int w4_few_stages(bool small) { return small ? 3 : 4; }
 __host__ __device__ constexpr int w4_few_stage_bytes(bool zeros, bool small) { return W4_FEW_STAGE + 16 * w4_few_scales(small) * (zeros ? 3 : 2); }
+#define W4_FEW_STAGES 4
 
 template <bool ZEROS, bool SMALL, typename TO>
 __global__ void __launch_bounds__(W4_FEW_THREADS, 1)
 gemm_w4_few_kernel(const __grid_constant__ CUtensorMap wmap, const bf16* __restrict__ x, long long ldx, const bf16* __restrict__ scales,
                    const unsigned char* __restrict__ zeros, int group, int groups, TO* __restrict__ out, long long ldo, int M, int N, int K, int slice,
-                   int pieces, int parts, int units, int* status, int trigger) {
-  constexpr int STAGES = w4_few_stages(SMALL), SC = w4_few_scales(SMALL);
+                   int parts, int units, int* status, int trigger) {
+  constexpr int STAGES = W4_FEW_STAGES, SC = w4_few_scales(SMALL);
   extern __shared__ unsigned char smem_dyn[];
   __shared__ float red[2][W4_FEW_WARPS][128];
-  __shared__ __align__(8) uint64_t full_bar[STAGES], empty_bar[STAGES];
+  __shared__ __align__(8) uint64_t full_bar[STAGES], empty_bar[STAGES], red_full[2], red_empty[2];
   const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
   unsigned char* ring = w4_smem_base(smem_dyn);
   unsigned short* sring = reinterpret_cast<unsigned short*>(ring + STAGES * W4_FEW_STAGE);     // [stage][16 rows][SC]
   unsigned char* zring = reinterpret_cast<unsigned char*>(sring + STAGES * 16 * SC);           // likewise
-  uint4* xs = reinterpret_cast<uint4*>(ring + STAGES * w4_few_stage_bytes(ZEROS, SMALL));       // [chunk][4][M rows][t]
-  float* sums = reinterpret_cast<float*>(xs + slice / 128 * 16 * M);                          // [unit][128], only where a cluster meets
+  float* sums = reinterpret_cast<float*>(ring + STAGES * w4_few_stage_bytes(ZEROS, SMALL));     // [unit][128], only where a cluster meets
   const int part = (int)cluster_cta_rank(), first = blockIdx.x / parts, stride = gridDim.x / parts;
   const int k_begin = part * slice, boxes = (min(K, k_begin + slice) - k_begin) / 256;         // K and slices are multiples of 256, none empty
-  const int mine = (units - first + stride - 1) / stride, rounds = (boxes + 15) / 16;          // units of this block (first < units), stages a unit
+  const int mine = (units - first + stride - 1) / stride;                                      // units of this block (first < units)
   if (trigger) pdl_trigger();
   if (threadIdx.x == 0) {
 #pragma unroll
-    for (int s = 0; s < STAGES; ++s) { mbar_init(&full_bar[s], 1 + W4_FEW_BRINGERS); mbar_init(&empty_bar[s], W4_FEW_WARPS); }
+    for (int s = 0; s < STAGES; ++s) { mbar_init(&full_bar[s], 1 + W4_FEW_HELPERS); mbar_init(&empty_bar[s], W4_FEW_WARPS); }
+#pragma unroll
+    for (int b = 0; b < 2; ++b) { mbar_init(&red_full[b], W4_FEW_WARPS); mbar_init(&red_empty[b], W4_FEW_HELPERS); }
     asm volatile("fence.mbarrier_init.release.cluster;\n" ::: "memory");
   }
   __syncthreads();
   bool ok = true;
-  if (warp >= W4_FEW_WARPS) {
-    const int b = warp - W4_FEW_WARPS;                      // brings the scales of rows 4 b .. 4 b + 3; the first of them the words as well
+  auto place = [&](int unit, int e, int* m, int* n) {         // row and column of sum e of a unit
+    const int ln = e >> 2, g = ln >> 2;
+    *m = (ln & 3) * 2 + (e & 1);
+    *n = (first + unit * stride) * 16 + (g & 1) * 4 + (g >> 1) + ((e >> 1) & 1) * 8;
+  };
+  if (warp >= W4_FEW_WARPS + W4_FEW_HELPERS) {                // adds the warps' sums up, in their order, a thread one
+    const int e = threadIdx.x - (W4_FEW_WARPS + W4_FEW_HELPERS) * 32;
+    pdl_wait();                                               // `out` may still be read by the kernel before
+    for (int unit = 0; unit < mine; ++unit) {
+      const int par = unit & 1;
+      ok = w4_wait(&red_full[par], (unsigned)((unit >> 1) & 1));
+      if (!ok) break;
+      float sum = 0.f;
+#pragma unroll
+      for (int v = 0; v < W4_FEW_WARPS; ++v) sum += red[par][v][e];
+      __syncwarp();
+      if (lane == 0) mbar_arrive(&red_empty[par]);
+      if (parts > 1) {
+        sums[unit * 128 + e] = sum;
+      } else {
+        int m, n;
+        place(unit, e, &m, &n);
+        if (n < N && m < M) out[(size_t)m * ldo + n] = from_f32<TO>(sum);
+      }
+    }
+  } else if (warp >= W4_FEW_WARPS) {
+    const int b = warp - W4_FEW_WARPS;                        // brings the scales of rows 4 b .. 4 b + 3; the first of them the words as well
+    const int pieces = slice / 256;
     if (b == 0 && lane == 0)
       asm volatile("cp.async.bulk.prefetch.tensor.3d.L2.global.tile [%0, {%1, %2, %3}];\n" ::"l"(&wmap), "r"(0), "r"(first * 16), "r"(k_begin / 256) : "memory");
     pdl_wait();
-    constexpr int PER = 4 * SC / 32;                        // scales a lane and stage
-    const int row = 4 * b + lane / 8, c0 = lane % 8;         // eight lanes a row
+    constexpr int PER = 4 * SC / 32;                          // scales a lane and stage
+    const int row = 4 * b + lane / 8, c0 = lane % 8;           // eight lanes a row
     int s = 0, issued = 0;
     unsigned phase = 1;
-    for (int unit = 0; unit < mine && ok; ++unit) {
+    for (int unit = 0; unit < mine; ++unit, ++issued) {
       const int n = (first + unit * stride) * 16 + row;
-      const size_t r = (size_t)(n < N ? n : 0) * groups;       // rows beyond N: words are zeros, nothing is stored
-      for (int rd = 0; rd < rounds; ++rd, ++issued) {
-        unsigned sv[PER], zv[PER];
+      const size_t r = (size_t)(n < N ? n : 0) * groups;         // rows beyond N: words are zeros, nothing is stored
+      unsigned sv[PER], zv[PER];
 #pragma unroll
-        for (int i = 0; i < PER; ++i) {                       // asked for before the stage is free
-          const int e = k_begin + rd * 4096 + (c0 + 8 * i) * (4096 / SC);
-          const int at = min(e / group, groups - 1);
-          sv[i] = w4_ld_scale(scales + r + at);
-          if (ZEROS) zv[i] = w4_ld_zero(zeros + r + at);
-        }
-        if (issued >= STAGES) ok = w4_wait(&empty_bar[s], phase);
-        if (!ok) {
-          if (lane == 0) set_status(status, SI_WAIT_LIMIT);
-          break;
-        }
-        if (b == 0 && lane == 0) {
-          mbar_expect_tx(&full_bar[s], (unsigned)pieces * 2048u);
-          tma_load_3d(ring + s * W4_FEW_STAGE, &wmap, &full_bar[s], 0, (first + unit * stride) * 16, k_begin / 256 + rd * 16);
-        }
-#pragma unroll
-        for (int i = 0; i < PER; ++i) {
-          sring[(s * 16 + row) * SC + c0 + 8 * i] = (unsigned short)sv[i];
-          if (ZEROS) zring[(s * 16 + row) * SC + c0 + 8 * i] = (unsigned char)zv[i];
-        }
-        __syncwarp();
-        if (lane == 0) mbar_arrive(&full_bar[s]);
-        if (++s == STAGES) { s = 0; phase ^= 1u; }
+      for (int i = 0; i < PER; ++i) {                           // asked for before the stage is free
+        const int at = min((k_begin + (c0 + 8 * i) * (W4_FEW_SLICE / SC)) / group, groups - 1);
+        sv[i] = w4_ld_scale(scales + r + at);
+        if (ZEROS) zv[i] = w4_ld_zero(zeros + r + at);
       }
+      if (issued >= STAGES) ok = w4_wait(&empty_bar[s], phase);
+      if (!ok) break;
+      if (b == 0 && lane == 0) {
+        mbar_expect_tx(&full_bar[s], (unsigned)pieces * 2048u);
+        tma_load_3d(ring + s * W4_FEW_STAGE, &wmap, &full_bar[s], 0, (first + unit * stride) * 16, k_begin / 256);
+      }
+#pragma unroll
+      for (int i = 0; i < PER; ++i) {
+        sring[(s * 16 + row) * SC + c0 + 8 * i] = (unsigned short)sv[i];
+        if (ZEROS) zring[(s * 16 + row) * SC + c0 + 8 * i] = (unsigned char)zv[i];
+      }
+      __syncwarp();
+      if (lane == 0) mbar_arrive(&full_bar[s]);
+      if (++s == STAGES) { s = 0; phase ^= 1u; }
     }
-    if (!ok && b == 0 && lane == 0)                           // the copies still under way, with a limit again
+    if (!ok && b == 0 && lane == 0)                             // the copies still under way, with a limit again
       for (int i = issued > STAGES ? issued - STAGES : 0; i < issued; ++i) mbar_wait(&full_bar[i % STAGES], (unsigned)((i / STAGES) & 1));
   } else {
     const int g = lane >> 2, t = lane & 3, row = (g & 1) * 4 + (g >> 1);
+    const bool busy = warp < boxes;
     pdl_wait();
-    for (int i = threadIdx.x; i < boxes * 8 * M; i += W4_FEW_WARPS * 32) {    // x: a thread takes a lane's 32 entries of a chunk
-      const int tt = i & 3, m = (i >> 2) % M, ch = (i >> 2) / M;
-      const bf16* from = x + (size_t)m * ldx + k_begin + ch * 128 + tt * 32;
+    uint4 xr[8];                                                // this warp's piece of x; a lane of a row that is not there takes row 0's: nothing of it is stored
+    {
+      const bf16* from = x + (size_t)(g < M ? g : 0) * ldx + k_begin + (busy ? warp : 0) * 256 + t * 32;
 #pragma unroll
-      for (int q = 0; q < 4; ++q) xs[((ch * 4 + q) * M + m) * 4 + tt] = w4_ld_x(from + 8 * q);
+      for (int i = 0; i < 8; ++i) xr[i] = w4_ld_x(from + (i >> 2) * 128 + (i & 3) * 8);
     }
-    asm volatile("bar.sync 1, %0;\n" ::"n"(W4_FEW_WARPS * 32) : "memory");
-    const uint4* xl = xs + (g < M ? g : 0) * 4 + t;           // a lane of a row of x that is not there takes row 0's: nothing of it is stored
-    const int x_step = 4 * M;                                 // from a word's entries to the next word's
     const unsigned char* wl = ring + warp * 2048 + row * 128;
     const int off[2] = {(t ^ row) << 4, ((4 + t) ^ row) << 4};
-    const int se = row * SC + (SMALL ? warp * 8 + t : warp * 2);      // this lane's scales of a stage: chunk h's 4 h (SMALL) or h further
-    float acc[4] = {0.f, 0.f, 0.f, 0.f};
-    int s = 0, par = 0;
+    const int se = row * SC + (SMALL ? warp * 8 + t : warp * 2);        // this lane's scales of a stage: chunk h's 4 h (SMALL) or h further
+    int s = 0;
     unsigned phase = 0;
 #pragma unroll 1
     for (int unit = 0; unit < mine; ++unit) {
-#pragma unroll 1
-      for (int rd = 0; rd < rounds; ++rd) {
-        if (ok) ok = w4_wait(&full_bar[s], phase);
-        const int bx = rd * 16 + warp;
-        if (bx < boxes) {                                     // alike for the warp
-          const unsigned char* box = wl + s * W4_FEW_STAGE;
-          const uint4* xb = xl + bx * 8 * x_step;
-          const unsigned short* sp = sring + s * 16 * SC + se;
-          const unsigned char* zp = zring + s * 16 * SC + se;
+      float acc[4] = {0.f, 0.f, 0.f, 0.f};
+      ok = w4_wait(&full_bar[s], phase);
+      if (!ok) break;
+      if (busy) {                                               // alike for the warp
+        const unsigned char* box = wl + s * W4_FEW_STAGE;
+        const unsigned short* sp = sring + s * 16 * SC + se;
+        const unsigned char* zp = zring + s * 16 * SC + se;
 #pragma unroll
-          for (int h = 0; h < 2; ++h) {
-            const int sh = SMALL ? 4 * h : h;
-            const uint4 lo = *reinterpret_cast<const uint4*>(box + off[h]), hi = *reinterpret_cast<const uint4*>(box + 1024 + off[h]);
-            const unsigned slo = sp[sh], shi = sp[8 * SC + sh];
-            const __nv_bfloat162 blo = ZEROS ? w4_bias((int)zp[sh]) : __float2bfloat162_rn(136.f);
-            const __nv_bfloat162 bhi = ZEROS ? w4_bias((int)zp[8 * SC + sh]) : __float2bfloat162_rn(136.f);
-            const unsigned lw[4] = {lo.x, lo.y, lo.z, lo.w}, hw[4] = {hi.x, hi.y, hi.z, hi.w};
-            const unsigned s0w = slo | (slo << 16), s1w = shi | (shi << 16);
-            float part0[4] = {0.f, 0.f, 0.f, 0.f};
+        for (int h = 0; h < 2; ++h) {
+          const int sh = SMALL ? 4 * h : h;
+          const uint4 lo = *reinterpret_cast<const uint4*>(box + off[h]), hi = *reinterpret_cast<const uint4*>(box + 1024 + off[h]);
+          const unsigned slo = sp[sh], shi = sp[8 * SC + sh];
+          const __nv_bfloat162 blo = ZEROS ? w4_bias((int)zp[sh]) : __float2bfloat162_rn(136.f);
+          const __nv_bfloat162 bhi = ZEROS ? w4_bias((int)zp[8 * SC + sh]) : __float2bfloat162_rn(136.f);
+          const unsigned lw[4] = {lo.x, lo.y, lo.z, lo.w}, hw[4] = {hi.x, hi.y, hi.z, hi.w};
+          const unsigned s0w = slo | (slo << 16), s1w = shi | (shi << 16);
+          float sum[4] = {0.f, 0.f, 0.f, 0.f};
 #pragma unroll
-            for (int q = 0; q < 4; ++q) {
-              const uint4 xv = xb[(h * 4 + q) * x_step];
-              unsigned a[4], c[4];
+          for (int q = 0; q < 4; ++q) {
+            const uint4 xv = xr[h * 4 + q];
+            unsigned a[4], c[4];
 #pragma unroll
-              for (int p = 0; p < 4; ++p) {
-                a[p] = w4_pair(lw[q], p, blo);
-                c[p] = w4_pair(hw[q], p, bhi);
-                if (SMALL) {
-                  const __nv_bfloat162 ra = __hmul2(*reinterpret_cast<__nv_bfloat162*>(&a[p]), *reinterpret_cast<const __nv_bfloat162*>(&s0w));
-                  const __nv_bfloat162 rc = __hmul2(*reinterpret_cast<__nv_bfloat162*>(&c[p]), *reinterpret_cast<const __nv_bfloat162*>(&s1w));
-                  a[p] = *reinterpret_cast<const unsigned*>(&ra);
-                  c[p] = *reinterpret_cast<const unsigned*>(&rc);
-                }
+            for (int p = 0; p < 4; ++p) {
+              a[p] = w4_pair(lw[q], p, blo);
+              c[p] = w4_pair(hw[q], p, bhi);
+              if (SMALL) {
+                const __nv_bfloat162 ra = __hmul2(*reinterpret_cast<__nv_bfloat162*>(&a[p]), *reinterpret_cast<const __nv_bfloat162*>(&s0w));
+                const __nv_bfloat162 rc = __hmul2(*reinterpret_cast<__nv_bfloat162*>(&c[p]), *reinterpret_cast<const __nv_bfloat162*>(&s1w));
+                a[p] = *reinterpret_cast<const unsigned*>(&ra);
+                c[p] = *reinterpret_cast<const unsigned*>(&rc);
               }
-              float (&to)[4] = SMALL ? acc : part0;
-              w4_mma(to, a[0], c[0], a[1], c[1], xv.x, xv.y);
-              w4_mma(to, a[2], c[2], a[3], c[3], xv.z, xv.w);
             }
-            if (!SMALL) {
-              const float s0 = __uint_as_float(slo << 16), s1 = __uint_as_float(shi << 16);
-              acc[0] += s0 * part0[0]; acc[1] += s0 * part0[1];
-              acc[2] += s1 * part0[2]; acc[3] += s1 * part0[3];
-            }
+            float (&to)[4] = SMALL ? acc : sum;
+            w4_mma(to, a[0], c[0], a[1], c[1], xv.x, xv.y);
+            w4_mma(to, a[2], c[2], a[3], c[3], xv.z, xv.w);
+          }
+          if (!SMALL) {
+            const float s0 = __uint_as_float(slo << 16), s1 = __uint_as_float(shi << 16);
+            acc[0] += s0 * sum[0]; acc[1] += s0 * sum[1];
+            acc[2] += s1 * sum[2]; acc[3] += s1 * sum[3];
           }
         }
-        __syncwarp();                                         // all lanes have read the stage
-        if (lane == 0) mbar_arrive(&empty_bar[s]);
-        if (++s == STAGES) { s = 0; phase ^= 1u; }
+      }
+      __syncwarp();                                             // all lanes have read the stage
+      if (lane == 0) mbar_arrive(&empty_bar[s]);
+      if (++s == STAGES) { s = 0; phase ^= 1u; }
+      const int par = unit & 1;
+      if (unit >= 2) {
+        ok = w4_wait(&red_empty[par], (unsigned)(((unit >> 1) - 1) & 1));
+        if (!ok) break;
       }
       *reinterpret_cast<float4*>(&red[par][warp][lane * 4]) = make_float4(acc[0], acc[1], acc[2], acc[3]);
-      acc[0] = acc[1] = acc[2] = acc[3] = 0.f;
-      // one barrier (of these warps) a unit: a buffer is written again two units later, behind the next unit's barrier
-      asm volatile("bar.sync 1, %0;\n" ::"n"(W4_FEW_WARPS * 32) : "memory");
-      // four lanes an output, each a quarter of the warps in order
-      const int e = threadIdx.x >> 2, v0 = (threadIdx.x & 3) * (W4_FEW_WARPS / 4);
-      float sum = 0.f;
-#pragma unroll
-      for (int v = 0; v < W4_FEW_WARPS / 4; ++v) sum += red[par][v0 + v][e];
-      sum += __shfl_xor_sync(0xffffffffu, sum, 1);
-      sum += __shfl_xor_sync(0xffffffffu, sum, 2);
-      if ((threadIdx.x & 3) == 0) {
-        if (parts > 1) {
-          sums[unit * 128 + e] = sum;
-        } else {
-          const int ln = e >> 2, gg = ln >> 2, m = (ln & 3) * 2 + (e & 1), n = (first + unit * stride) * 16 + (gg & 1) * 4 + (gg >> 1) + ((e >> 1) & 1) * 8;
-          if (n < N && m < M && ok) out[(size_t)m * ldo + n] = from_f32<TO>(sum);
-        }
-      }
-      par ^= 1;
+      __syncwarp();
+      if (lane == 0) mbar_arrive(&red_full[par]);
     }
-    if (!ok && lane == 0) set_status(status, SI_WAIT_LIMIT);
   }
+  if (!ok && lane == 0) set_status(status, SI_WAIT_LIMIT);
   __syncwarp();
   if (parts > 1) {
-    cluster_sync_all();                                       // every block's sums of its slice lie in its shared memory
-    for (int u = part; u < mine; u += parts)
-      if (threadIdx.x < 128) {
-        const int e = threadIdx.x;
-        float v[8];
+    cluster_sync_all();                                         // every block's sums of its slice lie in its shared memory
+    for (int i = threadIdx.x; i < mine * 128; i += W4_FEW_THREADS) {
+      const int unit = i >> 7, e = i & 127;
+      if (unit % parts != part) continue;
+      float v[8];
 #pragma unroll
-        for (int p = 0; p < 8; ++p) v[p] = p < parts ? w4_ld_cluster1(cluster_map_u32(sums + u * 128 + e, (unsigned)p)) : 0.f;
+      for (int p = 0; p < 8; ++p) v[p] = p < parts ? w4_ld_cluster1(cluster_map_u32(sums + i, (unsigned)p)) : 0.f;
 #pragma unroll
-        for (int p = 1; p < 8; ++p) v[0] += v[p];
-        const int ln = e >> 2, gg = ln >> 2, m = (ln & 3) * 2 + (e & 1), n = (first + u * stride) * 16 + (gg & 1) * 4 + (gg >> 1) + ((e >> 1) & 1) * 8;
-        if (n < N && m < M && ok) out[(size_t)m * ldo + n] = from_f32<TO>(v[0]);
-      }
-    cluster_sync_all();                                       // no block goes while another one reads its sums
+      for (int p = 1; p < 8; ++p) v[0] += v[p];
+      int m, n;
+      place(unit, e, &m, &n);
+      if (n < N && m < M && ok) out[(size_t)m * ldo + n] = from_f32<TO>(v[0]);
+    }
+    cluster_sync_all();                                         // no block goes while another one reads its sums
   }
 }
 
-// How k is cut for `units` units: blocks of a cluster, a block's slice, clusters, dynamic shared memory. False where it does not fit.
+// How k is cut: blocks of a cluster, a block's slice, clusters, dynamic shared memory. False where it does not fit.
 static int w4_clusters(int size);
 struct W4Few { int parts, slice, clusters; size_t smem; };
 static bool w4_few_shape(int M, int N, int K, bool zeros, bool small, W4Few* f) {
@@ -265,15 +271,14 @@ static bool w4_few_shape(int M, int N, int K, bool zeros, bool small, W4Few* f) 
   const int units = (N + 15) / 16, boxes = K / 256;
   for (int parts = 1; parts <= 8; parts *= 2) {
     const int per = (boxes + parts - 1) / parts;
-    if ((long long)per * (parts - 1) >= boxes) return false;                                  // a block without a piece
+    if ((long long)per * (parts - 1) >= boxes) return false;                                    // a block without a piece
+    if (per * 256 > W4_FEW_SLICE) continue;
     const int slots = w4_clusters(parts);
     f->parts = parts;
     f->slice = per * 256;
     f->clusters = units < slots ? units : slots;
-    const size_t sum_bytes = parts > 1 ? (size_t)((units + f->clusters - 1) / f->clusters) * 512 : 0;
-    f->smem = (size_t)w4_few_stages(small) * w4_few_stage_bytes(zeros, small) + (size_t)per * 512 * M + sum_bytes + 1024;
-    const bool more = 2 * units * parts <= si_sm_count() && per >= 2 * W4_FEW_WARPS;          // half of the SMs idle, and pieces enough to share
-    if (f->smem <= W4_FEW_SMEM && !(more && parts < 8)) return true;
+    f->smem = (size_t)W4_FEW_STAGES * w4_few_stage_bytes(zeros, small) + 1024 + (parts > 1 ? (size_t)((units + f->clusters - 1) / f->clusters) * 512 : 0);
+    return f->smem <= W4_FEW_SMEM;
   }
   return false;
 }
@@ -308,9 +313,8 @@ static int w4_few_launch(const W4Call& c, const W4Few& f) {
   auto k = gemm_w4_few_kernel<ZEROS, SMALL, TO>;
   cudaError_t e = cudaFuncSetAttribute(k, cudaFuncAttributeMaxDynamicSharedMemorySize, W4_FEW_SMEM);
   if (e != cudaSuccess) return (int)e;
-  const int pieces = f.slice / 256 < 16 ? f.slice / 256 : 16;
   CUtensorMap wm;
-  const int rc = w4_encode_pieces(&wm, c.w, c.N, c.K / 256, c.ldw, pieces);
+  const int rc = w4_encode_pieces(&wm, c.w, c.N, c.K / 256, c.ldw, f.slice / 256);
   if (rc) return rc;
   const int blocks = f.clusters * f.parts;
   cudaLaunchConfig_t cfg = {};
@@ -327,7 +331,7 @@ static int w4_few_launch(const W4Call& c, const W4Few& f) {
   attr[1].val.programmaticStreamSerializationAllowed = 1;
   cfg.attrs = attr;
   cfg.numAttrs = si_pdl_enabled() ? 2 : 1;
-  cudaLaunchKernelEx(&cfg, k, wm, c.x, c.ldx, c.scales, c.zeros, c.group, c.groups, (TO*)c.out, c.ldo, c.M, c.N, c.K, f.slice, pieces, f.parts,
+  cudaLaunchKernelEx(&cfg, k, wm, c.x, c.ldx, c.scales, c.zeros, c.group, c.groups, (TO*)c.out, c.ldo, c.M, c.N, c.K, f.slice, f.parts,
                      (c.N + 15) / 16, c.status, si_pdl_trigger_mode(blocks, si_sm_count()));
   return si_last_error();
 }
