@@ -344,13 +344,14 @@ static int w4_few(const W4Call& c, const W4Few& f) {
 
 // ---- more than 8 rows --------------------------------------------------------------------------------------------
 // out transposed: a tile is 128 rows of the weight matrix a CTA (the M of the instruction) by `bn` rows of x (its N, a multiple of 16), k steps of 128.
-// Four slots go round; to a slot belong 8 KB of words, the step's part of x, and 64 columns of tensor memory for the widened weights. Warp 0 fetches
-// x (two boxes of 64 entries, 128-byte swizzle), warp 1 the words (rows of 64 bytes, 64-byte swizzle). Warps 8 to 23 widen, four a slot, so that four
-// steps are in the making at once (all but fp32 arithmetic issues every second clock, and one warp a scheduler left more than half of those empty:
-// with eight warps a step took 1,000 clocks): a thread owns one row of the weight matrix, takes its 64 bytes out of shared memory (the swizzle spreads eight rows over all
-// banks), makes the 128 entries bf16 in registers and writes them to its lane of tensor memory, where the instruction reads its A: the widened weights
-// cost neither bandwidth nor room in shared memory. Warp 2 issues, eight instructions a step; warps 4 to 7 store. Up to 128 rows of x there are two
-// accumulators of 128 columns, beyond one of 256.
+// Four slots go round; to a slot belong the step's part of x and 64 columns of tensor memory for the widened weights. Warp 0 fetches x (two boxes of 64
+// entries, 128-byte swizzle), warp 1 the words (rows of 64 bytes, 64-byte swizzle) into eight stages of their own: with as many as slots, given back with
+// them, a load's way from memory stood between any two uses of a slot. Warps 8 to 23 widen, four a slot, so that four steps are in the making at once (all
+// but fp32 arithmetic issues every second clock, and one warp a scheduler left more than half of those empty: with eight warps a step took 1,000 clocks): a
+// thread owns one row of the weight matrix, takes its 64 bytes out of shared memory (the swizzle spreads eight rows over all banks), makes the 128 entries
+// bf16 in registers and writes them to its lane of tensor memory, where the instruction reads its A: the widened weights cost neither bandwidth nor room in
+// shared memory. Warp 2 issues, eight instructions a step; warps 4 to 7 store. Up to 128 rows of x there are two accumulators of 128 columns, beyond
+// one of 256.
 //
 // PAIR: two CTAs (a cluster) on a tile of 256 rows of the weight matrix, each with its 128 in its own tensor memory and half of the tile's rows of x; the
 // leader's instructions (cta_group::2) read both. With many rows x is what bounds a CTA alone: it takes in bn * 256 bytes of it for every 8 KB of
@@ -358,13 +359,14 @@ static int w4_few(const W4Call& c, const W4Few& f) {
 //
 // A wait costs the issuing warp 100 to 350 clocks even where there is nothing to wait for, and a commit not less than that, so there is one of each
 // a step: `ready` of a slot counts the bytes of x and the warps that widened (the leader's counts both CTAs'), and the one commit on `empty` gives back
-// all that belongs to the slot. The words' own barrier comes only after that, so the widening warps wait for it alone.
+// all that belongs to the slot.
 //
 // Blocks are persistent, one an SM. Without PAIR the k range of a tile may be cut over a cluster, whose blocks leave their sums in shared memory and
 // add a part of the rows each up over all blocks, in their order.
 #define W4_SLOTS 4
 #define W4_THREADS ((8 + 4 * W4_SLOTS) * 32)
-#define W4_TC_SMEM (W4_SLOTS * (128 * 64 + 128 * 256))      // with 128 rows of x a CTA at most
+#define W4_WORDS 8                                          // stages of words
+#define W4_TC_SMEM (W4_WORDS * 128 * 64 + W4_SLOTS * 128 * 256)      // with 128 rows of x a CTA at most
 
 __device__ __forceinline__ float4 w4_ld_cluster(unsigned cluster_addr) {
   float4 v;
@@ -381,8 +383,8 @@ __device__ __forceinline__ void w4_arrive_leader(uint64_t* bar) {
   asm volatile("mbarrier.arrive.relaxed.cluster.shared::cluster.b64 _, [%0];\n" ::"r"(cluster_map_u32(bar, 0)) : "memory");
 }
 // After a wait that ran out: the copies still under way are waited for, with a limit again, before the block's shared memory goes.
-__device__ __forceinline__ void w4_drain(uint64_t* full, int issued) {
-  for (int i = issued > W4_SLOTS ? issued - W4_SLOTS : 0; i < issued; ++i) mbar_wait(&full[i % W4_SLOTS], (unsigned)((i / W4_SLOTS) & 1));
+__device__ __forceinline__ void w4_drain(uint64_t* full, int stages, int issued) {
+  for (int i = issued > stages ? issued - stages : 0; i < issued; ++i) mbar_wait(&full[i % stages], (unsigned)((i / stages) & 1));
 }
 
 // The scales and zero points of one row of the weight matrix along its steps of 128 entries: those of a step are asked for ahead, when the
@@ -478,10 +480,10 @@ gemm_w4_tc_kernel(const __grid_constant__ CUtensorMap xmap, const __grid_constan
                   int m_tiles, int parts, int* status, int trigger) {
   constexpr int BK = 128, W_BYTES = 128 * 64, CTAS = PAIR ? 2 : 1, ROWS = 128 * CTAS, A_COL = 256;
   extern __shared__ unsigned char smem_dyn[];
-  __shared__ __align__(8) uint64_t w_full[W4_SLOTS], ready[W4_SLOTS], empty_bar[W4_SLOTS], acc_full[2], acc_empty[2];
+  __shared__ __align__(8) uint64_t w_full[W4_WORDS], w_empty[W4_WORDS], ready[W4_SLOTS], empty_bar[W4_SLOTS], acc_full[2], acc_empty[2];
   __shared__ unsigned tmem_slot;
   unsigned char* Ws = w4_smem_base(smem_dyn);
-  unsigned char* Xs = Ws + W4_SLOTS * W_BYTES;
+  unsigned char* Xs = Ws + W4_WORDS * W_BYTES;
   float* partial = reinterpret_cast<float*>(Ws);           // [bn][128] once the operands are used up (at most 128 KB)
   const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
   const int rank = PAIR ? (int)cluster_cta_rank() : 0, part = PAIR ? 0 : (int)cluster_cta_rank(), sharers = PAIR ? 2 : parts;
@@ -493,7 +495,9 @@ gemm_w4_tc_kernel(const __grid_constant__ CUtensorMap xmap, const __grid_constan
   if (trigger) pdl_trigger();
   if (threadIdx.x == 0) {
 #pragma unroll
-    for (int s = 0; s < W4_SLOTS; ++s) { mbar_init(&w_full[s], 1); mbar_init(&ready[s], 1 + 4 * CTAS); mbar_init(&empty_bar[s], 1); }
+    for (int s = 0; s < W4_SLOTS; ++s) { mbar_init(&ready[s], 1 + 4 * CTAS); mbar_init(&empty_bar[s], 1); }
+#pragma unroll
+    for (int s = 0; s < W4_WORDS; ++s) { mbar_init(&w_full[s], 1); mbar_init(&w_empty[s], 4); }
 #pragma unroll
     for (int b = 0; b < 2; ++b) { mbar_init(&acc_full[b], 1); mbar_init(&acc_empty[b], 4 * CTAS); }
     asm volatile("fence.mbarrier_init.release.cluster;\n" ::: "memory");
@@ -507,20 +511,22 @@ gemm_w4_tc_kernel(const __grid_constant__ CUtensorMap xmap, const __grid_constan
     if (lane == 0) {
       const bool is_w = warp == 1;
       if (is_w && first < tiles)
-        for (int i = 0; i < steps && i < W4_SLOTS; ++i)
+        for (int i = 0; i < steps && i < W4_WORDS; ++i)
           asm volatile("cp.async.bulk.prefetch.tensor.2d.L2.global.tile [%0, {%1, %2}];\n"
                        ::"l"(&wmap), "r"((k0 + i) * (BK / 8)), "r"(first / m_tiles * ROWS + rank * 128) : "memory");
       pdl_wait();
+      const int stages = is_w ? W4_WORDS : W4_SLOTS;
+      uint64_t* free_bar = is_w ? w_empty : empty_bar;
       int s = 0, issued = 0;
       unsigned phase = 1;
       bool ok = true;
       for (int tile = first; tile < tiles && ok; tile += stride) {
         const int y = is_w ? tile / m_tiles * ROWS + rank * 128 : tile % m_tiles * bn + rank * (bn / 2);
         for (int it = 0; it < steps; ++it, ++issued) {
-          if (issued >= W4_SLOTS && !mbar_wait(&empty_bar[s], phase)) {
+          if (issued >= stages && !mbar_wait(&free_bar[s], phase)) {
             set_status(status, SI_WAIT_LIMIT);
-            if (is_w) w4_drain(w_full, issued);
-            else if (rank == 0) w4_drain(ready, issued);
+            if (is_w) w4_drain(w_full, W4_WORDS, issued);
+            else if (rank == 0) w4_drain(ready, W4_SLOTS, issued);
             ok = false;
             break;
           }
@@ -539,7 +545,7 @@ gemm_w4_tc_kernel(const __grid_constant__ CUtensorMap xmap, const __grid_constan
               tma_load_2d(to + X_BYTES / 2, &xmap, &ready[s], (k0 + it) * BK + 64, y);
             }
           }
-          if (++s == W4_SLOTS) { s = 0; phase ^= 1u; }
+          if (++s == stages) { s = 0; phase ^= 1u; }
         }
       }
     }
@@ -582,11 +588,11 @@ gemm_w4_tc_kernel(const __grid_constant__ CUtensorMap xmap, const __grid_constan
     }
   } else if (warp >= 8) {
     const int slot = (warp - 8) >> 2, row = (warp & 3) * 32 + lane;      // four warps a slot: every fourth step is theirs
-    const unsigned char* wrow = Ws + slot * W_BYTES + row * 64;
+    const unsigned char* wrow = Ws + row * 64;
     const int swz = (row >> 1) & 3;
     const unsigned mine = tmem + ((unsigned)((warp & 3) * 32) << 16) + (unsigned)(A_COL + slot * 64);
     int at = slot;                                         // this group's next step, counted from the tile's first
-    unsigned phase = 0;
+    int stage = slot, turns = 0;                            // its words' stage, and how many steps it has made: a slot's words come to two stages in turn
     bool ok = true;
     pdl_wait();
     for (int tile = first; tile < tiles && ok; tile += stride, at -= steps) {
@@ -594,16 +600,20 @@ gemm_w4_tc_kernel(const __grid_constant__ CUtensorMap xmap, const __grid_constan
       W4Scales<ZEROS, SMALL> sc;
       sc.start(scales, zeros, n < N ? n : 0, group, groups, k0 + at);
       if (at < steps) sc.ask(W4_SLOTS);
-      for (; at < steps; at += W4_SLOTS, phase ^= 1u) {
+      for (; at < steps; at += W4_SLOTS, ++turns, stage ^= W4_SLOTS) {
         unsigned now[W4Scales<ZEROS, SMALL>::N], z[W4Scales<ZEROS, SMALL>::N];
 #pragma unroll
         for (int j = 0; j < W4Scales<ZEROS, SMALL>::N; ++j) { now[j] = sc.sv[j]; if (ZEROS) z[j] = sc.zv[j]; }
         if (at + W4_SLOTS < steps) sc.ask(W4_SLOTS);
-        ok = w4_wait(&w_full[slot], phase);                // the slot's columns are free as well: see above
+        ok = w4_wait(&w_full[stage], (unsigned)((turns >> 1) & 1));
+        if (!ok) break;
+        uint4 wv[4];
+        w4_take_row(wrow + stage * W_BYTES, swz, wv);
+        __syncwarp();
+        if (lane == 0) mbar_arrive(&w_empty[stage]);
+        if (turns > 0) ok = w4_wait(&empty_bar[slot], (unsigned)((turns - 1) & 1));
         if (!ok) break;
         tc05_fence_after_sync();
-        uint4 wv[4];
-        w4_take_row(wrow, swz, wv);
         w4_widen_row<ZEROS, SMALL>(wv, now, z, mine);
         tc05_fence_before_sync();
         __syncwarp();
