@@ -343,15 +343,14 @@ static int w4_few(const W4Call& c, const W4Few& f) {
 }
 
 // ---- more than 8 rows --------------------------------------------------------------------------------------------
-// out transposed: a tile is 128 rows of the weight matrix a CTA (the M of the instruction) by `bn` rows of x (its N, a multiple of 16), k steps of 128.
-// Four slots go round; to a slot belong the step's part of x and 64 columns of tensor memory for the widened weights. Warp 0 fetches x (two boxes of 64
-// entries, 128-byte swizzle), warp 1 the words (rows of 64 bytes, 64-byte swizzle) into eight stages of their own: with as many as slots, given back with
-// them, a load's way from memory stood between any two uses of a slot. Warps 8 to 23 widen, four a slot, so that four steps are in the making at once (all
-// but fp32 arithmetic issues every second clock, and one warp a scheduler left more than half of those empty: with eight warps a step took 1,000 clocks): a
+// out transposed: a tile is 128 rows of the weight matrix a CTA (the M of the instruction) by `bn` rows of x (its N, a multiple of 16), k steps of 256.
+// Two slots go round (three up to 64 rows of x); to a slot belong the step's part of x and 128 columns of tensor memory for the widened weights. Warp 0
+// fetches x (boxes of 64 entries, 128-byte swizzle), warp 1 the words, half a step at a time (rows of 64 bytes, 64-byte swizzle), into eight stages of
+// their own: given back with the slots, a load's way from memory stood between any two uses of one. Warps 8 to 23 widen, four to half a step, so that two
+// steps are in the making at once (all but fp32 arithmetic issues every second clock, and one warp a scheduler left more than half of those empty): a
 // thread owns one row of the weight matrix, takes its 64 bytes out of shared memory (the swizzle spreads eight rows over all banks), makes the 128 entries
 // bf16 in registers and writes them to its lane of tensor memory, where the instruction reads its A: the widened weights cost neither bandwidth nor room in
-// shared memory. Warp 2 issues, eight instructions a step; warps 4 to 7 store. Up to 128 rows of x there are two accumulators of 128 columns, beyond
-// one of 256.
+// shared memory. Warp 2 issues, sixteen instructions a step; warps 4 to 7 store. Up to 128 rows of x there are two accumulators, beyond one of 256 columns.
 //
 // PAIR: two CTAs (a cluster) on a tile of 256 rows of the weight matrix, each with its 128 in its own tensor memory and half of the tile's rows of x; the
 // leader's instructions (cta_group::2) read both. With many rows x is what bounds a CTA alone: it takes in bn * 256 bytes of it for every 8 KB of
@@ -363,10 +362,10 @@ static int w4_few(const W4Call& c, const W4Few& f) {
 //
 // Blocks are persistent, one an SM. Without PAIR the k range of a tile may be cut over a cluster, whose blocks leave their sums in shared memory and
 // add a part of the rows each up over all blocks, in their order.
-#define W4_SLOTS 4
-#define W4_THREADS ((8 + 4 * W4_SLOTS) * 32)
+#define W4_MAX_SLOTS 3
+#define W4_THREADS (24 * 32)
 #define W4_WORDS 8                                          // stages of words
-#define W4_TC_SMEM (W4_WORDS * 128 * 64 + W4_SLOTS * 128 * 256)      // with 128 rows of x a CTA at most
+#define W4_TC_SMEM (W4_WORDS * 128 * 64 + 2 * 128 * 512)    // two slots with 128 rows of x a CTA (three with 64 take less)
 
 __device__ __forceinline__ float4 w4_ld_cluster(unsigned cluster_addr) {
   float4 v;
@@ -478,24 +477,24 @@ __global__ void __launch_bounds__(W4_THREADS, 1)
 gemm_w4_tc_kernel(const __grid_constant__ CUtensorMap xmap, const __grid_constant__ CUtensorMap wmap, const bf16* __restrict__ scales,
                   const unsigned char* __restrict__ zeros, int group, int groups, TO* __restrict__ out, long long ldo, int M, int N, int K, int bn,
                   int m_tiles, int parts, int* status, int trigger) {
-  constexpr int BK = 128, W_BYTES = 128 * 64, CTAS = PAIR ? 2 : 1, ROWS = 128 * CTAS, A_COL = 256;
+  constexpr int BK = 256, W_BYTES = 128 * 64, CTAS = PAIR ? 2 : 1, ROWS = 128 * CTAS;
   extern __shared__ unsigned char smem_dyn[];
-  __shared__ __align__(8) uint64_t w_full[W4_WORDS], w_empty[W4_WORDS], ready[W4_SLOTS], empty_bar[W4_SLOTS], acc_full[2], acc_empty[2];
+  __shared__ __align__(8) uint64_t w_full[W4_WORDS], w_empty[W4_WORDS], ready[W4_MAX_SLOTS], empty_bar[W4_MAX_SLOTS], acc_full[2], acc_empty[2];
   __shared__ unsigned tmem_slot;
   unsigned char* Ws = w4_smem_base(smem_dyn);
   unsigned char* Xs = Ws + W4_WORDS * W_BYTES;
   float* partial = reinterpret_cast<float*>(Ws);           // [bn][128] once the operands are used up (at most 128 KB)
   const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
   const int rank = PAIR ? (int)cluster_cta_rank() : 0, part = PAIR ? 0 : (int)cluster_cta_rank(), sharers = PAIR ? 2 : parts;
-  const int X_BYTES = bn / CTAS * 256;
+  const int X_BYTES = bn / CTAS * 512, slots = bn <= 64 ? 3 : 2;
   const int nk = (K + BK - 1) / BK, tiles = (N + ROWS - 1) / ROWS * m_tiles;
   const int k0 = (int)((long long)nk * part / parts), steps = (int)((long long)nk * (part + 1) / parts) - k0;
   const int first = blockIdx.x / sharers, stride = gridDim.x / sharers;
-  const int nbuf = bn <= 128 ? 2 : 1;
+  const int nbuf = bn <= 128 ? 2 : 1, acc_w = bn <= 64 ? 64 : 128, a_col = bn <= 64 ? 128 : 256;      // columns of tensor memory: accumulators, then A
   if (trigger) pdl_trigger();
   if (threadIdx.x == 0) {
 #pragma unroll
-    for (int s = 0; s < W4_SLOTS; ++s) { mbar_init(&ready[s], 1 + 4 * CTAS); mbar_init(&empty_bar[s], 1); }
+    for (int s = 0; s < W4_MAX_SLOTS; ++s) { mbar_init(&ready[s], 1 + 8 * CTAS); mbar_init(&empty_bar[s], 1); }
 #pragma unroll
     for (int s = 0; s < W4_WORDS; ++s) { mbar_init(&w_full[s], 1); mbar_init(&w_empty[s], 4); }
 #pragma unroll
@@ -511,38 +510,37 @@ gemm_w4_tc_kernel(const __grid_constant__ CUtensorMap xmap, const __grid_constan
     if (lane == 0) {
       const bool is_w = warp == 1;
       if (is_w && first < tiles)
-        for (int i = 0; i < steps && i < W4_WORDS; ++i)
+        for (int i = 0; i < 2 * steps && i < W4_WORDS; ++i)
           asm volatile("cp.async.bulk.prefetch.tensor.2d.L2.global.tile [%0, {%1, %2}];\n"
-                       ::"l"(&wmap), "r"((k0 + i) * (BK / 8)), "r"(first / m_tiles * ROWS + rank * 128) : "memory");
+                       ::"l"(&wmap), "r"(k0 * (BK / 8) + i * 16), "r"(first / m_tiles * ROWS + rank * 128) : "memory");
       pdl_wait();
-      const int stages = is_w ? W4_WORDS : W4_SLOTS;
+      // the words come half a step at a time, x a whole one
+      const int stages = is_w ? W4_WORDS : slots, count = is_w ? 2 * steps : steps;
       uint64_t* free_bar = is_w ? w_empty : empty_bar;
       int s = 0, issued = 0;
       unsigned phase = 1;
       bool ok = true;
       for (int tile = first; tile < tiles && ok; tile += stride) {
         const int y = is_w ? tile / m_tiles * ROWS + rank * 128 : tile % m_tiles * bn + rank * (bn / 2);
-        for (int it = 0; it < steps; ++it, ++issued) {
+        for (int it = 0; it < count; ++it, ++issued) {
           if (issued >= stages && !mbar_wait(&free_bar[s], phase)) {
             set_status(status, SI_WAIT_LIMIT);
             if (is_w) w4_drain(w_full, W4_WORDS, issued);
-            else if (rank == 0) w4_drain(ready, W4_SLOTS, issued);
+            else if (rank == 0) w4_drain(ready, slots, issued);
             ok = false;
             break;
           }
           if (is_w) {
             mbar_expect_tx(&w_full[s], W_BYTES);
-            tma_load_2d(Ws + s * W_BYTES, &wmap, &w_full[s], (k0 + it) * (BK / 8), y);
+            tma_load_2d(Ws + s * W_BYTES, &wmap, &w_full[s], k0 * (BK / 8) + it * 16, y);
           } else {
             unsigned char* to = Xs + s * X_BYTES;
             if (rank == 0) mbar_expect_tx(&ready[s], (unsigned)(CTAS * X_BYTES));
-            if (PAIR) {
-              const unsigned bar = cluster_map_u32(&ready[s], 0);
-              tma_load_2d_pair(to, &xmap, bar, it * BK, y);
-              tma_load_2d_pair(to + X_BYTES / 2, &xmap, bar, it * BK + 64, y);
-            } else {
-              tma_load_2d(to, &xmap, &ready[s], (k0 + it) * BK, y);
-              tma_load_2d(to + X_BYTES / 2, &xmap, &ready[s], (k0 + it) * BK + 64, y);
+            const unsigned bar = cluster_map_u32(&ready[s], 0);
+#pragma unroll
+            for (int j = 0; j < 4; ++j) {
+              if (PAIR) tma_load_2d_pair(to + j * (X_BYTES / 4), &xmap, bar, it * BK + 64 * j, y);
+              else tma_load_2d(to + j * (X_BYTES / 4), &xmap, &ready[s], (k0 + it) * BK + 64 * j, y);
             }
           }
           if (++s == stages) { s = 0; phase ^= 1u; }
@@ -563,16 +561,16 @@ gemm_w4_tc_kernel(const __grid_constant__ CUtensorMap xmap, const __grid_constan
         if (local >= nbuf) ok = w4_wait(&acc_empty[d], (unsigned)((local / nbuf - 1) & 1));
         if (!ok) break;
         tc05_fence_after_sync();
-        const unsigned acc = tmem + (unsigned)(d * 128);
+        const unsigned acc = tmem + (unsigned)(d * acc_w);
         for (int it = 0; it < steps; ++it) {
           ok = w4_wait(&ready[s], phase);
           if (!ok) break;
           tc05_fence_after_sync();
           if (elect_one()) {
-            const unsigned a = tmem + (unsigned)(A_COL + s * 64);
+            const unsigned a = tmem + (unsigned)(a_col + s * 128);
 #pragma unroll
-            for (int k = 0; k < 8; ++k) {
-              const unsigned long long b = xd + (k >> 2) * (x_step / 2) + 2 * (k & 3);
+            for (int k = 0; k < 16; ++k) {
+              const unsigned long long b = xd + (k >> 2) * (x_step / 4) + 2 * (k & 3);
               if (PAIR) w4_mma_pair_tmem_a(acc, a + 8 * k, b, idesc, (it | k) != 0 ? 1u : 0u);
               else tc05_mma_bf16_tmem_a(acc, a + 8 * k, b, idesc, (it | k) != 0 ? 1u : 0u);
             }
@@ -581,43 +579,47 @@ gemm_w4_tc_kernel(const __grid_constant__ CUtensorMap xmap, const __grid_constan
           }
           __syncwarp();
           xd += x_step;
-          if (++s == W4_SLOTS) { s = 0; xd = xd0; phase ^= 1u; }
+          if (++s == slots) { s = 0; xd = xd0; phase ^= 1u; }
         }
       }
       if (!ok && lane == 0) set_status(status, SI_WAIT_LIMIT);
     }
   } else if (warp >= 8) {
-    const int slot = (warp - 8) >> 2, row = (warp & 3) * 32 + lane;      // four warps a slot: every fourth step is theirs
+    // four groups of four warps take the half steps in turn; half h of a step goes to columns 64 h of the slot
+    const int g = (warp - 8) >> 2, row = (warp & 3) * 32 + lane;
     const unsigned char* wrow = Ws + row * 64;
     const int swz = (row >> 1) & 3;
-    const unsigned mine = tmem + ((unsigned)((warp & 3) * 32) << 16) + (unsigned)(A_COL + slot * 64);
-    int at = slot;                                         // this group's next step, counted from the tile's first
-    int stage = slot, turns = 0;                            // its words' stage, and how many steps it has made: a slot's words come to two stages in turn
+    const unsigned mine = tmem + ((unsigned)((warp & 3) * 32) << 16) + (unsigned)(a_col + (g & 1) * 64);
+    int at = g;                                            // this group's next half step, counted from the tile's first
+    int stage = g, turns = 0;                              // its words' stage (two in turn), and how many it has made
+    int slot = g >> 1, uses = 0;                           // its slot, and how many times that was used before
     bool ok = true;
     pdl_wait();
-    for (int tile = first; tile < tiles && ok; tile += stride, at -= steps) {
+    for (int tile = first; tile < tiles && ok; tile += stride, at -= 2 * steps) {
       const int n = tile / m_tiles * ROWS + rank * 128 + row;
       W4Scales<ZEROS, SMALL> sc;
-      sc.start(scales, zeros, n < N ? n : 0, group, groups, k0 + at);
-      if (at < steps) sc.ask(W4_SLOTS);
-      for (; at < steps; at += W4_SLOTS, ++turns, stage ^= W4_SLOTS) {
+      sc.start(scales, zeros, n < N ? n : 0, group, groups, 2 * k0 + at);
+      if (at < 2 * steps) sc.ask(4);
+      for (; at < 2 * steps; at += 4, ++turns, stage ^= 4) {
         unsigned now[W4Scales<ZEROS, SMALL>::N], z[W4Scales<ZEROS, SMALL>::N];
 #pragma unroll
         for (int j = 0; j < W4Scales<ZEROS, SMALL>::N; ++j) { now[j] = sc.sv[j]; if (ZEROS) z[j] = sc.zv[j]; }
-        if (at + W4_SLOTS < steps) sc.ask(W4_SLOTS);
+        if (at + 4 < 2 * steps) sc.ask(4);
         ok = w4_wait(&w_full[stage], (unsigned)((turns >> 1) & 1));
         if (!ok) break;
         uint4 wv[4];
         w4_take_row(wrow + stage * W_BYTES, swz, wv);
         __syncwarp();
         if (lane == 0) mbar_arrive(&w_empty[stage]);
-        if (turns > 0) ok = w4_wait(&empty_bar[slot], (unsigned)((turns - 1) & 1));
+        if (uses > 0) ok = w4_wait(&empty_bar[slot], (unsigned)((uses - 1) & 1));
         if (!ok) break;
         tc05_fence_after_sync();
-        w4_widen_row<ZEROS, SMALL>(wv, now, z, mine);
+        w4_widen_row<ZEROS, SMALL>(wv, now, z, mine + (unsigned)(slot * 128));
         tc05_fence_before_sync();
         __syncwarp();
         if (lane == 0) { if (PAIR) w4_arrive_leader(&ready[slot]); else mbar_arrive(&ready[slot]); }
+        slot += 2;
+        if (slot >= slots) { slot -= slots; ++uses; }
       }
     }
     if (!ok && lane == 0) set_status(status, SI_WAIT_LIMIT);
@@ -638,7 +640,7 @@ gemm_w4_tc_kernel(const __grid_constant__ CUtensorMap xmap, const __grid_constan
 #pragma unroll 1
       for (int m0 = 0; m0 < bn; m0 += 32) {
         float v[32];
-        tmem_ld_32x32(tmem + lanes + (unsigned)(d * 128 + m0), v);
+        tmem_ld_32x32(tmem + lanes + (unsigned)(d * acc_w + m0), v);
         if (m0 + 32 >= bn) {                               // in registers: the issuer may have the accumulator back
           tc05_fence_before_sync();
           __syncwarp();
@@ -726,21 +728,21 @@ static int w4_clusters(int size) {
   return known[dev][size];
 }
 
-// The shape for which the busiest SM is done first, in clocks: a step is bn * 4 of the tensor cores (4,096 products a clock and SM) and 150 beside them, 800 at
-// least (instructions, a wait, a commit), and for a CTA alone what taking in its bn rows of x lasts (60 bytes a clock). Where there is one accumulator its
+// The shape for which the busiest SM is done first, in clocks: a step of 256 is bn * 8 of the tensor cores (4,096 products a clock and SM) and 200 beside them,
+// 1,000 at least (widening, a wait, a commit), and for a CTA alone what taking in its bn rows of x lasts (60 bytes a clock). Where there is one accumulator its
 // stores come on top. More and narrower tiles have to save a sixteenth: they cost more power, at whose cap long products run. us, 2,048 x 28,672 x 4,096:
 // 8 tiles of 256 361, 9 of 240 376, 11 of 192 386, 16 of 128 396; 512 x 4,096 x 14,336: 2 of 256 77, 3 of 176 69, 4 of 128 65.
 static W4Shape w4_shape(int M, int N, int K) {
-  const int nk = (K + 127) / 128, fewest = (M + 255) / 256;
+  const int nk = (K + 255) / 256, fewest = (M + 255) / 256;
   W4Shape best = {false, 128, 1, 1};
   long long least = -1;
   auto consider = [&](bool pair, int bn, int mt, int parts) {
     const long long tiles = (long long)((N + (pair ? 255 : 127)) / (pair ? 256 : 128)) * mt, slots = w4_clusters(pair ? 2 : parts);
     if (parts > 1 && tiles > slots) return;
     const int steps = (nk + parts - 1) / parts;
-    long long step = bn * 4 + 150;
-    if (step < 800) step = 800;
-    if (!pair && step < (8192 + bn * 256) / 60) step = (8192 + bn * 256) / 60;
+    long long step = bn * 8 + 200;
+    if (step < 1000) step = 1000;
+    if (!pair && step < (16384 + bn * 512) / 60) step = (16384 + bn * 512) / 60;
     const long long cost = (tiles + slots - 1) / slots * (steps * step + (bn > 128 ? 8 * bn : 300)) + 12 * bn + (parts > 1 ? 2500 : 0);
     if (least < 0 || cost * 16 < least * 15) { least = cost; best = W4Shape{pair, bn, mt, parts}; }
   };
