@@ -123,8 +123,6 @@ gemm_w4_few_kernel(const __grid_constant__ CUtensorMap wmap, const bf16* __restr
       float sum = 0.f;
 #pragma unroll
       for (int v = 0; v < W4_FEW_WARPS; ++v) sum += red[par][v][e];
-      __syncwarp();
-      if (lane == 0) mbar_arrive(&red_empty[par]);
       if (parts > 1) {
         sums[unit * 128 + e] = sum;
       } else {
@@ -132,6 +130,8 @@ gemm_w4_few_kernel(const __grid_constant__ CUtensorMap wmap, const bf16* __restr
         place(unit, e, &m, &n);
         if (n < N && m < M) out[(size_t)m * ldo + n] = from_f32<TO>(sum);
       }
+      __syncwarp();
+      if (lane == 0) mbar_arrive(&red_empty[par]);
     }
   } else if (warp >= W4_FEW_WARPS) {
     const int b = warp - W4_FEW_WARPS;                        // brings the scales of rows 4 b .. 4 b + 3; the first of them the words as well
@@ -230,9 +230,6 @@ gemm_w4_few_kernel(const __grid_constant__ CUtensorMap wmap, const bf16* __restr
           }
         }
       }
-      __syncwarp();                                             // all lanes have read the stage
-      if (lane == 0) mbar_arrive(&empty_bar[s]);
-      if (++s == STAGES) { s = 0; phase ^= 1u; }
       const int par = unit & 1;
       if (unit >= 2) {
         ok = w4_wait(&red_empty[par], (unsigned)(((unit >> 1) - 1) & 1));
@@ -240,7 +237,11 @@ gemm_w4_few_kernel(const __grid_constant__ CUtensorMap wmap, const bf16* __restr
       }
       *reinterpret_cast<float4*>(&red[par][warp][lane * 4]) = make_float4(acc[0], acc[1], acc[2], acc[3]);
       __syncwarp();
-      if (lane == 0) mbar_arrive(&red_full[par]);
+      if (lane == 0) {
+        mbar_arrive(&red_full[par]);
+        mbar_arrive(&empty_bar[s]);                             // a stage and a slot go back when what was read there has been used
+      }
+      if (++s == STAGES) { s = 0; phase ^= 1u; }
     }
   }
   if (!ok && lane == 0) set_status(status, SI_WAIT_LIMIT);
@@ -609,15 +610,16 @@ gemm_w4_tc_kernel(const __grid_constant__ CUtensorMap xmap, const __grid_constan
         if (!ok) break;
         uint4 wv[4];
         w4_take_row(wrow + stage * W_BYTES, swz, wv);
-        __syncwarp();
-        if (lane == 0) mbar_arrive(&w_empty[stage]);
         if (uses > 0) ok = w4_wait(&empty_bar[slot], (unsigned)((uses - 1) & 1));
         if (!ok) break;
         tc05_fence_after_sync();
         w4_widen_row<ZEROS, SMALL>(wv, now, z, mine + (unsigned)(slot * 128));
         tc05_fence_before_sync();
         __syncwarp();
-        if (lane == 0) { if (PAIR) w4_arrive_leader(&ready[slot]); else mbar_arrive(&ready[slot]); }
+        if (lane == 0) {
+          if (PAIR) w4_arrive_leader(&ready[slot]); else mbar_arrive(&ready[slot]);
+          mbar_arrive(&w_empty[stage]);                    // not before the words are used: reads of shared memory were seen to end up behind the wait for
+        }                                                  // the slot, after the stage's next words had come
         slot += 2;
         if (slot >= slots) { slot -= slots; ++uses; }
       }

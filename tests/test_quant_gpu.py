@@ -310,6 +310,25 @@ def test_gemm_w4_strides_and_alignment(M, ldx, ldw, shift):
         assert status.item() == 0 and torch.equal(buf[:, :N], want.to(dtype)) and (buf[:, N:] == 77).all()
 
 
+@pytest.mark.parametrize("M,N,K,group,zeros", [(12, 4096, 4096, 64, False), (100, 4096, 8192, 32, True), (200, 4096, 4096, 64, False), (700, 6144, 4096, 64, False),
+                                               (937, 2048, 8192, 32, True), (333, 4096, 4096, 128, True), (4, 4096, 8192, 32, False), (8, 28672, 2048, 128, True)])
+def test_gemm_w4_words_that_name_their_place(M, N, K, group, zeros):
+    """Weights that tell their piece of 32 entries and their row, rows of x that pick one piece each: what a slow warp reads out of a stage that has
+    already been filled again shows, with many blocks under way and rows long enough for many turns."""
+    piece = torch.arange(K, device=DEV) // 32
+    q = torch.where(torch.arange(K, device=DEV) % 2 == 0, piece & 15, piece >> 4).to(torch.uint8)
+    q = q.expand(N, K) ^ (torch.arange(N, device=DEV).to(torch.uint8) & 15)[:, None]
+    G = -(-K // group)
+    s, z = torch.ones(N, G, dtype=BF16, device=DEV), torch.full((N, G), 3, dtype=torch.uint8, device=DEV) if zeros else None
+    words = ops().pack_w4(q.contiguous())
+    x = torch.where(torch.arange(K, device=DEV) % 2 == 0, 1.0, 16.0) * (piece[None] == (torch.arange(M, device=DEV) % (K // 32))[:, None])
+    want = torch.mm(x.double(), (q.double() - (3 if zeros else 8)).t()).to(F32)
+    for _ in range(6):
+        out, status = torch.empty(M, N, device=DEV), status_word()
+        ops().gemm_w4(x.to(BF16), words, s, z, group, out, status)
+        assert status.item() == 0 and torch.equal(out, want)
+
+
 @pytest.mark.parametrize("M", [2, 40, 200])
 def test_gemm_w4_nan_stays_in_its_row_and_column(M):
     g = gen(M)
