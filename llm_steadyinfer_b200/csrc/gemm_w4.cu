@@ -65,6 +65,16 @@ __device__ __forceinline__ unsigned w4_ld_zero(const unsigned char* p) {
   asm volatile("ld.global.u8 %0, [%1];\n" : "=r"(v) : "l"(p) : "memory");
   return v;
 }
+__device__ __forceinline__ uint2 w4_ld_8(const void* p) {
+  uint2 v;
+  asm volatile("ld.global.v2.u32 {%0,%1}, [%2];\n" : "=r"(v.x), "=r"(v.y) : "l"(p) : "memory");
+  return v;
+}
+__device__ __forceinline__ unsigned w4_ld_4(const void* p) {
+  unsigned v;
+  asm volatile("ld.global.u32 %0, [%1];\n" : "=r"(v) : "l"(p) : "memory");
+  return v;
+}
 __device__ __forceinline__ float w4_ld_cluster1(unsigned cluster_addr) {
   float v;
   asm volatile("ld.shared::cluster.f32 %0, [%1];\n" : "=f"(v) : "r"(cluster_addr) : "memory");
@@ -139,30 +149,69 @@ gemm_w4_few_kernel(const __grid_constant__ CUtensorMap wmap, const bf16* __restr
     if (b == 0 && lane == 0)
       asm volatile("cp.async.bulk.prefetch.tensor.3d.L2.global.tile [%0, {%1, %2, %3}];\n" ::"l"(&wmap), "r"(0), "r"(first * 16), "r"(k_begin / 256) : "memory");
     pdl_wait();
-    constexpr int PER = 4 * SC / 32;                          // scales a lane and stage
-    const int row = 4 * b + lane / 8, c0 = lane % 8;           // eight lanes a row
     int s = 0, issued = 0;
     unsigned phase = 1;
     for (int unit = 0; unit < mine; ++unit, ++issued) {
-      const int n = (first + unit * stride) * 16 + row;
-      const size_t r = (size_t)(n < N ? n : 0) * groups;         // rows beyond N: words are zeros, nothing is stored
-      unsigned sv[PER], zv[PER];
+      const int u0 = (first + unit * stride) * 16;               // rows beyond N take row 0's scales: their words are zeros, nothing is stored
+      // a row's scales of a stage, asked for before the stage is free. SMALL: eight pieces of 32 (a row's are whole vectors: K is a multiple of 256),
+      // one scale each or one for two; else a chunk at a time, eight lanes a row
+      uint4 sw[2];
+      uint2 zw[2];
+      unsigned sv[4], zv[4];
+      if constexpr (SMALL) {
 #pragma unroll
-      for (int i = 0; i < PER; ++i) {                           // asked for before the stage is free
-        const int at = min((k_begin + (c0 + 8 * i) * (W4_FEW_SLICE / SC)) / group, groups - 1);
-        sv[i] = w4_ld_scale(scales + r + at);
-        if (ZEROS) zv[i] = w4_ld_zero(zeros + r + at);
+        for (int i = 0; i < 2; ++i) {
+          const int n = u0 + 4 * b + 2 * i + lane / 16, piece = k_begin / 32 + lane % 16 * 8;
+          const size_t r = (size_t)(n < N ? n : 0) * groups;
+          sw[i] = make_uint4(0, 0, 0, 0);
+          zw[i] = make_uint2(0, 0);
+          if (piece * 32 < K) {
+            if (group == 32) {
+              sw[i] = w4_ld_x(scales + r + piece);
+              if (ZEROS) zw[i] = w4_ld_8(zeros + r + piece);
+            } else {
+              const uint2 h = w4_ld_8(scales + r + piece / 2);
+              sw[i].x = h.x; sw[i].y = h.y;
+              if (ZEROS) zw[i].x = w4_ld_4(zeros + r + piece / 2);
+            }
+          }
+        }
+      } else {
+        const int n = u0 + 4 * b + lane / 8;
+        const size_t r = (size_t)(n < N ? n : 0) * groups;
+#pragma unroll
+        for (int i = 0; i < 4; ++i) {
+          const int at = min((k_begin + (lane % 8 + 8 * i) * 128) / group, groups - 1);
+          sv[i] = w4_ld_scale(scales + r + at);
+          if (ZEROS) zv[i] = w4_ld_zero(zeros + r + at);
+        }
       }
       if (issued >= STAGES) ok = w4_wait(&empty_bar[s], phase);
       if (!ok) break;
       if (b == 0 && lane == 0) {
         mbar_expect_tx(&full_bar[s], (unsigned)pieces * 2048u);
-        tma_load_3d(ring + s * W4_FEW_STAGE, &wmap, &full_bar[s], 0, (first + unit * stride) * 16, k_begin / 256);
+        tma_load_3d(ring + s * W4_FEW_STAGE, &wmap, &full_bar[s], 0, u0, k_begin / 256);
       }
+      if constexpr (SMALL) {
 #pragma unroll
-      for (int i = 0; i < PER; ++i) {
-        sring[(s * 16 + row) * SC + c0 + 8 * i] = (unsigned short)sv[i];
-        if (ZEROS) zring[(s * 16 + row) * SC + c0 + 8 * i] = (unsigned char)zv[i];
+        for (int i = 0; i < 2; ++i) {
+          const int at = (s * 16 + 4 * b + 2 * i + lane / 16) * SC + lane % 16 * 8;
+          if (group == 64) {                                     // one for two pieces; not sooner, the loads are still under way above
+            const uint2 h = make_uint2(sw[i].x, sw[i].y);
+            const unsigned q = zw[i].x;
+            sw[i] = make_uint4(__byte_perm(h.x, 0, 0x1010), __byte_perm(h.x, 0, 0x3232), __byte_perm(h.y, 0, 0x1010), __byte_perm(h.y, 0, 0x3232));
+            zw[i] = make_uint2(__byte_perm(q, 0, 0x1100), __byte_perm(q, 0, 0x3322));
+          }
+          *reinterpret_cast<uint4*>(sring + at) = sw[i];
+          if (ZEROS) *reinterpret_cast<uint2*>(zring + at) = zw[i];
+        }
+      } else {
+#pragma unroll
+        for (int i = 0; i < 4; ++i) {
+          const int at = (s * 16 + 4 * b + lane / 8) * SC + lane % 8 + 8 * i;
+          sring[at] = (unsigned short)sv[i];
+          if (ZEROS) zring[at] = (unsigned char)zv[i];
+        }
       }
       __syncwarp();
       if (lane == 0) mbar_arrive(&full_bar[s]);
@@ -378,7 +427,8 @@ __device__ __forceinline__ void w4_mma_pair_tmem_a(unsigned d, unsigned a, unsig
                ::"r"(d), "r"(a), "l"(b_desc), "r"(idesc), "r"(accumulate) : "memory");
 }
 // An arrival at the leader's barrier. What it orders lies in tensor memory, which the tcgen05 fences on both sides see to, so it is a relaxed one: a
-// release to the cluster waits for everything the warp has under way (the scales asked for ahead among it) and took 1,000 to 1,700 clocks a step.
+// release to the cluster waits for everything the warp has under way (the scales asked for ahead among it) and took 1,000 to 1,700 clocks a step, and
+// arrivals at home passed on by a warp of their own cost a tenth to two fifths of the whole (300 x 4,096 x 4,096: 17.7 us as it is, 23.6).
 __device__ __forceinline__ void w4_arrive_leader(uint64_t* bar) {
   asm volatile("mbarrier.arrive.relaxed.cluster.shared::cluster.b64 _, [%0];\n" ::"r"(cluster_map_u32(bar, 0)) : "memory");
 }
@@ -688,6 +738,7 @@ gemm_w4_tc_kernel(const __grid_constant__ CUtensorMap xmap, const __grid_constan
     }
     cluster_sync_all();                                    // no block goes while another one reads its sums
   }
+  __syncwarp();
   tc05_fence_before_sync();
   if (PAIR) cluster_sync_all(); else __syncthreads();       // no CTA frees tensor memory the other one's instructions use
   if (warp == 3) { if (PAIR) tmem_dealloc_pair(tmem, 512); else tmem_dealloc(tmem, 512); }
@@ -804,6 +855,7 @@ SI_EXPORT int si_gemm_w4(const void* x, long long ldx, const void* w, long long 
   c.x = (const bf16*)x; c.ldx = ldx; c.w = (const unsigned*)w; c.ldw = ldw; c.scales = (const bf16*)scales; c.zeros = (const unsigned char*)zeros;
   c.group = group; c.groups = (K - 1) / group + 1; c.out = out; c.ldo = ldo; c.M = M; c.N = N; c.K = K; c.status = status; c.stream = stream;
   W4Few f;
-  if (w4_few_shape(M, N, K, zeros != nullptr, group < 128, &f)) return out_dtype == SI_BF16 ? w4_few<bf16>(c, f) : w4_few<float>(c, f);
+  const bool wide = group >= 128 || ((uintptr_t)scales % 16 == 0 && (uintptr_t)zeros % 8 == 0);      // small groups' scales come eight at a time
+  if (wide && w4_few_shape(M, N, K, zeros != nullptr, group < 128, &f)) return out_dtype == SI_BF16 ? w4_few<bf16>(c, f) : w4_few<float>(c, f);
   return out_dtype == SI_BF16 ? w4_tc<bf16>(c) : w4_tc<float>(c);
 }

@@ -310,6 +310,25 @@ def test_gemm_w4_strides_and_alignment(M, ldx, ldw, shift):
         assert status.item() == 0 and torch.equal(buf[:, :N], want.to(dtype)) and (buf[:, N:] == 77).all()
 
 
+@pytest.mark.parametrize("M", [1, 7, 12, 150])
+@pytest.mark.parametrize("group", [32, 64, 128, 384])
+def test_gemm_w4_scales_anywhere_and_slices_of_k(M, group):
+    """Scales and zero points whose first entry lies on no boundary; rows long enough to be cut over several blocks, the last slice shorter."""
+    g = gen(M + group)
+    N, K = 176, 9984
+    words, s, z, w = w4_weight(g, N, K, group, True)
+    G = s.shape[1]
+    x = torch.randint(-2, 3, (M, K), generator=g, device=DEV).to(BF16)
+    want = torch.mm(x.double(), w.t()).to(F32)
+    for shift in (0, 1, 3):
+        sb, zb = torch.zeros(N * G + shift, dtype=BF16, device=DEV), torch.zeros(N * G + shift, dtype=torch.uint8, device=DEV)
+        sv, zv = sb[shift:].view(N, G), zb[shift:].view(N, G)
+        sv.copy_(s), zv.copy_(z)
+        out, status = torch.empty(M, N, device=DEV), status_word()
+        ops().gemm_w4(x, words, sv, zv, group, out, status)
+        assert status.item() == 0 and torch.equal(out, want)
+
+
 @pytest.mark.parametrize("M,N,K,group,zeros", [(12, 4096, 4096, 64, False), (100, 4096, 8192, 32, True), (200, 4096, 4096, 64, False), (700, 6144, 4096, 64, False),
                                                (937, 2048, 8192, 32, True), (333, 4096, 4096, 128, True), (4, 4096, 8192, 32, False), (8, 28672, 2048, 128, True)])
 def test_gemm_w4_words_that_name_their_place(M, N, K, group, zeros):
