@@ -238,10 +238,12 @@ static int q8_pair(const Q8Call& c) {
 // ---- 17 to 128 rows ----------------------------------------------------------------------------------------------
 // One pass over the weights, the product taken the other way round: `h` rows of w are the M of the instruction (one or two of 128 rows; what lies
 // in shared memory behind row h - 1 makes sums that nobody reads), the rows of a, padded to 16, its N, and the accumulator holds out
-// transposed. One block an SM, a ring of as many stages of [h x 128] of w and [rows x 128] of a as 200 KB hold. What bounds it: an SM was seen to
-// take in no more than some 62 GB/s this way, whatever is in flight, so the time is that of the SM with the most bytes, and the height h, any
-// multiple of 8 up to 256, is chosen with the cut of k so that the SMs share them evenly (q8_rows_shape). The k range of a tile may be cut over the
-// blocks of a cluster: each leaves its sums in its shared memory, and block r adds the r-th part of the rows up over all blocks, in their order.
+// transposed. One block an SM, a ring of as many stages of [h x 256] of w and [rows x 256] of a as 208 KB hold. What bounds it: a wait, the
+// instructions and a commit cost the issuing thread some 430 clocks a step whatever the step's bytes (steps of 128 took 520 in all, so 256 are
+// taken), and a block some 3 us to begin, to meet the others and to end. The height h, any multiple of 8 up to 256, is chosen with the cut of k so that the
+// SMs share the bytes evenly (q8_rows_shape). The k range of a tile may be cut over the blocks of a cluster: each leaves its sums in its shared
+// memory, and block r adds the r-th part of the rows up over all blocks, in their order. us (TB/s of the weights): 61 x 28,672 x 4,096 24.3 (4.8),
+// 61 x 4,096 x 14,336 14.2 (4.1), 61 x 6,144 x 4,096 9.8, 128 x 4,096 x 14,336 16.5.
 #define Q8_ROWS_MAX 128
 #define Q8_ROWS_SMEM (208 * 1024)
 #define Q8_ROWS_MAX_STAGES 8
@@ -285,7 +287,7 @@ gemm_q8_rows_kernel(const __grid_constant__ CUtensorMap amap, const __grid_const
   __syncthreads();
   tc05_fence_after_sync();
   const unsigned tmem = tmem_slot;
-  // Stages and phases are counted along: a division a step, in the one thread that feeds a pipeline, cost as much as the step (see above).
+  // Stages and phases are counted along: a division a step, in the one thread that feeds a pipeline, cost 80 clocks a step.
   if (warp < 2) {                                          // warp 0 fetches w, warp 1 a: each boxes of its own
     if (lane == 0) {
       const CUtensorMap* map = warp == 0 ? &wmap : &amap;

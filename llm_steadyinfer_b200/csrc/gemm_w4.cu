@@ -31,10 +31,12 @@ struct W4Call {
 // it at most), as with more rows.
 //
 // What bounds it is arithmetic: all but fp32 instructions issue every second clock, and eight weights cost three shifts, four masks and four
-// subtractions. Eight rows of 28,672 x 4,096, us: words and x by loads of the lanes, the next words on their way to registers 27.9 and, with all
-// arithmetic taken out, still 23 (a register that a load is to fill cannot be moved); words by a TMA load of every warp's own, scales by its lanes 28.3,
-// 240 instructions a chunk, 130 of them not the product's; by one TMA load a unit and warps for the scales, x in shared memory, the sums added by the same
-// warps behind a barrier 21.9, 203 instructions.
+// subtractions. Eight rows of 28,672 x 4,096 take 16.8 us (3.5 TB/s), 17.5 with zero points, 18.4 and 20.1 with groups of 64 or 32. Other forms, us: words
+// and x by loads of the lanes, the next words on their way to registers 27.9 and, with all arithmetic taken out, still 23 (a register that a load is to fill
+// cannot be moved); words by a TMA load of every warp's own, scales by its lanes 28.3, 240 instructions a chunk, 130 of them not the product's; by one TMA
+// load a unit and warps for the scales, x in shared memory, the sums added by the same warps behind a barrier 21.9, 203 instructions. Sums that start at
+// -(128 + z) times those of x, without the subtractions: 16.6, but 3.6 for 3.4 at 2,048 x 2,048, and an infinity in x gives NaN. Scales asked for three
+// units ahead: 16.7.
 //
 // More than 4,096 entries a row, or fewer units than SMs: a cluster shares the units, each block with its slice of k; the sums of all units wait in
 // shared memory until the cluster meets, and each block adds up and stores every parts-th unit, in the order of the blocks.
@@ -404,7 +406,7 @@ static int w4_few(const W4Call& c, const W4Few& f) {
 //
 // PAIR: two CTAs (a cluster) on a tile of 256 rows of the weight matrix, each with its 128 in its own tensor memory and half of the tile's rows of x; the
 // leader's instructions (cta_group::2) read both. With many rows x is what bounds a CTA alone: it takes in bn * 256 bytes of it for every 8 KB of
-// words, and an SM was seen to take in 50 to 80 GB/s (937 x 4,096 x 14,336: 97 us alone).
+// words, and an SM was seen to take in 50 to 80 GB/s (937 x 4,096 x 14,336: 81 us, 105 alone).
 //
 // A wait costs the issuing warp 100 to 350 clocks even where there is nothing to wait for, and a commit not less than that, so there is one of each
 // a step: `ready` of a slot counts the bytes of x and the warps that widened (the leader's counts both CTAs'), and the one commit on `empty` gives back
@@ -783,8 +785,11 @@ static int w4_clusters(int size) {
 
 // The shape for which the busiest SM is done first, in clocks: a step of 256 is bn * 8 of the tensor cores (4,096 products a clock and SM) and 200 beside them,
 // 1,000 at least (widening, a wait, a commit), and for a CTA alone what taking in its bn rows of x lasts (60 bytes a clock). Where there is one accumulator its
-// stores come on top. More and narrower tiles have to save a sixteenth: they cost more power, at whose cap long products run. us, 2,048 x 28,672 x 4,096:
-// 8 tiles of 256 361, 9 of 240 376, 11 of 192 386, 16 of 128 396; 512 x 4,096 x 14,336: 2 of 256 77, 3 of 176 69, 4 of 128 65.
+// stores come on top. More and narrower tiles have to save a sixteenth: they cost more power, at whose cap long products run. us, the rule's choice first
+// (P: two CTAs a tile, then columns and cuts of k): 16 x 4,096 x 4,096 16/4 8.1, 16/2 9.5, 16/1 13.8; 61 x 6,144 x 4,096 64/2 11.3, 64/1 15.4; 128 x
+// 28,672 x 4,096 P128 31.6, 128/1 33.3; 128 x 4,096 x 14,336 128/4 20.5, 64/2 25.4; 200 x 4,096 x 14,336 112/2 28.6, P64 43.3; 300 x 4,096 x 4,096 P80 18.0,
+// 80/1 17.5; 512 x 4,096 x 14,336 P128 52.5, 128/1 55.2, P176 57.6, P256 75.5; 937 x 4,096 x 14,336 P240 81, P112 100; 2,048 x 28,672 x 4,096 P256 363, P128
+// 357, P192 371.
 static W4Shape w4_shape(int M, int N, int K) {
   const int nk = (K + 255) / 256, fewest = (M + 255) / 256;
   W4Shape best = {false, 128, 1, 1};
