@@ -47,15 +47,16 @@ static int encode_u8_2d(CUtensorMap* map, const void* base, long long rows, long
   return r == CUDA_SUCCESS ? 0 : 1000 + (int)r;
 }
 
-// ---- more than 128 rows ------------------------------------------------------------------------------------------
-// The pipeline of gemm_tc05.cu's pair kernel with e4m3 operands: a k step is 128 entries (128 bytes a row, the swizzle's span), four
-// instructions of K = 32. Two CTAs (a cluster) take a tile of 256 x BN: each fetches its 128 rows of a and BN / 2 of w a step, the leader issues
+// ---- many rows ------------------------------------------------------------------------------------------
+// The pipeline of gemm_tc05.cu's pair kernel with e4m3 operands: boxes of 128 entries (128 bytes a row, the swizzle's span), four instructions of
+// K = 32 each. A k step is one box where the tile has 256 columns, else two: a wait, a commit and the loop cost some 430 clocks a step, which the instructions
+// of narrow tiles do not fill (256 x 4,096 x 14,336, 64 columns: 33.7 us with one box, 23.9 with two; 2,048 x 6,144 x 4,096, 256 columns: 39 and 45). Two CTAs (a cluster) take a tile of 256 x BN: each fetches its 128 rows of a and BN / 2 of w a step, the leader issues
 // over both CTAs' shared memory, each CTA stores its 128 rows. Two accumulators in tensor memory: a tile is stored while the next one runs.
-template <int STAGES, typename TO, int BN>
+template <int STAGES, typename TO, int BN, int BK>
 __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(192)
-gemm_q8_pair_kernel(const __grid_constant__ CUtensorMap amap, const __grid_constant__ CUtensorMap bmap, const float* __restrict__ sa,
-                    const float* __restrict__ sw, TO* __restrict__ out, long long ldo, int M, int N, int K, int* status, int trigger) {
-  constexpr int BM = 128, BK = 128;
+gemm_q8_pair_kernel(const __grid_constant__ CUtensorMap amap, const __grid_constant__ CUtensorMap bmap, const float* sa,
+                    const float* sw, TO* __restrict__ out, long long ldo, int M, int N, int K, int* status, int trigger) {
+  constexpr int BM = 128, BOXES = BK / 128;               // boxes of 128 entries a step
   constexpr int CW = BN < 128 ? BN : 128;                // columns that an epilogue thread holds at once
   constexpr int A_BYTES = BM * BK, B_BYTES = (BN / 2) * BK;
   extern __shared__ u8 smem_dyn[];
@@ -83,23 +84,27 @@ gemm_q8_pair_kernel(const __grid_constant__ CUtensorMap amap, const __grid_const
   const unsigned tmem = tmem_slot;
   if (warp == 0) {
     if (lane == 0) {
-      for (int kb = 0; kb < nk && kb < STAGES; ++kb) tma_prefetch_2d(&bmap, kb * BK, (pair / m_tiles) * BN + (int)rank * (BN / 2));
+      for (int kb = 0; kb < BOXES * nk && kb < BOXES * STAGES; ++kb) tma_prefetch_2d(&bmap, kb * 128, (pair / m_tiles) * BN + (int)rank * (BN / 2));
       pdl_wait();
-      int it = 0;
+      int it = 0, s = 0;
+      unsigned phase = 1;                                // a stage's first use needs no wait
       bool ok = true;
       for (int tile = pair; tile < tiles && ok; tile += pairs) {
         const int m0 = (tile % m_tiles) * 2 * BM + (int)rank * BM, n0 = (tile / m_tiles) * BN + (int)rank * (BN / 2);
         for (int kb = 0; kb < nk; ++kb, ++it) {
-          const int s = it % STAGES;
-          if (it >= STAGES && !mbar_wait(&empty_bar[s], (unsigned)(((it / STAGES) - 1) & 1))) {
+          if (it >= STAGES && !mbar_wait(&empty_bar[s], phase)) {
             set_status(status, SI_WAIT_LIMIT);
             ok = false;
             break;
           }
           const unsigned bar = cluster_map_u32(&full_bar[s], 0);
           if (rank == 0) mbar_expect_tx(&full_bar[s], 2 * (A_BYTES + B_BYTES));
-          tma_load_2d_pair(Bs + s * B_BYTES, &bmap, bar, kb * BK, n0);
-          tma_load_2d_pair(As + s * A_BYTES, &amap, bar, kb * BK, m0);
+#pragma unroll
+          for (int j = 0; j < BOXES; ++j) {
+            tma_load_2d_pair(Bs + s * B_BYTES + j * (B_BYTES / BOXES), &bmap, bar, kb * BK + j * 128, n0);
+            tma_load_2d_pair(As + s * A_BYTES + j * (A_BYTES / BOXES), &amap, bar, kb * BK + j * 128, m0);
+          }
+          if (++s == STAGES) { s = 0; phase ^= 1u; }
         }
       }
       if (!ok && rank == 0) drain_copies(full_bar, STAGES, it);
@@ -108,7 +113,8 @@ gemm_q8_pair_kernel(const __grid_constant__ CUtensorMap amap, const __grid_const
     if (rank == 0) {
       constexpr unsigned idesc = q8_idesc(2 * BM, BN);
       const unsigned long long ad0 = umma_desc_sw128(As, 16, 1024), bd0 = umma_desc_sw128(Bs, 16, 1024);
-      int it = 0, local = 0;
+      int s = 0, local = 0;
+      unsigned phase = 0;
       bool ok = true;
       for (int tile = pair; tile < tiles && ok; tile += pairs, ++local) {
         const int buf = local & 1;
@@ -116,19 +122,20 @@ gemm_q8_pair_kernel(const __grid_constant__ CUtensorMap amap, const __grid_const
         if (!ok) break;
         tc05_fence_after_sync();
         const unsigned acc = tmem + buf * BN;
-        for (int kb = 0; kb < nk; ++kb, ++it) {
-          const int s = it % STAGES;
-          ok = mbar_wait_warp(&full_bar[s], (unsigned)((it / STAGES) & 1));
+        for (int kb = 0; kb < nk; ++kb) {
+          ok = mbar_wait_warp(&full_bar[s], phase);
           if (!ok) break;
           tc05_fence_after_sync();
           const unsigned long long ad = ad0 + (unsigned)s * (A_BYTES / 16), bd = bd0 + (unsigned)s * (B_BYTES / 16);
           if (elect_one()) {
 #pragma unroll
-            for (int k = 0; k < BK / 32; ++k) q8_mma_pair(acc, ad + 2 * k, bd + 2 * k, idesc, (kb | k) != 0 ? 1u : 0u);
+            for (int k = 0; k < BK / 32; ++k)
+              q8_mma_pair(acc, ad + (k >> 2) * (A_BYTES / BOXES / 16) + 2 * (k & 3), bd + (k >> 2) * (B_BYTES / BOXES / 16) + 2 * (k & 3), idesc, (kb | k) != 0 ? 1u : 0u);
             tc05_commit_pair(&empty_bar[s], 3);
             if (kb == nk - 1) tc05_commit_pair(&acc_full[buf], 3);
           }
           __syncwarp();
+          if (++s == STAGES) { s = 0; phase ^= 1u; }
         }
       }
       if (!ok && lane == 0) set_status(status, SI_WAIT_LIMIT);
@@ -197,16 +204,17 @@ gemm_q8_pair_kernel(const __grid_constant__ CUtensorMap amap, const __grid_const
   if (warp == 1) tmem_dealloc_pair(tmem, 2 * BN);
 }
 
-// Columns of a pair's tile, as for bf16 (gemm_tc05.cu): a narrower tile where tiles of 256 leave most SMs idle and it saves a fifth of the
-// rows that are fetched one round after the other.
-static int q8_pair_columns(int M, int N) {
-  const long long slots = si_sm_count() / 2, m_tiles = (M + 255) / 256;
-  if (m_tiles * ((N + 255) / 256) > slots) return 256;
-  long long least = 128 + 256 / 2;
+// Columns of a pair's tile: those for which the busiest pair is done first. In clocks: 256 entries of k take 1,120, 750 or 630 with tiles of 256, 128 and
+// 64 columns, what comes before and after them 15,800, 10,560 and 9,300 once. us with 64, 128, 256: 512 x 4,096 x 14,336 41, 28, 42; 512 x 2,048 x
+// 2,048 7.7, 8.1, 12.6; 1,024 x 6,144 x 4,096 36, 24, 28; 1,024 x 4,096 x 14,336 78, 50, 46; 2,048 x 6,144 x 4,096 70, 52, 39.
+static int q8_pair_columns(int M, int N, int K, long long* cost) {
+  const long long slots = si_sm_count() / 2, m_tiles = (M + 255) / 256, nk = (K + 255) / 256;
   int best = 256;
-  for (int bn = 128; bn >= 64; bn /= 2) {
-    const long long tiles = m_tiles * ((N + bn - 1) / bn), cost = (tiles + slots - 1) / slots * (128 + bn / 2);
-    if (cost < least && cost * 5 <= (128 + 256 / 2) * 4) { least = cost; best = bn; }
+  *cost = -1;
+  for (int bn = 256; bn >= 64; bn /= 2) {
+    const long long rounds = (m_tiles * ((N + bn - 1) / bn) + slots - 1) / slots;
+    const long long c = rounds * nk * (bn == 256 ? 1120 : bn == 128 ? 750 : 630) + (bn == 256 ? 15800 : bn == 128 ? 10560 : 9300);
+    if (*cost < 0 || c < *cost) { *cost = c; best = bn; }
   }
   return best;
 }
@@ -218,9 +226,9 @@ struct Q8Call {
 
 template <typename TO, int BN>
 static int q8_pair(const Q8Call& c) {
-  constexpr int STAGES = BN == 256 ? 6 : BN == 128 ? 8 : 10;
-  const size_t smem = (size_t)STAGES * (128 * 128 + BN / 2 * 128) + 1024;
-  auto k = gemm_q8_pair_kernel<STAGES, TO, BN>;
+  constexpr int BK = BN == 256 ? 128 : 256, STAGES = BN == 256 ? 6 : BN == 128 ? 4 : 5;
+  const size_t smem = (size_t)STAGES * (128 + BN / 2) * BK + 1024;
+  auto k = gemm_q8_pair_kernel<STAGES, TO, BN, BK>;
   cudaError_t e = cudaFuncSetAttribute(k, cudaFuncAttributeMaxDynamicSharedMemorySize, (int)smem);
   if (e != cudaSuccess) return (int)e;
   CUtensorMap am, bm;
@@ -235,7 +243,7 @@ static int q8_pair(const Q8Call& c) {
   return si_last_error();
 }
 
-// ---- 17 to 128 rows ----------------------------------------------------------------------------------------------
+// ---- 17 to 256 rows ----------------------------------------------------------------------------------------------
 // One pass over the weights, the product taken the other way round: `h` rows of w are the M of the instruction (one or two of 128 rows; what lies
 // in shared memory behind row h - 1 makes sums that nobody reads), the rows of a, padded to 16, its N, and the accumulator holds out
 // transposed. One block an SM, a ring of as many stages of [h x 256] of w and [rows x 256] of a as 208 KB hold. What bounds it: a wait, the
@@ -244,7 +252,7 @@ static int q8_pair(const Q8Call& c) {
 // SMs share the bytes evenly (q8_rows_shape). The k range of a tile may be cut over the blocks of a cluster: each leaves its sums in its shared
 // memory, and block r adds the r-th part of the rows up over all blocks, in their order. us (TB/s of the weights): 61 x 28,672 x 4,096 24.3 (4.8),
 // 61 x 4,096 x 14,336 14.2 (4.1), 61 x 6,144 x 4,096 9.8, 128 x 4,096 x 14,336 16.5.
-#define Q8_ROWS_MAX 128
+#define Q8_ROWS_MAX 256
 #define Q8_ROWS_SMEM (208 * 1024)
 #define Q8_ROWS_MAX_STAGES 8
 __device__ __forceinline__ float4 ld_cluster_f32x4(unsigned cluster_addr) {
@@ -260,8 +268,8 @@ __host__ __device__ inline int q8_rows_stages(int h, int mpad) {
 
 template <typename TO>
 __global__ void __launch_bounds__(352, 1)
-gemm_q8_rows_kernel(const __grid_constant__ CUtensorMap amap, const __grid_constant__ CUtensorMap wmap, const float* __restrict__ sa,
-                    const float* __restrict__ sw, TO* __restrict__ out, long long ldo, int M, int N, int K, int h, int parts, int* status, int trigger) {
+gemm_q8_rows_kernel(const __grid_constant__ CUtensorMap amap, const __grid_constant__ CUtensorMap wmap, const float* sa,
+                    const float* sw, TO* __restrict__ out, long long ldo, int M, int N, int K, int h, int parts, int* status, int trigger) {
   constexpr int BK = 256;                                  // two boxes of 128 entries: a wait and a commit for eight instructions
   extern __shared__ u8 smem_dyn[];
   __shared__ __align__(8) uint64_t full_bar[Q8_ROWS_MAX_STAGES], empty_bar[Q8_ROWS_MAX_STAGES], acc_full;
@@ -271,11 +279,11 @@ gemm_q8_rows_kernel(const __grid_constant__ CUtensorMap amap, const __grid_const
   const int mpad = (M + 15) & ~15, W_BYTES = h * BK, A_BYTES = mpad * BK, STAGES = q8_rows_stages(h, mpad);
   u8* Ws = smem;
   u8* As = smem + STAGES * W_BYTES;
-  float* partial = reinterpret_cast<float*>(smem);         // [mpad][h] once the operands are used up (at most 128 KB)
+  float* partial = reinterpret_cast<float*>(smem);         // [mpad][h] once the operands are used up
   const int nk = (K + BK - 1) / BK, halves = h > 128 ? 2 : 1;
   const int part = (int)cluster_cta_rank(), n0 = (int)(blockIdx.x / parts) * h;
   const int k0 = (int)((long long)nk * part / parts), k1 = (int)((long long)nk * (part + 1) / parts), steps = k1 - k0;
-  const unsigned acc_cols = mpad <= 32 ? 32 : mpad <= 64 ? 64 : 128;
+  const unsigned acc_cols = mpad <= 32 ? 32 : mpad <= 64 ? 64 : mpad <= 128 ? 128 : 256;
   if (trigger) pdl_trigger();
   if (threadIdx.x == 0) {
     for (int s = 0; s < STAGES; ++s) { mbar_init(&full_bar[s], 2); mbar_init(&empty_bar[s], 1); }
@@ -438,39 +446,39 @@ static int q8_rows_clusters(int parts) {
     cudaLaunchAttribute attr[2];
     const cudaLaunchConfig_t cfg = q8_rows_config<TO>((unsigned)parts, parts, 0, attr);
     int n = 0;
-    if (cudaOccupancyMaxActiveClusters(&n, gemm_q8_rows_kernel<TO>, &cfg) != cudaSuccess || n < 1) { cudaGetLastError(); n = 1; }
+    if (cudaFuncSetAttribute(gemm_q8_rows_kernel<TO>, cudaFuncAttributeMaxDynamicSharedMemorySize, Q8_ROWS_SMEM + 1024) != cudaSuccess ||
+        cudaOccupancyMaxActiveClusters(&n, gemm_q8_rows_kernel<TO>, &cfg) != cudaSuccess || n < 1) { cudaGetLastError(); n = 1; }
     known[dev][parts] = n;
   }
   return known[dev][parts];
 }
 
 // Height of a tile and blocks that share one: the pair for which the busiest SM is done first. In clocks: a step of 256 takes 850 however few its
-// rows are (instructions, a wait, a commit), 400 more for the second instruction row, or its bytes at 32 a clock if that is more; a block
-// 6,000 to begin and to end, and 2,500 more where a cluster meets.
+// rows are (instructions, a wait, a commit), 400 more for the second instruction row, or, if that is more, its bytes of w at 32 a clock and of a, which
+// come from the L2 cache, at 51; a block 6,000 to begin and to end, 2,500 more where a cluster meets, and 50 a row of a to store.
 template <typename TO>
-static void q8_rows_shape(int N, int K, int mpad, int* height, int* cut) {
+static long long q8_rows_shape(int N, int K, int mpad, int* height, int* cut) {
   const int nk = (K + 255) / 256;
   long long least = -1;
   for (int parts = 1; parts <= 8 && parts <= nk; parts *= 2) {
     const int slots = q8_rows_clusters<TO>(parts), steps = (nk + parts - 1) / parts;
     for (int h = 16; h <= 256; h += 8) {
-      if (q8_rows_stages(h, mpad) < 2) break;
+      if (q8_rows_stages(h, mpad) < 2 || (parts > 1 && mpad * h * 4 > Q8_ROWS_SMEM)) break;       // two stages, and the sums that a cluster adds up
       const long long tiles = (N + h - 1) / h, rounds = (tiles + slots - 1) / slots;
-      const long long busy = h > 128 ? 1250 : 850, bytes = (long long)(h + mpad) * 8;
+      const long long busy = h > 128 ? 1250 : 850, bytes = h * 8 + mpad * 5;
       const long long cost = rounds * (steps * (busy > bytes ? busy : bytes) + (parts > 1 ? 8500 : 6000));
       if (least < 0 || cost < least) { least = cost; *height = h; *cut = parts; }
     }
   }
+  return least + 50 * mpad;
 }
 
 template <typename TO>
-static int q8_rows(const Q8Call& c) {
+static int q8_rows(const Q8Call& c, int h, int parts) {
   auto k = gemm_q8_rows_kernel<TO>;
   cudaError_t e = cudaFuncSetAttribute(k, cudaFuncAttributeMaxDynamicSharedMemorySize, Q8_ROWS_SMEM + 1024);
   if (e != cudaSuccess) return (int)e;
   const int mpad = (c.M + 15) & ~15;
-  int h = 128, parts = 1;
-  q8_rows_shape<TO>(c.N, c.K, mpad, &h, &parts);
   CUtensorMap am, wm;
   int rc = encode_u8_2d(&am, c.a, c.M, c.K, c.lda, (unsigned)mpad);
   if (!rc) rc = encode_u8_2d(&wm, c.w, c.N, c.K, c.ldw, (unsigned)h);
@@ -510,8 +518,8 @@ __device__ __forceinline__ uint4 q8_ld_a(const u8* p, bool take) {
 
 template <int MT, int WARPS, int U, typename TO>
 __global__ void __launch_bounds__(WARPS * 32, 512 / (WARPS * 32))
-gemm_q8_skinny_kernel(const u8* __restrict__ a, long long lda, const float* __restrict__ sa, const u8* __restrict__ w, long long ldw,
-                      const float* __restrict__ sw, TO* __restrict__ out, long long ldo, int M, int N, int K, int tiles, int trigger) {
+gemm_q8_skinny_kernel(const u8* a, long long lda, const float* sa, const u8* w, long long ldw,
+                      const float* sw, TO* __restrict__ out, long long ldo, int M, int N, int K, int tiles, int trigger) {
   __shared__ float red[2][WARPS * MT * 32][4];
   if (trigger) pdl_trigger();
   const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31, g = lane >> 2, t = lane & 3;
@@ -605,11 +613,19 @@ static int q8_skinny(const Q8Call& c) {
   return si_last_error();
 }
 
+// Up to 256 rows the two tcgen05 kernels' costs are compared. us (one CTA and k cut, pairs): 112 x 2,048 x 2,048 8.5, 6.8; 112 x 4,096 x 4,096 9.3, 10.4;
+// 136 x 4,096 x 14,336 17.0, 23.5; 136 x 28,672 x 4,096 32.5, 31.6; 176 x 2,048 x 8,192 14.3, 14.9; 256 x 4,096 x 4,096 13.7, 10.5.
 template <typename TO>
 static int q8_any(const Q8Call& c) {
   if (c.K % 16 == 0 && (c.M <= 8 || (c.M <= 16 && (long long)c.N * c.K <= Q8_SKINNY_16_MOST))) return q8_skinny<TO>(c);
-  if (c.M <= Q8_ROWS_MAX) return q8_rows<TO>(c);
-  switch (q8_pair_columns(c.M, c.N)) {
+  long long pair_cost;
+  const int bn = q8_pair_columns(c.M, c.N, c.K, &pair_cost);
+  if (c.M <= Q8_ROWS_MAX) {
+    int h = 128, parts = 1;
+    const long long cost = q8_rows_shape<TO>(c.N, c.K, (c.M + 15) & ~15, &h, &parts);
+    if (cost <= pair_cost) return q8_rows<TO>(c, h, parts);
+  }
+  switch (bn) {
     case 64: return q8_pair<TO, 64>(c);
     case 128: return q8_pair<TO, 128>(c);
     default: return q8_pair<TO, 256>(c);

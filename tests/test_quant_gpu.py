@@ -180,6 +180,19 @@ def test_gemm_q8_whole_entries(M, N, K):
         assert torch.equal(out, want.to(F32).to(dtype))          # the sum is exact in fp32, the scales only move its exponent
 
 
+@pytest.mark.parametrize("M,N,K", [(129, 264, 8240), (176, 1000, 8240), (256, 136, 20000), (200, 64, 32768), (136, 4096, 8192), (112, 2048, 2048), (300, 4096, 8192),
+                                   (700, 6144, 2048), (8, 28672, 2048), (16, 4096, 4096), (61, 11264, 2048), (1100, 1024, 2816)])
+def test_gemm_q8_many_turns(M, N, K):
+    """Long rows and many tiles: every stage of shared memory is filled over and over, again and again."""
+    g = gen(M + N + K)
+    a, w, sa, sw = whole_codes(g, M, K), whole_codes(g, N, K), powers(g, M), powers(g, N)
+    want = (torch.mm(a.double(), w.double().t()) * sa.double().unsqueeze(1) * sw.double()).to(F32)
+    for _ in range(6):
+        out, status = torch.full((M, N), float("nan"), device=DEV), status_word()
+        ops().gemm_q8(a, sa, w, sw, out, status)
+        assert status.item() == 0 and torch.equal(out, want)
+
+
 @pytest.mark.parametrize("M,N,K", [(1, 4096, 4096), (8, 2048, 5632), (16, 6144, 4096), (61, 4096, 14336), (128, 1000, 2048), (300, 1336, 2816), (600, 2048, 1000)])
 def test_gemm_q8_real_entries(M, N, K):
     g = gen(K)
