@@ -80,7 +80,7 @@ struct NormArgs {
 };
 
 template <typename TX, typename TW, int CHUNKS>
-__global__ void __launch_bounds__(512) norm_q8_kernel(const NormArgs a, unsigned char* __restrict__ out, float* __restrict__ scale,
+__global__ void __launch_bounds__(512) norm_q8_kernel(const NormArgs a, unsigned char* out, float* scale,
                                                       int width, int num_rows, int trigger) {
   __shared__ float scratch[64];
   if (trigger) pdl_trigger();
@@ -157,7 +157,7 @@ __global__ void __launch_bounds__(512) norm_q8_kernel(const NormArgs a, unsigned
 }
 
 template <typename TX, typename TW>
-__global__ void norm_q8_scalar_kernel(const NormArgs a, unsigned char* __restrict__ out, float* __restrict__ scale, int width) {
+__global__ void norm_q8_scalar_kernel(const NormArgs a, unsigned char* out, float* scale, int width) {
   __shared__ float scratch[64];
   pdl_wait();
   const int r = blockIdx.x;
@@ -188,16 +188,21 @@ __global__ void norm_q8_scalar_kernel(const NormArgs a, unsigned char* __restric
   }
 }
 
-// silu(g) * u with the quick exponential and quotient: off by 2 + 1.2 |g| units where g is negative (and exp(-g) large), by four where it is positive; zero only
-// where exp(-g) is beyond 2^126, and so g exp(g) below any code. The accurate ones took 84 us for 2,048 x 14,336 (the accurate quotient alone 50 of
-// them): at forty instructions an entry arithmetic was what bounded the kernel.
-__device__ __forceinline__ float silu_mul_q8(float g, float u) { return __fdividef(g, 1.f + __expf(-g)) * u; }
+// silu(g) * u with the hardware's exponential of base 2 and reciprocal: off by 2 + 1.2 |g| units where g is negative (and exp(-g) large), by four where it
+// is positive; zero only where exp(-g) is beyond 2^126, and so g exp(g) below any code (subnormal intermediates are taken as zero, which changes no
+// other value). With the accurate functions arithmetic bounded the kernel: 84 us for 2,048 x 14,336, the accurate quotient alone 50 of them.
+__device__ __forceinline__ float silu_mul_q8(float g, float u) {
+  float e, q;
+  asm("ex2.approx.ftz.f32 %0, %1;" : "=f"(e) : "f"(g * -1.4426950408889634f));
+  asm("rcp.approx.ftz.f32 %0, %1;" : "=f"(q) : "f"(1.f + e));
+  return g * q * u;
+}
 
 // x as it is: the loaded entries stay packed in registers and are widened twice, before and after the reduction. A block goes through rows, and asks for
 // its next one before it reduces this one.
 template <typename TX, int CHUNKS>
 __global__ void __launch_bounds__(512, sizeof(TX) == 2 || CHUNKS < 4 ? 2 : 1)
-rows_q8_kernel(const TX* __restrict__ x, long long ldx, unsigned char* __restrict__ out, float* __restrict__ scale, int width, int num_rows, int trigger) {
+rows_q8_kernel(const TX* x, long long ldx, unsigned char* out, float* scale, int width, int num_rows, int trigger) {
   __shared__ float scratch[2][64];
   if (trigger) pdl_trigger();
   pdl_wait();
@@ -242,9 +247,11 @@ rows_q8_kernel(const TX* __restrict__ x, long long ldx, unsigned char* __restric
 }
 
 // The gated activation: gate f in column (f / group) * 2 * group + f % group, its up `group` columns further.
+// `shift`: group's logarithm, or -1 where it is no power of two: a division for every eight entries was a tenth to a quarter of the whole (2,048 x 14,336
+// 31.0 us with it and 28.2 without, 5.2 TB/s; 2,048 x 8,192 20.1 and 15.5).
 template <typename TX, int CHUNKS>
-__global__ void __launch_bounds__(512, 2) gated_q8_kernel(const TX* __restrict__ gu, unsigned char* __restrict__ out, float* __restrict__ scale, int width,
-                                                          int group, int trigger) {
+__global__ void __launch_bounds__(512, CHUNKS <= 2 && sizeof(TX) == 2 ? 3 : 2) gated_q8_kernel(const TX* gu, unsigned char* out, float* scale, int width, int group, int shift,
+                                                                   int trigger) {
   __shared__ float scratch[64];
   if (trigger) pdl_trigger();
   pdl_wait();
@@ -255,7 +262,7 @@ __global__ void __launch_bounds__(512, 2) gated_q8_kernel(const TX* __restrict__
   for (int c = 0; c < CHUNKS; ++c) {
     const int ch = threadIdx.x + c * blockDim.x;
     if (ch < nchunks) {
-      const int f = ch * 8, at = f / group * group + f;              // (f / group) * 2 * group + f % group
+      const int f = ch * 8, at = (shift >= 0 ? f >> shift << shift : f / group * group) + f;              // (f / group) * 2 * group + f % group
       gate[c].load(row + at);
       up[c].load(row + at + group);
     }
@@ -288,8 +295,8 @@ __global__ void __launch_bounds__(512, 2) gated_q8_kernel(const TX* __restrict__
 }
 
 template <typename TX, bool GATED>
-__global__ void rows_q8_scalar_kernel(const TX* __restrict__ x, long long ldx, unsigned char* __restrict__ out,
-                                      float* __restrict__ scale, int width, int group) {
+__global__ void rows_q8_scalar_kernel(const TX* x, long long ldx, unsigned char* out,
+                                      float* scale, int width, int group) {
   __shared__ float scratch[64];
   pdl_wait();
   const TX* row = x + (size_t)blockIdx.x * ldx;
@@ -355,8 +362,7 @@ SI_EXPORT int si_add_rmsnorm_q8(float* resid, const void* delta, const void* del
 
 template <typename TX, bool GATED>
 static void launch_rows(const void* x, long long ldx, void* out, float* scale, int num_rows, int width, int group, cudaStream_t stream) {
-  const dim3 block(row_threads(width));
-  dim3 grid(num_rows);
+  dim3 grid(num_rows), block(row_threads(width));
   const TX* xp = (const TX*)x;
   unsigned char* o = (unsigned char*)out;
   const bool vec = width % 8 == 0 && width <= Q8_MAX_VEC_WIDTH && (!GATED || group % 8 == 0) && ldx % (16 / (int)sizeof(TX)) == 0 &&
@@ -365,12 +371,14 @@ static void launch_rows(const void* x, long long ldx, void* out, float* scale, i
     si_launch(rows_q8_scalar_kernel<TX, GATED>, grid, block, 0, stream, xp, ldx, o, scale, width, group);
     return;
   }
-  const int per = (width / 8 + block.x - 1) / block.x, trigger = si_pdl_trigger_small(num_rows);
+  const int least = (width / 8 + block.x - 1) / block.x, per = least <= 2 ? least : 4, trigger = si_pdl_trigger_small(num_rows);
+  block.x = ((width / 8 + per - 1) / per + 31) / 32 * 32;           // no more than have work: 2,048 x 5,632 gated 12.8 us with 512 threads, 11.1 with 352
   const int most = si_sm_count() * (int)(1024 / block.x);          // blocks that run at once
   if (!GATED && num_rows > most) grid.x = most;
-#define ROWS_Q8(C) do { if constexpr (GATED) si_launch(gated_q8_kernel<TX, C>, grid, block, 0, stream, xp, o, scale, width, group, trigger); \
+  const int shift = (group & (group - 1)) == 0 ? __builtin_ctz(group) : -1;
+#define ROWS_Q8(C) do { if constexpr (GATED) si_launch(gated_q8_kernel<TX, C>, grid, block, 0, stream, xp, o, scale, width, group, shift, trigger); \
                         else si_launch(rows_q8_kernel<TX, C>, grid, block, 0, stream, xp, ldx, o, scale, width, num_rows, trigger); } while (0)
-  if (per <= 1) ROWS_Q8(1); else if (per <= 2) ROWS_Q8(2); else ROWS_Q8(4);
+  if (per == 1) ROWS_Q8(1); else if (per == 2) ROWS_Q8(2); else ROWS_Q8(4);
 #undef ROWS_Q8
 }
 
