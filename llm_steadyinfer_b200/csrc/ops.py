@@ -2348,6 +2348,8 @@ def _matrix(t, what: str):
     if len(shape) != 2 or (strides[1] != 1 and shape[1] > 1):
         raise KernelError(f"{what} must be a matrix whose rows are contiguous")
     rows, cols = shape
+    if rows > _MOST or cols > _MOST:
+        raise KernelError(f"{what}: {rows} rows of {cols} are more than 32 bits count")
     return rows, cols, strides[0] if rows > 1 else cols
 
 
@@ -2357,6 +2359,7 @@ def _f32_of(t, n: int, what: str) -> None:
 
 
 _F32, _BF16 = torch.float32, torch.bfloat16
+_MOST = 0x7ff00000                             # of rows and of columns: room for a kernel's own steps beyond the last
 
 
 def _q8_out(out, scale, R: int, width: int, what: str) -> None:
@@ -2364,6 +2367,8 @@ def _q8_out(out, scale, R: int, width: int, what: str) -> None:
         raise KernelError(f"{what}: out must be contiguous float8_e4m3fn [{R}, {width}]")
     if scale.dtype is not _F32 or scale.numel() != R or not scale.is_contiguous():
         raise KernelError(f"{what}: scale must be contiguous fp32 of {R} elements")
+    if R > _MOST or width > _MOST:
+        raise KernelError(f"{what}: {R} rows of {width} are more than 32 bits count")
 
 
 def add_rmsnorm_q8(resid, delta, weight, eps: float, out, scale, rows=None, ahead=None, delta2=None, dst=None) -> None:
@@ -2478,7 +2483,7 @@ def gemm_q8(a, a_scale, w, w_scale, out, status=None) -> None:
 def gemm_w4(x, w, scales, zeros, group: int, out, status=None) -> None:
     """out[m, n] = sum_k x[m, k] * scales[n, k / group] * (q[n, k] - zeros[n, k / group]) with weights of four bits: x bf16 [M, K] (rows
     contiguous, K a multiple of 8), ``w`` int32 [N, K / 8], entry i of the eight in a word at bit ``W4_SHIFTS[i]`` (see ``pack_w4``); scales bf16
-    [N, ceil(K / group)], zeros uint8 like them or None (8 everywhere), ``group`` 32, 64 or a multiple of 128; out bf16 or fp32 [M, N]; sums fp32.
+    [N, ceil(K / group)], zeros uint8 like them (0 .. 15) or None (8 everywhere), ``group`` 32, 64 or a multiple of 128; out bf16 or fp32 [M, N]; sums fp32.
     A weight times its scale is rounded to bf16 before it is multiplied, except up to eight rows with groups of 128 and more. ``status``: as in
     ``gemm_q8``."""
     stream = _here("gemm_w4", x, w, scales, zeros, out, status)
@@ -2492,6 +2497,8 @@ def gemm_w4(x, w, scales, zeros, group: int, out, status=None) -> None:
         raise KernelError("gemm_w4: out's rows overlap")
     if group not in (32, 64) and (group <= 0 or group % 128):
         raise KernelError(f"gemm_w4: group {group} is not 32, 64 or a multiple of 128")
+    if group > K > 0 and group > 128:
+        group = -(-K // 128) * 128                               # one group a row, however far it would reach
     G = -(-K // group)
     if scales.dtype is not _BF16 or scales.shape != (N, G) or not scales.is_contiguous():
         raise KernelError(f"gemm_w4: scales must be contiguous bfloat16 [{N}, {G}]")

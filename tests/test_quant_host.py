@@ -132,6 +132,29 @@ def test_products_pass_and_empty_ones_launch_nothing(checks_alone):
     assert len(checks_alone) == n
 
 
+def test_sizes_beyond_32_bits_are_refused(checks_alone):
+    meta = lambda *shape, dtype=torch.float32: torch.empty(*shape, dtype=dtype, device="meta")
+    many = 2 ** 31
+    for call in (lambda: ops.quantize_q8(meta(many, 8), meta(many, 8, dtype=E4M3), meta(many)),
+                 lambda: ops.swiglu_q8(meta(many, 16), meta(many, 8, dtype=E4M3), meta(many)),
+                 lambda: ops.add_rmsnorm_q8(meta(many, 8), None, meta(8), 1e-5, meta(many, 8, dtype=E4M3), meta(many)),
+                 lambda: ops.gemm_q8(meta(many, 16, dtype=E4M3), meta(many), meta(8, 16, dtype=E4M3), meta(8), meta(many, 8)),
+                 lambda: ops.gemm_w4(meta(1, 32, dtype=BF16), meta(many, 4, dtype=torch.int32), meta(many, 1, dtype=BF16), None, 128, meta(1, many))):
+        with pytest.raises(ops.KernelError, match="32 bits"):
+            call()
+    assert checks_alone == []
+
+
+@pytest.mark.parametrize("group", [384, 2 ** 32 + 128, 2 ** 40])
+def test_a_group_beyond_the_row_is_one_group(monkeypatch, group):
+    seen = []
+    monkeypatch.setattr(ops, "_here", lambda *a: 0)
+    monkeypatch.setattr(ops, "gemm_tc05_available", lambda: True)
+    monkeypatch.setattr(ops, "_fn", lambda lib, symbol, argtypes: lambda *args: seen.append(args[6]) or 0)
+    ops.gemm_w4(z(2, 160, dtype=BF16), z(3, 20, dtype=torch.int32), z(3, 1, dtype=BF16), None, group, z(2, 3))
+    assert seen == [256]
+
+
 def test_a_tensor_of_another_device_is_refused(monkeypatch):
     class Elsewhere:
         is_cuda = True
