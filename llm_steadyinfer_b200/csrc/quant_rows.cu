@@ -189,8 +189,8 @@ __global__ void norm_q8_scalar_kernel(const NormArgs a, unsigned char* out, floa
 }
 
 // silu(g) * u with the hardware's exponential of base 2 and reciprocal: off by 2 + 1.2 |g| units where g is negative (and exp(-g) large), by four where it
-// is positive; zero only where exp(-g) is beyond 2^126, and so g exp(g) below any code (subnormal intermediates are taken as zero, which changes no
-// other value). With the accurate functions arithmetic bounded the kernel: 84 us for 2,048 x 14,336, the accurate quotient alone 50 of them.
+// is positive; zero where exp(-g) is beyond 2^126 (g below -87), a value below any code beside entries of ordinary size (subnormal intermediates are taken
+// as zero, which changes no other value). With the accurate functions arithmetic bounded the kernel: 84 us for 2,048 x 14,336, the accurate quotient alone 50 of them.
 __device__ __forceinline__ float silu_mul_q8(float g, float u) {
   float e, q;
   asm("ex2.approx.ftz.f32 %0, %1;" : "=f"(e) : "f"(g * -1.4426950408889634f));

@@ -361,6 +361,21 @@ def test_gemm_w4_words_that_name_their_place(M, N, K, group, zeros):
         assert status.item() == 0 and torch.equal(out, want)
 
 
+@pytest.mark.parametrize("M", [1, 8, 9])
+@pytest.mark.parametrize("K", [4352, 8192, 16640, 32768, 33024])
+@pytest.mark.parametrize("group", [64, 128])
+def test_gemm_w4_rows_longer_than_a_block_holds(M, K, group):
+    """Few rows of up to 32,768 entries are cut over a cluster, of more go to the kernel for many: entries -1 .. 1, so that every sum is exact."""
+    g = gen(M + K + group)
+    N = 83
+    words, s, z, w = w4_weight(g, N, K, group, True)
+    x = torch.randint(-1, 2, (M, K), generator=g, device=DEV).to(BF16)
+    want = torch.mm(x.double(), w.t()).to(F32)
+    out, status = torch.full((M, N), float("nan"), device=DEV), status_word()
+    ops().gemm_w4(x, words, s, z, group, out, status)
+    assert status.item() == 0 and torch.equal(out, want)
+
+
 @pytest.mark.parametrize("M", [2, 40, 200])
 def test_gemm_w4_nan_stays_in_its_row_and_column(M):
     g = gen(M)
