@@ -639,11 +639,17 @@ SI_EXPORT int si_gemm_q8_ok(const void* a, long long lda, const void* w, long lo
 
 // a [M, K] and w [N, K] e4m3, rows `lda` and `ldw` bytes apart (multiples of 16, bases too); sa [M], sw [N] fp32; out [M, N], rows `ldo` entries
 // apart, SI_BF16 or SI_F32. Returns 0, a CUDA error code, or -2 (size or layout refused).
-SI_EXPORT int si_gemm_q8(const void* a, long long lda, const float* sa, const void* w, long long ldw, const float* sw, void* out,
+static int gemm_q8(const void* a, long long lda, const float* sa, const void* w, long long ldw, const float* sw, void* out,
                          long long ldo, int out_dtype, int M, int N, int K, int* status, cudaStream_t stream) {
   if (M <= 0 || N <= 0) return 0;
   if (K <= 0 || K > 0x3fffffff || !si_gemm_q8_ok(a, lda, w, ldw, K)) return -2;
   Q8Call c;
   c.a = a; c.lda = lda; c.sa = sa; c.w = w; c.ldw = ldw; c.sw = sw; c.out = out; c.ldo = ldo; c.M = M; c.N = N; c.K = K; c.status = status; c.stream = stream;
   return out_dtype == SI_BF16 ? q8_any<bf16>(c) : q8_any<float>(c);
+}
+
+// The same with its arguments in one array, in their order (see quant_rows.cu).
+SI_EXPORT int si_gemm_q8(const long long* a) {
+  return gemm_q8((const void*)a[0], a[1], (const float*)a[2], (const void*)a[3], a[4], (const float*)a[5], (void*)a[6], a[7], (int)a[8], (int)a[9],
+                 (int)a[10], (int)a[11], (int*)a[12], (cudaStream_t)a[13]);
 }

@@ -852,7 +852,7 @@ SI_EXPORT int si_gemm_w4_ok(const void* x, long long ldx, const void* w, long lo
 
 // x [M, K] bf16, rows `ldx` apart; w [N, K / 8] int32 words, rows `ldw` words apart; scales bf16 [N, ceil(K / group)], zeros uint8 like them or null;
 // group 32, 64 or a multiple of 128; out [M, N], rows `ldo` apart, SI_BF16 or SI_F32. Returns 0, a CUDA error code, or -2 (size or layout refused).
-SI_EXPORT int si_gemm_w4(const void* x, long long ldx, const void* w, long long ldw, const void* scales, const void* zeros, int group, void* out,
+static int gemm_w4(const void* x, long long ldx, const void* w, long long ldw, const void* scales, const void* zeros, int group, void* out,
                          long long ldo, int out_dtype, int M, int N, int K, int* status, cudaStream_t stream) {
   if (M <= 0 || N <= 0) return 0;
   if (K <= 0 || K % 8 || K > 0x3fffffff || !(group == 32 || group == 64 || (group > 0 && group % 128 == 0)) || !si_gemm_w4_ok(x, ldx, w, ldw, K)) return -2;
@@ -863,4 +863,10 @@ SI_EXPORT int si_gemm_w4(const void* x, long long ldx, const void* w, long long 
   const bool wide = group >= 128 || ((uintptr_t)scales % 16 == 0 && (uintptr_t)zeros % 8 == 0);      // small groups' scales come eight at a time
   if (wide && w4_few_shape(M, N, K, zeros != nullptr, group < 128, &f)) return out_dtype == SI_BF16 ? w4_few<bf16>(c, f) : w4_few<float>(c, f);
   return out_dtype == SI_BF16 ? w4_tc<bf16>(c) : w4_tc<float>(c);
+}
+
+// The same with its arguments in one array, in their order (see quant_rows.cu).
+SI_EXPORT int si_gemm_w4(const long long* a) {
+  return gemm_w4((const void*)a[0], a[1], (const void*)a[2], a[3], (const void*)a[4], (const void*)a[5], (int)a[6], (void*)a[7], a[8], (int)a[9], (int)a[10],
+                 (int)a[11], (int)a[12], (int*)a[13], (cudaStream_t)a[14]);
 }

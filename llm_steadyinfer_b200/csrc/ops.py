@@ -7,6 +7,7 @@ from __future__ import annotations
 import ctypes
 import functools
 import os
+import struct
 from typing import Optional
 
 import torch
@@ -2317,11 +2318,19 @@ W4_SHIFTS = (0, 16, 4, 20, 8, 24, 12, 28)      # the bit of entry i of the eight
 
 # These calls check their arguments without building a message before one is needed: a decode step makes many of them, and each lasts a few
 # microseconds on the GPU.
-_ROWS_Q8_ARGS = [_c_p, _c_int, _c_ll, _c_p, _c_p, _c_int, _c_int, _c_p]
-_SWIGLU_Q8_ARGS = [_c_p, _c_int, _c_p, _c_p, _c_int, _c_int, _c_int, _c_p]
-_NORM_Q8_ARGS = [_c_p, _c_p, _c_p, _c_int, _c_p, _c_p, _c_int, _c_p, _c_p, _c_p, _c_int, _c_int, _c_f, _c_p, _c_ll, _c_p]
-_GEMM_Q8_ARGS = [_c_p, _c_ll, _c_p, _c_p, _c_ll, _c_p, _c_p, _c_ll, _c_int, _c_int, _c_int, _c_int, _c_p, _c_p]
-_GEMM_W4_ARGS = [_c_p, _c_ll, _c_p, _c_ll, _c_p, _c_p, _c_int, _c_p, _c_ll, _c_int, _c_int, _c_int, _c_int, _c_p, _c_p]
+# For the same reason the aligned forms take their arguments in one array of eight bytes each.
+_ARRAY = [ctypes.c_char_p]
+_ROWS_Q8_ARGS = struct.Struct("=8q")
+_NORM_Q8_ARGS = struct.Struct("=12qd3q")
+_GEMM_Q8_ARGS = struct.Struct("=14q")
+_GEMM_W4_ARGS = struct.Struct("=15q")
+_GEMM_QUANT_Q8_ARGS = [_c_p, _c_ll, _c_p, _c_p, _c_ll, _c_p, _c_p, _c_ll, _c_int, _c_int, _c_int, _c_int, _c_p]
+_GEMM_QUANT_W4_ARGS = [_c_p, _c_ll, _c_p, _c_ll, _c_p, _c_p, _c_int, _c_p, _c_ll, _c_int, _c_int, _c_int, _c_int, _c_p]
+_current_device = getattr(torch._C, "_cuda_getDevice", None) or torch.cuda.current_device      # without the question whether CUDA is up: a tensor of its is here
+
+
+def _at(t) -> int:
+    return 0 if t is None else t.data_ptr()
 
 
 def _here(what: str, *ts) -> int:
@@ -2332,7 +2341,7 @@ def _here(what: str, *ts) -> int:
             index = -1
             break
     if index >= 0:
-        at = _device_index if _device_index is not None else torch.cuda.current_device()
+        at = _device_index if _device_index is not None else _current_device()
         if index == at:
             return _raw_stream(at) if _raw_stream is not None else torch.cuda.current_stream().cuda_stream
         raise KernelError(f"{what}: the tensors are on device {index}, the kernel is launched on device {at}")
@@ -2407,9 +2416,9 @@ def add_rmsnorm_q8(resid, delta, weight, eps: float, out, scale, rows=None, ahea
     if R == 0:
         return
     ahead_bytes = min(ahead.numel() * ahead.element_size(), AHEAD_BYTES) if ahead is not None and ahead.is_contiguous() else 0
-    rc = _fn("quant_rows", "si_add_rmsnorm_q8", _NORM_Q8_ARGS)(
-        resid.data_ptr(), _ptr(delta), _ptr(delta2), xd, _ptr(rows), weight.data_ptr(), wd, _ptr(dst), out.data_ptr(), scale.data_ptr(), R, d, eps,
-        ahead.data_ptr() if ahead_bytes else None, ahead_bytes, stream)
+    rc = _fn("quant_rows", "si_add_rmsnorm_q8", _ARRAY)(_NORM_Q8_ARGS.pack(
+        resid.data_ptr(), _at(delta), _at(delta2), xd, _at(rows), weight.data_ptr(), wd, _at(dst), out.data_ptr(), scale.data_ptr(), R, d, eps,
+        ahead.data_ptr() if ahead_bytes else 0, ahead_bytes, stream))
     _check(rc, "add_rmsnorm_q8" if rc == 0 else f"add_rmsnorm_q8(hidden={d})")
 
 
@@ -2431,7 +2440,7 @@ def swiglu_q8(gu, out, scale, group=None) -> None:
         return
     if F <= 0 or group <= 0 or F % group:
         raise KernelError("swiglu_q8: the group must divide F")
-    rc = _fn("quant_rows", "si_swiglu_q8", _SWIGLU_Q8_ARGS)(gu.data_ptr(), dt, out.data_ptr(), scale.data_ptr(), T, F, group, stream)
+    rc = _fn("quant_rows", "si_swiglu_q8", _ARRAY)(_ROWS_Q8_ARGS.pack(gu.data_ptr(), dt, out.data_ptr(), scale.data_ptr(), T, F, group, stream))
     _check(rc, "swiglu_q8" if rc == 0 else f"swiglu_q8(F={F})")
 
 
@@ -2447,7 +2456,7 @@ def quantize_q8(x, out, scale) -> None:
         return
     if n <= 0:
         raise KernelError("quantize_q8: rows without entries")
-    rc = _fn("quant_rows", "si_quantize_q8", _ROWS_Q8_ARGS)(x.data_ptr(), dt, ldx, out.data_ptr(), scale.data_ptr(), R, n, stream)
+    rc = _fn("quant_rows", "si_quantize_q8", _ARRAY)(_ROWS_Q8_ARGS.pack(x.data_ptr(), dt, ldx, out.data_ptr(), scale.data_ptr(), R, n, stream))
     _check(rc, "quantize_q8" if rc == 0 else f"quantize_q8(n={n})")
 
 
@@ -2472,10 +2481,10 @@ def gemm_q8(a, a_scale, w, w_scale, out, status=None) -> None:
         raise KernelError("gemm_q8: rows without entries")
     pa, pw = a.data_ptr(), w.data_ptr()
     if (pa | pw | lda | ldw) % 16 == 0 and lda >= K and ldw >= K and gemm_tc05_available():
-        rc = _fn("gemm_q8", "si_gemm_q8", _GEMM_Q8_ARGS)(pa, lda, a_scale.data_ptr(), pw, ldw, w_scale.data_ptr(), out.data_ptr(), ldo, od, M, N, K,
-                                                         _ptr(status), stream)
+        rc = _fn("gemm_q8", "si_gemm_q8", _ARRAY)(_GEMM_Q8_ARGS.pack(pa, lda, a_scale.data_ptr(), pw, ldw, w_scale.data_ptr(), out.data_ptr(), ldo, od,
+                                                                     M, N, K, _at(status), stream))
     else:                                                        # rows that do not start on 16-byte boundaries
-        rc = _fn("gemm_quant", "si_gemm_quant_q8", _GEMM_Q8_ARGS[:-1])(pa, lda, a_scale.data_ptr(), pw, ldw, w_scale.data_ptr(), out.data_ptr(), ldo, od,
+        rc = _fn("gemm_quant", "si_gemm_quant_q8", _GEMM_QUANT_Q8_ARGS)(pa, lda, a_scale.data_ptr(), pw, ldw, w_scale.data_ptr(), out.data_ptr(), ldo, od,
                                                                        M, N, K, stream)
     _check(rc, "gemm_q8" if rc == 0 else f"gemm_q8(M={M}, N={N}, K={K})")
 
@@ -2513,10 +2522,10 @@ def gemm_w4(x, w, scales, zeros, group: int, out, status=None) -> None:
         raise KernelError("gemm_w4: rows without entries")
     px, pw = x.data_ptr(), w.data_ptr()
     if (px | pw) % 16 == 0 and ldx % 8 == 0 and ldw % 4 == 0 and K % 32 == 0 and ldx >= K and ldw * 8 >= K and gemm_tc05_available():
-        rc = _fn("gemm_w4", "si_gemm_w4", _GEMM_W4_ARGS)(px, ldx, pw, ldw, scales.data_ptr(), _ptr(zeros), group, out.data_ptr(), ldo, od, M, N, K,
-                                                         _ptr(status), stream)
+        rc = _fn("gemm_w4", "si_gemm_w4", _ARRAY)(_GEMM_W4_ARGS.pack(px, ldx, pw, ldw, scales.data_ptr(), _at(zeros), group, out.data_ptr(), ldo, od,
+                                                                     M, N, K, _at(status), stream))
     else:                                                        # rows that are not in 16-byte pieces
-        rc = _fn("gemm_quant", "si_gemm_quant_w4", _GEMM_W4_ARGS[:-1])(px, ldx, pw, ldw, scales.data_ptr(), _ptr(zeros), group, out.data_ptr(), ldo, od,
+        rc = _fn("gemm_quant", "si_gemm_quant_w4", _GEMM_QUANT_W4_ARGS)(px, ldx, pw, ldw, scales.data_ptr(), _ptr(zeros), group, out.data_ptr(), ldo, od,
                                                                        M, N, K, stream)
     _check(rc, "gemm_w4" if rc == 0 else f"gemm_w4(M={M}, N={N}, K={K}, group={group})")
 

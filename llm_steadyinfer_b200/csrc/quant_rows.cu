@@ -11,6 +11,7 @@
 // pieces, or wider than 16,384, take a scalar kernel that reads the row twice (the second time from cache).
 // NaN: a NaN entry becomes a NaN code and leaves the maximum to the others (fmaxf); with an infinite entry the factor is zero and the
 // entry itself becomes NaN. The norm of a row with either is NaN where the formula says so.
+#include <string.h>
 #include "quant_common.cuh"
 
 typedef __nv_bfloat16 bf16;
@@ -339,7 +340,7 @@ static void launch_norm(const NormArgs& a, unsigned char* out, float* scale, int
 
 // resid [*, width] fp32; delta, delta2 (may be null) like it in x_dtype; weight [width] in w_dtype; dst (may be null, may be resid);
 // out [num_rows, width] e4m3, scale [num_rows] fp32. Returns 0, a CUDA error code, or -2 (size refused).
-SI_EXPORT int si_add_rmsnorm_q8(float* resid, const void* delta, const void* delta2, int x_dtype, const int* rows, const void* weight,
+static int add_rmsnorm_q8(float* resid, const void* delta, const void* delta2, int x_dtype, const int* rows, const void* weight,
                                 int w_dtype, float* dst, void* out, float* scale, int num_rows, int width, float eps, const void* ahead,
                                 long long ahead_bytes, cudaStream_t stream) {
   if (num_rows <= 0) return 0;
@@ -383,7 +384,7 @@ static void launch_rows(const void* x, long long ldx, void* out, float* scale, i
 }
 
 // x [num_rows, width], rows `ldx` entries apart -> out [num_rows, width] e4m3, scale [num_rows].
-SI_EXPORT int si_quantize_q8(const void* x, int dtype, long long ldx, void* out, float* scale, int num_rows, int width, cudaStream_t stream) {
+static int quantize_q8(const void* x, int dtype, long long ldx, void* out, float* scale, int num_rows, int width, cudaStream_t stream) {
   if (num_rows <= 0) return 0;
   if (width <= 0) return -2;
   if (dtype == SI_BF16) launch_rows<bf16, false>(x, ldx, out, scale, num_rows, width, 1, stream);
@@ -392,10 +393,25 @@ SI_EXPORT int si_quantize_q8(const void* x, int dtype, long long ldx, void* out,
 }
 
 // gu [num_rows, 2 * inter], rows one behind the other, gates and ups interleaved in groups of `group` columns -> out [num_rows, inter].
-SI_EXPORT int si_swiglu_q8(const void* gu, int dtype, void* out, float* scale, int num_rows, int inter, int group, cudaStream_t stream) {
+static int swiglu_q8(const void* gu, int dtype, void* out, float* scale, int num_rows, int inter, int group, cudaStream_t stream) {
   if (num_rows <= 0) return 0;
   if (inter <= 0 || group <= 0 || inter % group || inter > 0x3fffffff) return -2;
   if (dtype == SI_BF16) launch_rows<bf16, true>(gu, 2LL * inter, out, scale, num_rows, inter, group, stream);
   else launch_rows<float, true>(gu, 2LL * inter, out, scale, num_rows, inter, group, stream);
   return si_last_error();
+}
+
+// The functions above with their arguments in one array, in their order (eps as a double): handing over up to sixteen one by one cost the calling side
+// 2.3 us, an array 0.6.
+SI_EXPORT int si_add_rmsnorm_q8(const long long* a) {
+  double eps;
+  memcpy(&eps, a + 12, 8);
+  return add_rmsnorm_q8((float*)a[0], (const void*)a[1], (const void*)a[2], (int)a[3], (const int*)a[4], (const void*)a[5], (int)a[6], (float*)a[7],
+                        (void*)a[8], (float*)a[9], (int)a[10], (int)a[11], (float)eps, (const void*)a[13], a[14], (cudaStream_t)a[15]);
+}
+SI_EXPORT int si_quantize_q8(const long long* a) {
+  return quantize_q8((const void*)a[0], (int)a[1], a[2], (void*)a[3], (float*)a[4], (int)a[5], (int)a[6], (cudaStream_t)a[7]);
+}
+SI_EXPORT int si_swiglu_q8(const long long* a) {
+  return swiglu_q8((const void*)a[0], (int)a[1], (void*)a[2], (float*)a[3], (int)a[4], (int)a[5], (int)a[6], (cudaStream_t)a[7]);
 }

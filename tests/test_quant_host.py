@@ -150,7 +150,7 @@ def test_a_group_beyond_the_row_is_one_group(monkeypatch, group):
     seen = []
     monkeypatch.setattr(ops, "_here", lambda *a: 0)
     monkeypatch.setattr(ops, "gemm_tc05_available", lambda: True)
-    monkeypatch.setattr(ops, "_fn", lambda lib, symbol, argtypes: lambda *args: seen.append(args[6]) or 0)
+    monkeypatch.setattr(ops, "_fn", lambda lib, symbol, argtypes: lambda packed: seen.append(ops._GEMM_W4_ARGS.unpack(packed)[6]) or 0)
     ops.gemm_w4(z(2, 160, dtype=BF16), z(3, 20, dtype=torch.int32), z(3, 1, dtype=BF16), None, group, z(2, 3))
     assert seen == [256]
 
