@@ -8,7 +8,8 @@
 // All three are one pass over memory: a block takes a row, every thread keeps its part of it (eight entries a load, up to 32) in
 // registers over the one reduction that the row needs. The norm needs no second one: max |y| = rsqrt(...) * max |weight * h|, so the sum of
 // squares and the maximum are reduced together. Arithmetic is fp32; the only rounding is the one to e4m3. Rows that are not in 16-byte
-// pieces, or wider than 16,384, take a scalar kernel that reads the row twice (the second time from cache).
+// pieces go entry by entry (us, 4,093 columns and 4,096: norm of 2,048 rows 25, 17; 4,096 rows as they are 17, 12); rows wider than 16,384 take a scalar
+// kernel that reads them twice (the second time from cache).
 // NaN: a NaN entry becomes a NaN code and leaves the maximum to the others (fmaxf); with an infinite entry the factor is zero and the
 // entry itself becomes NaN. The norm of a row with either is NaN where the formula says so.
 #include <string.h>
@@ -157,6 +158,47 @@ __global__ void __launch_bounds__(512) norm_q8_kernel(const NormArgs a, unsigned
   }
 }
 
+// Rows that are not in 16-byte pieces: entry by entry, but in one pass as well, a thread's K in registers. (Read twice by a loop, with one entry
+// under way a thread, 2,048 x 4,093 took 36 us, 4,096 x 4,093 as they are 39, 2,048 x 14,330 gated 113 for 63.)
+template <typename TX, typename TW, int K>
+__global__ void __launch_bounds__(1024) norm_q8_odd_kernel(const NormArgs a, unsigned char* out, float* scale, int width) {
+  __shared__ float scratch[64];
+  pdl_wait();
+  const int r = blockIdx.x;
+  const size_t src = (size_t)(a.rows ? a.rows[r] : r) * width;
+  const TX* d1 = (const TX*)a.delta;
+  const TX* d2 = (const TX*)a.delta2;
+  const TW* weight = (const TW*)a.weight;
+  float x[K];
+#pragma unroll
+  for (int k = 0; k < K; ++k) {
+    const size_t i = src + min((int)(threadIdx.x + k * blockDim.x), width - 1);      // beyond the end the last entry again: no branch between the loads
+    x[k] = a.resid[i];
+    if (d1) x[k] += to_f32<TX>(d1[i]);
+    if (d2) x[k] += to_f32<TX>(d2[i]);
+  }
+  float ss = 0.f, top = 0.f;
+#pragma unroll
+  for (int k = 0; k < K; ++k) {
+    const int i = threadIdx.x + k * blockDim.x;
+    if (i < width) {
+      if (a.dst) a.dst[src + i] = x[k];
+      ss += x[k] * x[k];
+      x[k] *= to_f32<TW>(weight[i]);
+      top = fmaxf(top, fabsf(x[k]));
+    }
+  }
+  const float2 both = block_sum_max(ss, top, scratch);
+  const float inv = rsqrtf(both.x / (float)width + a.eps);
+  const float amax = both.y * inv, f = q8_factor(amax);
+  if (threadIdx.x == 0) scale[r] = q8_scale(amax);
+#pragma unroll
+  for (int k = 0; k < K; ++k) {
+    const int i = threadIdx.x + k * blockDim.x;
+    if (i < width) out[(size_t)r * width + i] = q8_pack1(x[k] * inv * f);
+  }
+}
+
 template <typename TX, typename TW>
 __global__ void norm_q8_scalar_kernel(const NormArgs a, unsigned char* out, float* scale, int width) {
   __shared__ float scratch[64];
@@ -248,7 +290,7 @@ rows_q8_kernel(const TX* x, long long ldx, unsigned char* out, float* scale, int
 }
 
 // The gated activation: gate f in column (f / group) * 2 * group + f % group, its up `group` columns further.
-// `shift`: group's logarithm, or -1 where it is no power of two: a division for every eight entries was a tenth to a quarter of the whole (2,048 x 14,336
+// `shift`: group's logarithm, 31 where a row is one group, or -1 where it is no power of two: a division for every eight entries was a tenth to a quarter of the whole (2,048 x 14,336
 // 31.0 us with it and 28.2 without, 5.2 TB/s; 2,048 x 8,192 20.1 and 15.5).
 template <typename TX, int CHUNKS>
 __global__ void __launch_bounds__(512, CHUNKS <= 2 && sizeof(TX) == 2 ? 3 : 2) gated_q8_kernel(const TX* gu, unsigned char* out, float* scale, int width, int group, int shift,
@@ -295,6 +337,39 @@ __global__ void __launch_bounds__(512, CHUNKS <= 2 && sizeof(TX) == 2 ? 3 : 2) g
   }
 }
 
+template <typename TX, bool GATED, int K>
+__global__ void __launch_bounds__(1024) rows_q8_odd_kernel(const TX* x, long long ldx, unsigned char* out, float* scale, int width, int group, int shift) {
+  __shared__ float scratch[64];
+  pdl_wait();
+  const TX* row = x + (size_t)blockIdx.x * ldx;
+  float v[K], top = 0.f;
+#pragma unroll
+  for (int b = 0; b < K; b += 8) {                        // eight at a time: sixteen gates and ups with their addresses are more than a thread's registers
+    float up[GATED ? 8 : 1];
+#pragma unroll
+    for (int k = 0; k < 8; ++k) {                         // beyond the end the last entry again: no branch between the loads, no other maximum
+      const int i = min((int)(threadIdx.x + (b + k) * blockDim.x), width - 1);
+      const int at = !GATED ? i : (shift >= 0 ? i >> shift << shift : i / group * group) + i;
+      v[b + k] = to_f32<TX>(row[at]);
+      if (GATED) up[k] = to_f32<TX>(row[at + group]);
+    }
+#pragma unroll
+    for (int k = 0; k < 8; ++k) {
+      if (GATED) v[b + k] = silu_mul_q8(v[b + k], up[k]);
+      top = fmaxf(top, fabsf(v[b + k]));
+    }
+    if (GATED) asm volatile("" ::: "memory");
+  }
+  top = block_sum_max(0.f, top, scratch).y;
+  const float f = q8_factor(top);
+  if (threadIdx.x == 0) scale[blockIdx.x] = q8_scale(top);
+#pragma unroll
+  for (int k = 0; k < K; ++k) {
+    const int i = threadIdx.x + k * blockDim.x;
+    if (i < width) out[(size_t)blockIdx.x * width + i] = q8_pack1(v[k] * f);
+  }
+}
+
 template <typename TX, bool GATED>
 __global__ void rows_q8_scalar_kernel(const TX* x, long long ldx, unsigned char* out,
                                       float* scale, int width, int group) {
@@ -322,11 +397,17 @@ static int row_threads(int width, int most = 512) {
   return chunks >= most ? most : (chunks + 31) / 32 * 32;
 }
 
+static dim3 odd_threads(int width, int each) { return dim3(((width + each - 1) / each + 31) / 32 * 32); }
+
 template <typename TX, typename TW>
 static void launch_norm(const NormArgs& a, unsigned char* out, float* scale, int width, int num_rows, bool vec, cudaStream_t stream) {
   const dim3 block(row_threads(width, vec && num_rows >= 1024 && width <= Q8_MAX_VEC_WIDTH / 2 ? 256 : 512));
   if (!vec) {
-    si_launch(norm_q8_scalar_kernel<TX, TW>, dim3(num_rows), block, 0, stream, a, out, scale, width);
+#define NORM_ODD(K) si_launch(norm_q8_odd_kernel<TX, TW, K>, dim3(num_rows), odd_threads(width, K), 0, stream, a, out, scale, width)
+    if (width <= 8 * 1024) NORM_ODD(8);
+    else if (width <= 16 * 1024) NORM_ODD(16);
+    else si_launch(norm_q8_scalar_kernel<TX, TW>, dim3(num_rows), block, 0, stream, a, out, scale, width);
+#undef NORM_ODD
     return;
   }
   const int per = (width / 8 + block.x - 1) / block.x, sms = si_sm_count();
@@ -368,15 +449,19 @@ static void launch_rows(const void* x, long long ldx, void* out, float* scale, i
   unsigned char* o = (unsigned char*)out;
   const bool vec = width % 8 == 0 && width <= Q8_MAX_VEC_WIDTH && (!GATED || group % 8 == 0) && ldx % (16 / (int)sizeof(TX)) == 0 &&
                    (uintptr_t)x % 16 == 0 && (uintptr_t)out % 8 == 0;
+  const int shift = group >= width ? 31 : (group & (group - 1)) == 0 ? __builtin_ctz(group) : -1;      // one group: 31, nothing is left of a column
   if (!vec) {
-    si_launch(rows_q8_scalar_kernel<TX, GATED>, grid, block, 0, stream, xp, ldx, o, scale, width, group);
+#define ROWS_ODD(K) si_launch(rows_q8_odd_kernel<TX, GATED, K>, grid, odd_threads(width, K), 0, stream, xp, ldx, o, scale, width, group, shift)
+    if (width <= 8 * 1024) ROWS_ODD(8);
+    else if (width <= 16 * 1024) ROWS_ODD(16);
+    else si_launch(rows_q8_scalar_kernel<TX, GATED>, grid, block, 0, stream, xp, ldx, o, scale, width, group);
+#undef ROWS_ODD
     return;
   }
   const int least = (width / 8 + block.x - 1) / block.x, per = least <= 2 ? least : 4, trigger = si_pdl_trigger_small(num_rows);
   block.x = ((width / 8 + per - 1) / per + 31) / 32 * 32;           // no more than have work: 2,048 x 5,632 gated 12.8 us with 512 threads, 11.1 with 352
   const int most = si_sm_count() * (int)(1024 / block.x);          // blocks that run at once
   if (!GATED && num_rows > most) grid.x = most;
-  const int shift = (group & (group - 1)) == 0 ? __builtin_ctz(group) : -1;
 #define ROWS_Q8(C) do { if constexpr (GATED) si_launch(gated_q8_kernel<TX, C>, grid, block, 0, stream, xp, o, scale, width, group, shift, trigger); \
                         else si_launch(rows_q8_kernel<TX, C>, grid, block, 0, stream, xp, ldx, o, scale, width, num_rows, trigger); } while (0)
   if (per == 1) ROWS_Q8(1); else if (per == 2) ROWS_Q8(2); else ROWS_Q8(4);

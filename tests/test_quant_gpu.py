@@ -50,7 +50,7 @@ def norm_exact(resid, deltas, weight, eps, rows=None):
 
 # width 1,336 has whole chunks of eight; 1,001 and 5 have not; 16,392 is wider than what a block holds in registers
 @pytest.mark.parametrize("xdtype,wdtype", [(BF16, BF16), (BF16, F32), (F32, F32), (F32, BF16)])
-@pytest.mark.parametrize("R,d", [(1, 4096), (3, 1336), (70, 1001), (2, 5), (1, 1), (300, 2048), (2, 16384), (2, 16392)])
+@pytest.mark.parametrize("R,d", [(1, 4096), (3, 1336), (70, 1001), (2, 5), (1, 1), (300, 2048), (2, 16384), (2, 16392), (40, 4099), (3, 9001), (2, 16383), (2, 16385)])
 def test_add_rmsnorm_q8(xdtype, wdtype, R, d):
     g = gen(R * d)
     resid = torch.randn(R, d, generator=g, device=DEV) * 3
@@ -93,7 +93,7 @@ def test_add_rmsnorm_q8_of_chosen_rows(d):
 
 @pytest.mark.parametrize("dtype", [BF16, F32])
 @pytest.mark.parametrize("R,F,group", [(1, 8192, 8), (5, 1336, 8), (3, 1336, None), (4, 90, 9), (2, 7, 1), (1, 1, None), (200, 2816, 8), (2, 14336, 8),
-                                       (2, 16392, 8), (3, 24, 12)])
+                                       (2, 16392, 8), (3, 24, 12), (3, 4099, None), (2, 9001, None), (2, 9012, 12), (2, 8200, 4), (2, 16383, None), (2, 16385, 5)])
 def test_swiglu_q8(dtype, R, F, group):
     gu = (torch.randn(R, 2 * F, generator=gen(F), device=DEV) * 3).to(dtype)
     out, scale = torch.empty(R, F, dtype=E4M3, device=DEV), torch.empty(R, device=DEV)
@@ -108,7 +108,7 @@ def test_swiglu_q8(dtype, R, F, group):
 
 @pytest.mark.parametrize("dtype", [BF16, F32])
 @pytest.mark.parametrize("R,n,stride", [(1, 4096, 4096), (61, 4096, 6144), (7, 1001, 1001), (3, 1000, 1003), (2, 1, 5), (700, 64, 72), (2, 16384, 16384),
-                                        (3, 20000, 20000)])
+                                        (3, 20000, 20000), (3, 4099, 4099), (2, 9001, 9003), (2, 16383, 16383), (2, 16385, 16385)])
 def test_quantize_q8(dtype, R, n, stride):
     x = (torch.randn(R, stride, generator=gen(n), device=DEV) * 5).to(dtype)[:, :n]
     out, scale = torch.empty(R, n, dtype=E4M3, device=DEV), torch.empty(R, device=DEV)
