@@ -8,6 +8,11 @@
 // holds every value exactly: e4m3 to fp16 (its range and its three mantissa bits fit), bf16 stays. A 4-bit weight times its scale is rounded
 // to bf16 there (off by at most 2^-8 of its value), as gemm_w4.cu does for many rows. Sums are fp32. Rows of 32 entries lie 80 bytes apart:
 // ldmatrix's eight rows then fall into different banks.
+//
+// Where tiles are fewer than blocks that run at once, the k steps of one are shared by the blocks of a cluster; each leaves its sums in its shared memory
+// and adds a part of the rows up over all blocks, in their order (us with one block a tile and so: 8 bits 8 x 4,000 x 4,088 137, 25; 61 x 500 x 7,000 236, 35;
+// 4 bits 212, 37 and 303, 45).
+#include "tma_common.cuh"
 #include "quant_common.cuh"
 
 typedef __nv_bfloat16 bf16;
@@ -50,6 +55,12 @@ __device__ __forceinline__ void gq_load(const unsigned char* row, int k, int len
   }
 }
 
+__device__ __forceinline__ float gq_ld_cluster(unsigned cluster_addr) {
+  float v;
+  asm volatile("ld.shared::cluster.f32 %0, [%1];\n" : "=f"(v) : "r"(cluster_addr) : "memory");
+  return v;
+}
+
 struct QuantProduct {
   const void* x; long long ldx;           // e4m3 or bf16, entries between rows
   const void* w; long long ldw;           // e4m3 (entries) or int32 words of eight entries (words)
@@ -60,11 +71,15 @@ struct QuantProduct {
 };
 
 template <bool W4, typename TO>
-__global__ void __launch_bounds__(256) gemm_quant_kernel(const QuantProduct p, TO* __restrict__ out, long long ldo, int n_tiles) {
-  __shared__ __align__(16) unsigned short As[2][GQ_BM * GQ_LD], Bs[2][GQ_BN * GQ_LD];
+__global__ void __launch_bounds__(256) gemm_quant_kernel(const QuantProduct p, TO* out, long long ldo, int n_tiles, int parts) {
+  __shared__ __align__(16) unsigned char raw[GQ_BM * GQ_BN * 4];              // two buffers of both operands, then the block's sums
+  unsigned short (*As)[GQ_BM * GQ_LD] = reinterpret_cast<unsigned short (*)[GQ_BM * GQ_LD]>(raw);
+  unsigned short (*Bs)[GQ_BN * GQ_LD] = reinterpret_cast<unsigned short (*)[GQ_BN * GQ_LD]>(raw + 2 * sizeof(*As));
+  static_assert(2 * (sizeof(*As) + sizeof(*Bs)) <= sizeof(raw), "the operands fit");
   pdl_wait();
   const int tid = threadIdx.x, warp = tid >> 5, lane = tid & 31;
-  const int m0 = (int)(blockIdx.x / n_tiles) * GQ_BM, n0 = (int)(blockIdx.x % n_tiles) * GQ_BN;
+  const int tile = (int)(blockIdx.x / parts), part = parts > 1 ? (int)cluster_cta_rank() : 0;
+  const int m0 = tile / n_tiles * GQ_BM, n0 = tile % n_tiles * GQ_BN;
   // who fetches what of a step: eight entries of a row of x, sixteen of a row of W
   const int am = tid >> 2, ak = (tid & 3) * 8, bn = tid >> 1, bk = (tid & 1) * 16;
   const bool a_in = m0 + am < p.M, b_in = n0 + bn < p.N;
@@ -119,12 +134,12 @@ __global__ void __launch_bounds__(256) gemm_quant_kernel(const QuantProduct p, T
 #pragma unroll
     for (int j = 0; j < 4; ++j) acc[i][j][0] = acc[i][j][1] = acc[i][j][2] = acc[i][j][3] = 0.f;
   const int wm = (warp >> 2) * 32, wn = (warp & 3) * 32;
-  const int steps = (p.K + GQ_BK - 1) / GQ_BK;
-  fetch(0);
-  put(0, 0);
+  const int all = (p.K + GQ_BK - 1) / GQ_BK, first = (int)((long long)all * part / parts), steps = (int)((long long)all * (part + 1) / parts);
+  fetch(first * GQ_BK);
+  put(0, first * GQ_BK);
   __syncthreads();
-  for (int st = 0; st < steps; ++st) {
-    const int buf = st & 1;
+  for (int st = first; st < steps; ++st) {
+    const int buf = (st - first) & 1;
     if (st + 1 < steps) fetch((st + 1) * GQ_BK);
 #pragma unroll
     for (int kk = 0; kk < GQ_BK; kk += 16) {
@@ -141,6 +156,33 @@ __global__ void __launch_bounds__(256) gemm_quant_kernel(const QuantProduct p, T
     }
     if (st + 1 < steps) put(buf ^ 1, (st + 1) * GQ_BK);       // the other buffer: all warps left it before the last barrier
     __syncthreads();
+  }
+  if (parts > 1) {
+    float* sums = reinterpret_cast<float*>(raw);
+#pragma unroll
+    for (int i = 0; i < 2; ++i)
+#pragma unroll
+      for (int j = 0; j < 4; ++j)
+#pragma unroll
+        for (int e = 0; e < 4; ++e) sums[(wm + i * 16 + (lane >> 2) + (e >> 1) * 8) * GQ_BN + wn + j * 8 + (lane & 3) * 2 + (e & 1)] = acc[i][j][e];
+    cluster_sync_all();                                       // every block's sums lie in its shared memory
+    const int lo = GQ_BM * part / parts, rows = GQ_BM / parts;
+    for (int i = tid; i < rows * GQ_BN; i += 256) {
+      const int m = m0 + lo + i / GQ_BN, n = n0 + i % GQ_BN;
+      const float* at = sums + lo * GQ_BN + i;
+      float t[8], v;
+#pragma unroll
+      for (int c = 0; c < 8; ++c) t[c] = c < parts ? gq_ld_cluster(cluster_map_u32(at, (unsigned)c)) : 0.f;
+      v = t[0];
+#pragma unroll
+      for (int c = 1; c < 8; ++c) v += t[c];
+      if (m < p.M && n < p.N) {
+        if (!W4) v = v * p.x_scale[m] * p.w_scale[n];
+        out[(size_t)m * ldo + n] = from_f32<TO>(v);
+      }
+    }
+    cluster_sync_all();                                       // no block goes while another one reads its sums
+    return;
   }
 #pragma unroll
   for (int i = 0; i < 2; ++i)
@@ -160,9 +202,24 @@ __global__ void __launch_bounds__(256) gemm_quant_kernel(const QuantProduct p, T
 template <bool W4>
 static int gq_launch(const QuantProduct& p, void* out, long long ldo, int out_dtype, cudaStream_t stream) {
   const long long n_tiles = (p.N + GQ_BN - 1) / GQ_BN, tiles = n_tiles * ((p.M + GQ_BM - 1) / GQ_BM);
-  if (tiles > 0x7fffffffLL) return -2;
-  if (out_dtype == SI_BF16) si_launch(gemm_quant_kernel<W4, bf16>, dim3((unsigned)tiles), dim3(256), 0, stream, p, (bf16*)out, ldo, (int)n_tiles);
-  else si_launch(gemm_quant_kernel<W4, float>, dim3((unsigned)tiles), dim3(256), 0, stream, p, (float*)out, ldo, (int)n_tiles);
+  if (tiles > 0x0fffffffLL) return -2;
+  int parts = 1;                                               // two blocks an SM, eight steps a block at least
+  while (parts < 8 && tiles * parts * 2 <= 2 * si_sm_count() && (p.K + GQ_BK - 1) / GQ_BK >= 16 * parts) parts *= 2;
+  cudaLaunchAttribute attr[2];
+  cudaLaunchConfig_t cfg = {};
+  cfg.gridDim = dim3((unsigned)(tiles * parts));
+  cfg.blockDim = dim3(256);
+  cfg.stream = stream;
+  attr[0].id = cudaLaunchAttributeClusterDimension;
+  attr[0].val.clusterDim.x = (unsigned)parts;
+  attr[0].val.clusterDim.y = 1;
+  attr[0].val.clusterDim.z = 1;
+  attr[1].id = cudaLaunchAttributeProgrammaticStreamSerialization;
+  attr[1].val.programmaticStreamSerializationAllowed = 1;
+  cfg.attrs = attr;
+  cfg.numAttrs = si_pdl_enabled() ? 2 : 1;
+  if (out_dtype == SI_BF16) cudaLaunchKernelEx(&cfg, gemm_quant_kernel<W4, bf16>, p, (bf16*)out, ldo, (int)n_tiles, parts);
+  else cudaLaunchKernelEx(&cfg, gemm_quant_kernel<W4, float>, p, (float*)out, ldo, (int)n_tiles, parts);
   return si_last_error();
 }
 

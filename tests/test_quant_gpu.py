@@ -376,6 +376,24 @@ def test_gemm_w4_rows_longer_than_a_block_holds(M, K, group):
     assert status.item() == 0 and torch.equal(out, want)
 
 
+@pytest.mark.parametrize("M", [1, 20, 70])
+@pytest.mark.parametrize("N,K", [(500, 7000), (90, 4097), (33, 8191), (2000, 2003), (50, 8184), (300, 4088)])
+def test_products_of_rows_on_no_boundary_cut_over_blocks(M, N, K):
+    g = gen(M + N + K)
+    a, w, sa, sw = whole_codes(g, M, K), whole_codes(g, N, K), powers(g, M), powers(g, N)
+    want = (torch.mm(a.double(), w.double().t()) * sa.double().unsqueeze(1) * sw.double()).to(F32)
+    for _ in range(3):
+        out = torch.full((M, N), float("nan"), device=DEV)
+        ops().gemm_q8(a, sa, w, sw, out)
+        assert torch.equal(out, want)
+    if K % 8 == 0:
+        words, s, z, w4 = w4_weight(g, N, K, 64, True)
+        x = torch.randint(-2, 3, (M, K), generator=g, device=DEV).to(BF16)
+        buf = torch.full((M, N + 3), 7.0, device=DEV)
+        ops().gemm_w4(x, words, s, z, 64, buf[:, :N])
+        assert torch.equal(buf[:, :N], torch.mm(x.double(), w4.t()).to(F32)) and (buf[:, N:] == 7).all()
+
+
 @pytest.mark.parametrize("M", [2, 40, 200])
 def test_gemm_w4_nan_stays_in_its_row_and_column(M):
     g = gen(M)
