@@ -158,6 +158,7 @@ gemm_q8_pair_kernel(const __grid_constant__ CUtensorMap amap, const __grid_const
 #pragma unroll 1
       for (int h = 0; h < BN / CW; ++h) {
         float v[CW / 32][32];
+        __syncwarp();                            // an aligned load: not every lane stored in the turn before
 #pragma unroll
         for (int c = 0; c < CW / 32; ++c) tmem_ld_32x32_issue(src + h * CW + c * 32, v[c]);
         tmem_ld_wait();
@@ -363,6 +364,7 @@ gemm_q8_rows_kernel(const __grid_constant__ CUtensorMap amap, const __grid_const
 #pragma unroll 1
     for (int m0 = 0; m0 < mpad && ok; m0 += 32) {
       float v[32];
+      __syncwarp();                                        // an aligned load: not every lane stored in the turn before
       tmem_ld_32x32(src + m0, v);
       if (parts == 1) {
 #pragma unroll
@@ -376,7 +378,6 @@ gemm_q8_rows_kernel(const __grid_constant__ CUtensorMap amap, const __grid_const
     }
   }
   if (parts > 1) {
-    __syncwarp();
     cluster_sync_all();                                   // every block's sums lie in its shared memory
     if (warp >= 3) {
       // four columns a thread, the parts' sums all on their way before the first is used
@@ -411,6 +412,7 @@ gemm_q8_rows_kernel(const __grid_constant__ CUtensorMap amap, const __grid_const
     }
     cluster_sync_all();                                   // no block goes while another one reads its sums
   }
+  __syncwarp();
   tc05_fence_before_sync();
   __syncthreads();
   if (warp == 2) tmem_dealloc(tmem, 2 * acc_cols);

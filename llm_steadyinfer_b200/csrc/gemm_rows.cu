@@ -190,7 +190,6 @@ gemm_rows_tile_kernel(const __grid_constant__ CUtensorMap xmap, const __grid_con
   if (parts > 1) {
     // every block's partial sum is in its shared memory: the cluster meets, block `part` adds its rows up over
     // all blocks in their order, and the cluster meets again before any block, and its shared memory, goes
-    __syncwarp();
     cluster_sync_all();
     if (warp >= 2) {
       const int q = warp & 3;

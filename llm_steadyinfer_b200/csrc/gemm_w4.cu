@@ -296,7 +296,6 @@ gemm_w4_few_kernel(const __grid_constant__ CUtensorMap wmap, const bf16* __restr
     }
   }
   if (!ok && lane == 0) set_status(status, SI_WAIT_LIMIT);
-  __syncwarp();
   if (parts > 1) {
     cluster_sync_all();                                         // every block's sums of its slice lie in its shared memory
     for (int i = threadIdx.x; i < mine * 128; i += W4_FEW_THREADS) {
@@ -694,6 +693,7 @@ gemm_w4_tc_kernel(const __grid_constant__ CUtensorMap xmap, const __grid_constan
 #pragma unroll 1
       for (int m0 = 0; m0 < bn; m0 += 32) {
         float v[32];
+        __syncwarp();                                      // an aligned load: not every lane stored in the turn before
         tmem_ld_32x32(tmem + lanes + (unsigned)(d * acc_w + m0), v);
         if (m0 + 32 >= bn) {                               // in registers: the issuer may have the accumulator back
           tc05_fence_before_sync();
@@ -711,7 +711,6 @@ gemm_w4_tc_kernel(const __grid_constant__ CUtensorMap xmap, const __grid_constan
     }
   }
   if (!PAIR && parts > 1) {                                // one tile a cluster
-    __syncwarp();
     cluster_sync_all();                                    // every block's sums lie in its shared memory
     const int m_base = first % m_tiles * bn, n0 = first / m_tiles * 128;
     const int lo = bn * part / parts, hi = min(M - m_base, bn * (part + 1) / parts);

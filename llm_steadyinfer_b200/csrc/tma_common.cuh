@@ -158,7 +158,10 @@ __device__ __forceinline__ unsigned cluster_cta_rank() {
   asm volatile("mov.u32 %0, %%cluster_ctarank;\n" : "=r"(r));
   return r;
 }
+// The barrier's instructions are of the aligned form, which all lanes of a warp have to make together: lanes that left a loop or a branch at
+// different times meet first.
 __device__ __forceinline__ void cluster_sync_all() {
+  __syncwarp();
   asm volatile("barrier.cluster.arrive.release.aligned;\n" ::: "memory");
   asm volatile("barrier.cluster.wait.acquire.aligned;\n" ::: "memory");
 }

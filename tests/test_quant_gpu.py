@@ -509,3 +509,19 @@ def test_two_streams_at_once():
                 o.gemm_w4(xs[k], words, s, z, 128, outs[k][i], None)
     torch.cuda.synchronize()
     assert all(torch.equal(outs[k][i], want[k]) for k in range(2) for i in range(8))
+
+
+@pytest.mark.parametrize("M,N,K", [(17, 24, 4096), (17, 72, 8192), (23, 200, 4096), (33, 40, 14336), (41, 1000, 4096), (65, 104, 8192), (129, 56, 4096), (250, 24, 8192)])
+def test_products_whose_blocks_add_up_few_sums(M, N, K):
+    """Tiles cut over a cluster whose blocks have, at the end, sums to add for a part of a warp's lanes only, and columns that no lane stores."""
+    g = gen(M + N + K)
+    a, w, sa, sw = whole_codes(g, M, K), whole_codes(g, N, K), powers(g, M), powers(g, N)
+    want = (torch.mm(a.double(), w.double().t()) * sa.double().unsqueeze(1) * sw.double()).to(F32)
+    words, s, z, w4 = w4_weight(g, N, K, 128, True)
+    x = torch.randint(-1, 2, (M, K), generator=g, device=DEV).to(BF16)
+    want4 = torch.mm(x.double(), w4.t()).to(F32)
+    for _ in range(3):
+        out, out4, status = torch.full((M, N), float("nan"), device=DEV), torch.full((M, N), float("nan"), device=DEV), status_word()
+        ops().gemm_q8(a, sa, w, sw, out, status)
+        ops().gemm_w4(x, words, s, z, 128, out4, status)
+        assert status.item() == 0 and torch.equal(out, want) and torch.equal(out4, want4)

@@ -220,3 +220,21 @@ def test_quantize_w4_on_the_cpu():
         assert ((q.dense().double() - w.double()).abs() <= step * (1 + 15 * 2.0 ** -8)).all()
     with pytest.raises(ValueError, match="multiple of 8"):
         quantize(w[:, :100].contiguous()[:, :99], "w4")
+
+
+def test_aligned_cluster_barriers_are_met_by_whole_warps():
+    """``barrier.cluster`` in its aligned form is undefined unless all lanes of a warp make it together; behind a loop or a branch that lanes leave at
+    different times nothing but a warp barrier sees to that. So the one helper that issues it brings the warp together first, and no kernel issues it itself."""
+    import glob
+    import os
+    folder = os.path.dirname(ops.__file__)
+    found = {}
+    for path in sorted(glob.glob(os.path.join(folder, "*.cu*"))):
+        with open(path) as f:
+            text = f.read()
+        if "barrier.cluster" in text:
+            found[os.path.basename(path)] = text
+    assert list(found) == ["tma_common.cuh"]
+    body = found["tma_common.cuh"].split("void cluster_sync_all() {")[1].split("}")[0]
+    assert found["tma_common.cuh"].count("barrier.cluster.arrive") == 1 and found["tma_common.cuh"].count("barrier.cluster.wait") == 1
+    assert body.index("__syncwarp();") < body.index("barrier.cluster.arrive") < body.index("barrier.cluster.wait")
