@@ -475,14 +475,16 @@ __device__ __forceinline__ void w4_take_row(const unsigned char* row, int swz, u
 #pragma unroll
   for (int j = 0; j < 4; ++j) wv[j] = *reinterpret_cast<const uint4*>(row + ((j ^ swz) << 4));
 }
-// ... as bf16 into 64 columns of its lane of tensor memory, a piece of 32 entries (16 columns) at a time.
-template <bool ZEROS, bool SMALL>
-__device__ __forceinline__ void w4_widen_row(const uint4 (&wv)[4], const unsigned* scale, const unsigned* zero, unsigned a) {
+// ... as bf16 into 64 columns of its lane of tensor memory, a piece of 32 entries (16 columns) at a time. TAIL: the row ends `left` entries from here. What
+// the step holds beyond stands for nothing, but its words are zeros, which the last group's zero point and scale may make infinite, and x's zeros with that
+// NaN; so their scale is zero. (A form of its own: the choice of a scale a piece would be a thirtieth of the instructions of every step.)
+template <bool ZEROS, bool SMALL, bool TAIL>
+__device__ __forceinline__ void w4_widen_row(const uint4 (&wv)[4], const unsigned* scale, const unsigned* zero, unsigned a, int left) {
 #pragma unroll
   for (int j = 0; j < 4; ++j) {
     const int i = SMALL ? j : 0;
     const __nv_bfloat162 bias = ZEROS ? w4_bias((int)zero[i]) : __float2bfloat162_rn(136.f);
-    const unsigned s2 = scale[i] | (scale[i] << 16);
+    const unsigned s2 = TAIL && 32 * j >= left ? 0u : scale[i] | (scale[i] << 16);
     const unsigned words[4] = {wv[j].x, wv[j].y, wv[j].z, wv[j].w};
     unsigned v[16];
 #pragma unroll
@@ -664,7 +666,9 @@ gemm_w4_tc_kernel(const __grid_constant__ CUtensorMap xmap, const __grid_constan
         if (uses > 0) ok = w4_wait(&empty_bar[slot], (unsigned)((uses - 1) & 1));
         if (!ok) break;
         tc05_fence_after_sync();
-        w4_widen_row<ZEROS, SMALL>(wv, now, z, mine + (unsigned)(slot * 128));
+        const int left = K - (2 * k0 + at) * 128;            // a multiple of 32, as K is
+        if (left >= 128) w4_widen_row<ZEROS, SMALL, false>(wv, now, z, mine + (unsigned)(slot * 128), left);
+        else w4_widen_row<ZEROS, SMALL, true>(wv, now, z, mine + (unsigned)(slot * 128), left);
         tc05_fence_before_sync();
         __syncwarp();
         if (lane == 0) {

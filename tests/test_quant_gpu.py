@@ -525,3 +525,28 @@ def test_products_whose_blocks_add_up_few_sums(M, N, K):
         ops().gemm_q8(a, sa, w, sw, out, status)
         ops().gemm_w4(x, words, s, z, 128, out4, status)
         assert status.item() == 0 and torch.equal(out, want) and torch.equal(out4, want4)
+
+
+@pytest.mark.parametrize("M", [1, 9, 40, 130, 300])
+@pytest.mark.parametrize("K,group,zeros", [(288, 64, False), (288, 128, True), (416, 32, True), (416, 512, False), (4000, 128, False), (2848, 64, True)])
+def test_gemm_w4_large_scales_behind_the_rows_end(M, K, group, zeros):
+    """Rows that end inside a step, the last group's scale so large that anything but zero times it is infinite in what a step holds beyond the end: its entries
+    stand for zero, but for one of size one step beside an x so small that the product is ordinary."""
+    g = gen(M + K + group)
+    N = 200
+    G = -(-K // group)
+    q = torch.randint(0, 16, (N, K), generator=g, device=DEV)
+    z = torch.randint(1, 15, (N, G), generator=g, device=DEV).to(torch.uint8) if zeros else None
+    s = torch.exp2(torch.randint(-1, 2, (N, G), generator=g, device=DEV).float())
+    s[:, -1] = 2.0 ** 127
+    lo = (G - 1) * group
+    q[:, lo:] = z[:, -1:].long() if zeros else 8
+    q[:, lo + 1] += torch.randint(-1, 2, (N,), generator=g, device=DEV)
+    x = torch.randint(-4, 5, (M, K), generator=g, device=DEV).float()
+    x[:, lo + 1] *= 2.0 ** -126
+    at = torch.arange(K, device=DEV) // group
+    w = (q.double() - (z.double()[:, at] if zeros else 8.0)) * s.double()[:, at]
+    want = torch.mm(x.double(), w.t()).to(F32)
+    out, status = torch.full((M, N), float("nan"), device=DEV), status_word()
+    ops().gemm_w4(x.to(BF16), ops().pack_w4(q), s.to(BF16), z, group, out, status)
+    assert status.item() == 0 and torch.equal(out, want)
