@@ -53,7 +53,7 @@ static int encode_u8_2d(CUtensorMap* map, const void* base, long long rows, long
 // of narrow tiles do not fill (256 x 4,096 x 14,336, 64 columns: 33.7 us with one box, 23.9 with two; 2,048 x 6,144 x 4,096, 256 columns: 39 and 45). Two CTAs (a cluster) take a tile of 256 x BN: each fetches its 128 rows of a and BN / 2 of w a step, the leader issues
 // over both CTAs' shared memory, each CTA stores its 128 rows. Two accumulators in tensor memory: a tile is stored while the next one runs.
 template <int STAGES, typename TO, int BN, int BK>
-__global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(192)
+__global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(192, 1)
 gemm_q8_pair_kernel(const __grid_constant__ CUtensorMap amap, const __grid_constant__ CUtensorMap bmap, const float* sa,
                     const float* sw, TO* __restrict__ out, long long ldo, int M, int N, int K, int* status, int trigger) {
   constexpr int BM = 128, BOXES = BK / 128;               // boxes of 128 entries a step
@@ -149,6 +149,7 @@ gemm_q8_pair_kernel(const __grid_constant__ CUtensorMap amap, const __grid_const
       const int buf = local & 1;
       const int row = (tile % m_tiles) * 2 * BM + (int)rank * BM + q * 32 + lane, n0 = (tile / m_tiles) * BN;
       const float rs = row < M ? sa[row] : 0.f;
+      const bool plain = q8_plain(rs, q8_range(sw, n0, min(n0 + BN, N)));
       if (!mbar_wait_warp(&acc_full[buf], (unsigned)((local >> 1) & 1))) {
         if (lane == 0) set_status(status, SI_WAIT_LIMIT);
         break;
@@ -173,10 +174,15 @@ gemm_q8_pair_kernel(const __grid_constant__ CUtensorMap amap, const __grid_const
           if (row < M && n < N) {
             TO* dst = out + (size_t)row * ldo + n;
             if (vec && n + 32 <= N) {
+              if (plain) {
 #pragma unroll
-              for (int i = 0; i < 8; ++i) {
-                const float4 s4 = reinterpret_cast<const float4*>(sw + n)[i];
-                v[c][4 * i] *= rs * s4.x; v[c][4 * i + 1] *= rs * s4.y; v[c][4 * i + 2] *= rs * s4.z; v[c][4 * i + 3] *= rs * s4.w;
+                for (int i = 0; i < 8; ++i) {
+                  const float4 s4 = reinterpret_cast<const float4*>(sw + n)[i];
+                  v[c][4 * i] *= rs * s4.x; v[c][4 * i + 1] *= rs * s4.y; v[c][4 * i + 2] *= rs * s4.z; v[c][4 * i + 3] *= rs * s4.w;
+                }
+              } else {
+#pragma unroll
+                for (int i = 0; i < 32; ++i) v[c][i] = q8_scaled_wide(v[c][i], rs, sw[n + i]);
               }
               if constexpr (sizeof(TO) == 4) {
 #pragma unroll
@@ -193,7 +199,7 @@ gemm_q8_pair_kernel(const __grid_constant__ CUtensorMap amap, const __grid_const
               }
             } else {
 #pragma unroll
-              for (int i = 0; i < 32; ++i) if (n + i < N) dst[i] = from_f32<TO>(v[c][i] * (rs * sw[n + i]));
+              for (int i = 0; i < 32; ++i) if (n + i < N) dst[i] = from_f32<TO>(plain ? v[c][i] * (rs * sw[n + i]) : q8_scaled_wide(v[c][i], rs, sw[n + i]));
             }
           }
         }
@@ -357,6 +363,9 @@ gemm_q8_rows_kernel(const __grid_constant__ CUtensorMap amap, const __grid_const
     const int acc = (warp - 3) >> 2, c = acc * 128 + (warp & 3) * 32 + lane, n = n0 + c;
     const bool in = c < h && n < N;
     const float cs = in ? sw[n] : 0.f;
+    float2 rows = make_float2(1.f, 1.f);
+    if (parts == 1) rows = q8_range(sa, 0, M);              // alike for the block: all lanes take part
+    const bool plain = !in || q8_plain(cs, rows);
     const bool ok = mbar_wait_warp(&acc_full, 0);         // every part has a step at least
     if (!ok && lane == 0) set_status(status, SI_WAIT_LIMIT);
     tc05_fence_after_sync();
@@ -367,9 +376,13 @@ gemm_q8_rows_kernel(const __grid_constant__ CUtensorMap amap, const __grid_const
       __syncwarp();                                        // an aligned load: not every lane stored in the turn before
       tmem_ld_32x32(src + m0, v);
       if (parts == 1) {
+        if (!plain) {
+#pragma unroll
+          for (int j = 0; j < 32; ++j) if (m0 + j < M) v[j] = q8_scaled_wide(v[j], sa[m0 + j], cs);
+        }
 #pragma unroll
         for (int j = 0; j < 32; ++j)
-          if (m0 + j < M && in) out[(size_t)(m0 + j) * ldo + n] = from_f32<TO>(v[j] * (sa[m0 + j] * cs));
+          if (m0 + j < M && in) out[(size_t)(m0 + j) * ldo + n] = from_f32<TO>(plain ? v[j] * (sa[m0 + j] * cs) : v[j]);
       } else {
 #pragma unroll
         for (int j = 0; j < 32; ++j)
@@ -397,7 +410,14 @@ gemm_q8_rows_kernel(const __grid_constant__ CUtensorMap amap, const __grid_const
         if (vec && n + 4 <= N) {
           float y[4];
 #pragma unroll
-          for (int j = 0; j < 4; ++j) y[j] = r[j] * (rs * sw[n + j]);
+          for (int j = 0; j < 4; ++j) y[j] = rs * sw[n + j];
+          if (q8_normal(y[0]) && q8_normal(y[1]) && q8_normal(y[2]) && q8_normal(y[3])) {
+#pragma unroll
+            for (int j = 0; j < 4; ++j) y[j] *= r[j];
+          } else {
+#pragma unroll
+            for (int j = 0; j < 4; ++j) y[j] = q8_scaled_wide(r[j], rs, sw[n + j]);
+          }
           if constexpr (sizeof(TO) == 4) {
             *reinterpret_cast<float4*>(dst) = make_float4(y[0], y[1], y[2], y[3]);
           } else {
@@ -406,7 +426,7 @@ gemm_q8_rows_kernel(const __grid_constant__ CUtensorMap amap, const __grid_const
           }
         } else {
 #pragma unroll
-          for (int j = 0; j < 4; ++j) if (n + j < N) dst[j] = from_f32<TO>(r[j] * (rs * sw[n + j]));
+          for (int j = 0; j < 4; ++j) if (n + j < N) dst[j] = from_f32<TO>(q8_scaled(r[j], rs, sw[n + j]));
         }
       }
     }
@@ -585,7 +605,7 @@ gemm_q8_skinny_kernel(const u8* a, long long lda, const float* sa, const u8* w, 
 #pragma unroll
       for (int v = 0; v < WARPS; ++v) s += red[par][(v * MT + mt) * 32 + ln][e];
       const int n = now * 16 + (ln >> 2) + ((e >> 1) ? 8 : 0), m = mt * 8 + (ln & 3) * 2 + (e & 1);
-      if (n < N && m < M) out[(size_t)m * ldo + n] = from_f32<TO>(s * (sa[m] * sw[n]));
+      if (n < N && m < M) out[(size_t)m * ldo + n] = from_f32<TO>(q8_scaled(s, sa[m], sw[n]));
     }
   }
 }

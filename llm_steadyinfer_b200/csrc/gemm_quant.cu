@@ -177,7 +177,7 @@ __global__ void __launch_bounds__(256) gemm_quant_kernel(const QuantProduct p, T
 #pragma unroll
       for (int c = 1; c < 8; ++c) v += t[c];
       if (m < p.M && n < p.N) {
-        if (!W4) v = v * p.x_scale[m] * p.w_scale[n];
+        if (!W4) v = q8_scaled(v, p.x_scale[m], p.w_scale[n]);
         out[(size_t)m * ldo + n] = from_f32<TO>(v);
       }
     }
@@ -193,7 +193,7 @@ __global__ void __launch_bounds__(256) gemm_quant_kernel(const QuantProduct p, T
         const int m = m0 + wm + i * 16 + (lane >> 2) + (e >> 1) * 8, n = n0 + wn + j * 8 + (lane & 3) * 2 + (e & 1);
         if (m < p.M && n < p.N) {
           float v = acc[i][j][e];
-          if (!W4) v = v * p.x_scale[m] * p.w_scale[n];
+          if (!W4) v = q8_scaled(v, p.x_scale[m], p.w_scale[n]);
           out[(size_t)m * ldo + n] = from_f32<TO>(v);
         }
       }

@@ -18,6 +18,29 @@
 __device__ __forceinline__ float q8_scale(float amax) { return fmaxf(amax, SI_Q8_LEAST) / SI_E4M3_MAX; }
 __device__ __forceinline__ float q8_factor(float amax) { return SI_E4M3_MAX / fmaxf(amax, SI_Q8_LEAST); }
 
+// A product's sum times the row's and the column's scale. Scales reach from 2^-100 / 448 to 2^119 and a sum from 2^-18 up, so that each of the two
+// orders in fp32 loses some result that is an ordinary number: the product of the scales may be subnormal, zero or infinite, and so may the sum times
+// one of them. Where the product of the scales is a normal number it is taken; else 64 bits are, which hold all of it.
+__device__ __forceinline__ bool q8_normal(float p) { return fabsf(p) >= 1.1754943508222875e-38f && fabsf(p) <= 3.4028234663852886e38f; }
+__device__ __forceinline__ float q8_scaled_wide(float sum, float sa, float sw) { return (float)((double)sum * (double)sa * (double)sw); }
+__device__ __forceinline__ float q8_scaled(float sum, float sa, float sw) {
+  const float p = sa * sw;
+  return q8_normal(p) ? sum * p : q8_scaled_wide(sum, sa, sw);
+}
+// The least and the largest size of the scales s[from .. to), for every lane of a warp (as whole numbers, which order sizes alike; NaN is the largest). A
+// tile asks once, before it waits for its sums: with a test an output 61 x 28,672 x 4,096 took 27.0 us for 25.2.
+__device__ __forceinline__ float2 q8_range(const float* s, int from, int to) {
+  unsigned least = 0x7fffffffu, most = 0;
+  for (int i = from + (int)(threadIdx.x & 31); i < to; i += 32) {
+    const unsigned b = __float_as_uint(s[i]) & 0x7fffffffu;
+    least = min(least, b);
+    most = max(most, b);
+  }
+  return make_float2(__uint_as_float(__reduce_min_sync(0xffffffffu, least)), __uint_as_float(__reduce_max_sync(0xffffffffu, most)));
+}
+// Whether the product of `scale` and any of that range is a normal number.
+__device__ __forceinline__ bool q8_plain(float scale, float2 range) { return q8_normal(scale * range.x) && q8_normal(scale * range.y); }
+
 __device__ __forceinline__ unsigned q8_pack2(float a, float b) {      // two codes, a in the low byte
   return (unsigned)__nv_cvt_float2_to_fp8x2(make_float2(a, b), __NV_SATFINITE, __NV_E4M3);
 }

@@ -550,3 +550,20 @@ def test_gemm_w4_large_scales_behind_the_rows_end(M, K, group, zeros):
     out, status = torch.full((M, N), float("nan"), device=DEV), status_word()
     ops().gemm_w4(x.to(BF16), ops().pack_w4(q), s.to(BF16), z, group, out, status)
     assert status.item() == 0 and torch.equal(out, want)
+
+
+@pytest.mark.parametrize("M", [1, 8, 16, 40, 128, 300, 600])
+@pytest.mark.parametrize("N,K", [(160, 512), (150, 500), (24, 8192), (4096, 256), (61, 4100), (1000, 4096)])
+def test_gemm_q8_scales_whose_product_is_no_fp32_number(M, N, K):
+    """Scales down to 2^-100 and up to 2^119 (a row's scale is its largest entry over 448): their product may lie beyond fp32 on either side where the result does
+    not, and the sum times one of them may where the result does not either. All are powers of two: one rounding, where the result is subnormal."""
+    g = gen(M + N + K)
+    a, w = whole_codes(g, M, K), whole_codes(g, N, K)
+    w[3::7] = 0                                                  # sums that are zero, whatever the scales
+    sa = torch.exp2(torch.tensor([-75.0, 0, 119, -100, 60], device=DEV))[torch.arange(M, device=DEV) % 5 if M > 4 else torch.arange(M, device=DEV) + 2]
+    sw = torch.exp2(torch.tensor([-75.0, -60, 100, 0, -119, 70, -30], device=DEV))[torch.arange(N, device=DEV) % 7 if N < 1000 else torch.arange(N, device=DEV) // 7 % 7]
+    want = (torch.mm(a.double(), w.double().t()) * sa.double().unsqueeze(1) * sw.double()).to(F32)
+    for dtype in (F32, BF16):
+        out, status = torch.full((M, N), float("nan"), dtype=dtype, device=DEV), status_word()
+        ops().gemm_q8(a, sa, w, sw, out, status)
+        assert status.item() == 0 and torch.equal(out, want.to(dtype))
