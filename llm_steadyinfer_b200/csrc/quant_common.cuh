@@ -15,9 +15,28 @@
 #define SI_E4M3_MAX 448.f
 #define SI_Q8_LEAST 7.888609052210118e-31f      // 2^-100
 
-__device__ __forceinline__ float q8_scale(float amax) { return fmaxf(amax, SI_Q8_LEAST) / SI_E4M3_MAX; }
-__device__ __forceinline__ float q8_factor(float amax) { return SI_E4M3_MAX / fmaxf(amax, SI_Q8_LEAST); }
-
+// What a row's entries are divided by on their way to codes: y / scale, rounded to fp32 as a division would, then to e4m3. A product with the inverse rounded
+// to fp32 is up to two units off, and puts entries halfway between two codes on either side: of bf16 entries below a bf16 maximum one in 3,000. So the inverse
+// is kept in two parts, the hardware's approximation (2^-23) and what is left of one behind it; the fused sum of their products with y is off by half a unit
+// and 2^-45 of the value, and exact where the quotient is. Two entries at a time: as many instructions as one product an entry. The scale's own quotient is a
+// product and its exact remainder. An infinite maximum leaves zeros, and NaN of infinite entries.
+struct Q8Row {
+  float scale, inverse, rest;
+  __device__ __forceinline__ explicit Q8Row(float amax) {
+    constexpr float part = 1.f / SI_E4M3_MAX;
+    amax = fmaxf(amax, SI_Q8_LEAST);
+    const bool finite = amax <= 3.4028234663852886e38f;
+    const float q = amax * part;
+    scale = finite ? __fmaf_rn(__fmaf_rn(q, -SI_E4M3_MAX, amax), part, q) : amax;
+    asm("rcp.approx.ftz.f32 %0, %1;" : "=f"(inverse) : "f"(scale));
+    rest = finite ? __fmaf_rn(-inverse, scale, 1.f) * inverse : 0.f;
+  }
+  __device__ __forceinline__ float operator()(float y) const { return __fmaf_rn(y, inverse, y * rest); }
+  __device__ __forceinline__ void operator()(float& a, float& b) const {
+    asm("{\n.reg .b64 y, f, g;\nmov.b64 y, {%0, %1};\nmov.b64 f, {%2, %2};\nmov.b64 g, {%3, %3};\n"
+        "mul.rn.f32x2 g, y, g;\nfma.rn.f32x2 y, y, f, g;\nmov.b64 {%0, %1}, y;\n}\n" : "+f"(a), "+f"(b) : "f"(inverse), "f"(rest));
+  }
+};
 // A product's sum times the row's and the column's scale. Scales reach from 2^-100 / 448 to 2^119 and a sum from 2^-18 up, so that each of the two
 // orders in fp32 loses some result that is an ordinary number: the product of the scales may be subnormal, zero or infinite, and so may the sum times
 // one of them. Where the product of the scales is a normal number it is taken; else 64 bits are, which hold all of it.
@@ -44,10 +63,12 @@ __device__ __forceinline__ bool q8_plain(float scale, float2 range) { return q8_
 __device__ __forceinline__ unsigned q8_pack2(float a, float b) {      // two codes, a in the low byte
   return (unsigned)__nv_cvt_float2_to_fp8x2(make_float2(a, b), __NV_SATFINITE, __NV_E4M3);
 }
-__device__ __forceinline__ uint2 q8_pack8(const float (&v)[8]) {
+__device__ __forceinline__ uint2 q8_pack8(const Q8Row& to, float (&v)[8]) {
+#pragma unroll
+  for (int i = 0; i < 8; i += 2) to(v[i], v[i + 1]);
   return make_uint2(q8_pack2(v[0], v[1]) | (q8_pack2(v[2], v[3]) << 16), q8_pack2(v[4], v[5]) | (q8_pack2(v[6], v[7]) << 16));
 }
-__device__ __forceinline__ unsigned char q8_pack1(float a) { return (unsigned char)__nv_cvt_float_to_fp8(a, __NV_SATFINITE, __NV_E4M3); }
+__device__ __forceinline__ unsigned char q8_pack1(const Q8Row& to, float a) { return (unsigned char)__nv_cvt_float_to_fp8(to(a), __NV_SATFINITE, __NV_E4M3); }
 
 // Pair p (entries 2p, 2p + 1) of a word of eight 4-bit entries as two bf16 of value 128 + q: bf16 counts in ones from 128 to 255, so
 // the four bits go straight into the mantissa.

@@ -144,16 +144,16 @@ __global__ void __launch_bounds__(512) norm_q8_kernel(const NormArgs a, unsigned
   }
   const float2 both = block_sum_max(ss, top, scratch);
   const float inv = rsqrtf(both.x / (float)width + a.eps);
-  const float amax = both.y * inv, f = q8_factor(amax);          // applied after inv: their product may pass fp32's range
-  if (threadIdx.x == 0) scale[r] = q8_scale(amax);
+  const Q8Row to(both.y * inv);
+  if (threadIdx.x == 0) scale[r] = to.scale;
   unsigned char* o = out + (size_t)r * width;
 #pragma unroll
   for (int c = 0; c < CHUNKS; ++c) {
     const int ch = threadIdx.x + c * blockDim.x;
     if (ch < nchunks) {
 #pragma unroll
-      for (int i = 0; i < 8; ++i) x[c][i] = x[c][i] * inv * f;
-      *reinterpret_cast<uint2*>(o + ch * 8) = q8_pack8(x[c]);
+      for (int i = 0; i < 8; ++i) x[c][i] *= inv;
+      *reinterpret_cast<uint2*>(o + ch * 8) = q8_pack8(to, x[c]);
     }
   }
 }
@@ -190,12 +190,12 @@ __global__ void __launch_bounds__(1024) norm_q8_odd_kernel(const NormArgs a, uns
   }
   const float2 both = block_sum_max(ss, top, scratch);
   const float inv = rsqrtf(both.x / (float)width + a.eps);
-  const float amax = both.y * inv, f = q8_factor(amax);
-  if (threadIdx.x == 0) scale[r] = q8_scale(amax);
+  const Q8Row to(both.y * inv);
+  if (threadIdx.x == 0) scale[r] = to.scale;
 #pragma unroll
   for (int k = 0; k < K; ++k) {
     const int i = threadIdx.x + k * blockDim.x;
-    if (i < width) out[(size_t)r * width + i] = q8_pack1(x[k] * inv * f);
+    if (i < width) out[(size_t)r * width + i] = q8_pack1(to, x[k] * inv);
   }
 }
 
@@ -223,11 +223,11 @@ __global__ void norm_q8_scalar_kernel(const NormArgs a, unsigned char* out, floa
   }
   const float2 both = block_sum_max(ss, top, scratch);
   const float inv = rsqrtf(both.x / (float)width + a.eps);
-  const float amax = both.y * inv, f = q8_factor(amax);
-  if (threadIdx.x == 0) scale[r] = q8_scale(amax);
+  const Q8Row to(both.y * inv);
+  if (threadIdx.x == 0) scale[r] = to.scale;
   for (int i = threadIdx.x; i < width; i += blockDim.x) {            // what this thread stored itself, where the stream was written
     const float h = a.dst ? a.dst[src + i] : entry(i);
-    out[(size_t)r * width + i] = q8_pack1(h * to_f32<TW>(weight[i]) * inv * f);
+    out[(size_t)r * width + i] = q8_pack1(to, h * to_f32<TW>(weight[i]) * inv);
   }
 }
 
@@ -274,16 +274,14 @@ rows_q8_kernel(const TX* x, long long ldx, unsigned char* out, float* scale, int
         for (int i = 0; i < 8; ++i) top = fmaxf(top, fabsf(v[i]));
       }
     top = block_sum_max(0.f, top, scratch[par]).y;      // a buffer is written again two rows later, behind the next row's barrier
-    const float f = q8_factor(top);
-    if (threadIdx.x == 0) scale[r] = q8_scale(top);
+    const Q8Row to(top);
+    if (threadIdx.x == 0) scale[r] = to.scale;
 #pragma unroll
     for (int c = 0; c < CHUNKS; ++c) {
       const int ch = threadIdx.x + c * blockDim.x;
       if (ch < nchunks) {
         raw[c].get(v);
-#pragma unroll
-        for (int i = 0; i < 8; ++i) v[i] *= f;
-        *reinterpret_cast<uint2*>(out + (size_t)r * width + ch * 8) = q8_pack8(v);
+        *reinterpret_cast<uint2*>(out + (size_t)r * width + ch * 8) = q8_pack8(to, v);
       }
     }
   }
@@ -324,15 +322,13 @@ __global__ void __launch_bounds__(512, CHUNKS <= 2 && sizeof(TX) == 2 ? 3 : 2) g
       }
     }
   top = block_sum_max(0.f, top, scratch).y;
-  const float f = q8_factor(top);
-  if (threadIdx.x == 0) scale[r] = q8_scale(top);
+  const Q8Row to(top);
+  if (threadIdx.x == 0) scale[r] = to.scale;
 #pragma unroll
   for (int c = 0; c < CHUNKS; ++c) {
     const int ch = threadIdx.x + c * blockDim.x;
     if (ch < nchunks) {
-#pragma unroll
-      for (int i = 0; i < 8; ++i) v[c][i] *= f;
-      *reinterpret_cast<uint2*>(out + (size_t)r * width + ch * 8) = q8_pack8(v[c]);
+      *reinterpret_cast<uint2*>(out + (size_t)r * width + ch * 8) = q8_pack8(to, v[c]);
     }
   }
 }
@@ -361,12 +357,12 @@ __global__ void __launch_bounds__(1024) rows_q8_odd_kernel(const TX* x, long lon
     if (GATED) asm volatile("" ::: "memory");
   }
   top = block_sum_max(0.f, top, scratch).y;
-  const float f = q8_factor(top);
-  if (threadIdx.x == 0) scale[blockIdx.x] = q8_scale(top);
+  const Q8Row to(top);
+  if (threadIdx.x == 0) scale[blockIdx.x] = to.scale;
 #pragma unroll
   for (int k = 0; k < K; ++k) {
     const int i = threadIdx.x + k * blockDim.x;
-    if (i < width) out[(size_t)blockIdx.x * width + i] = q8_pack1(v[k] * f);
+    if (i < width) out[(size_t)blockIdx.x * width + i] = q8_pack1(to, v[k]);
   }
 }
 
@@ -384,9 +380,9 @@ __global__ void rows_q8_scalar_kernel(const TX* x, long long ldx, unsigned char*
   float top = 0.f;
   for (int i = threadIdx.x; i < width; i += blockDim.x) top = fmaxf(top, fabsf(entry(i)));
   top = block_sum_max(0.f, top, scratch).y;
-  const float f = q8_factor(top);
-  if (threadIdx.x == 0) scale[blockIdx.x] = q8_scale(top);
-  for (int i = threadIdx.x; i < width; i += blockDim.x) out[(size_t)blockIdx.x * width + i] = q8_pack1(entry(i) * f);
+  const Q8Row to(top);
+  if (threadIdx.x == 0) scale[blockIdx.x] = to.scale;
+  for (int i = threadIdx.x; i < width; i += blockDim.x) out[(size_t)blockIdx.x * width + i] = q8_pack1(to, entry(i));
 }
 
 #define Q8_MAX_VEC_WIDTH (4 * 8 * 512)

@@ -567,3 +567,22 @@ def test_gemm_q8_scales_whose_product_is_no_fp32_number(M, N, K):
         out, status = torch.full((M, N), float("nan"), dtype=dtype, device=DEV), status_word()
         ops().gemm_q8(a, sa, w, sw, out, status)
         assert status.item() == 0 and torch.equal(out, want.to(dtype))
+
+
+@pytest.mark.parametrize("shift", [0, 1])
+@pytest.mark.parametrize("dtype", [BF16, F32])
+def test_codes_are_the_nearest_to_the_quotient(dtype, shift):
+    """out[r] = x[r] / scale[r] rounded to e4m3, to the bit: every mantissa a row's largest entry can have in bfloat16, beside every bfloat16 entry of the
+    fourteen binades below it. Many of them lie halfway between two codes."""
+    top = torch.arange(128, 256, device=DEV).float()
+    entries = (torch.arange(128, 256, device=DEV).float() * torch.exp2(torch.arange(-14, 1, device=DEV).float()).unsqueeze(1)).reshape(-1)
+    x = torch.cat([torch.minimum(entries, top.unsqueeze(1)), top.unsqueeze(1).expand(128, 8)], 1)
+    x = x * torch.exp2(torch.arange(128, device=DEV).float() % 5 - 2).unsqueeze(1) * torch.where(torch.arange(x.shape[1], device=DEV) % 2 == 0, 1.0, -1.0)
+    n = x.shape[1]
+    buf = torch.empty(128 * n + shift, dtype=dtype, device=DEV)[shift:].view(128, n)
+    buf.copy_(x)
+    out, scale = torch.empty(128, n, dtype=E4M3, device=DEV), torch.empty(128, device=DEV)
+    ops().quantize_q8(buf, out, scale)
+    # both sides divide in fp32 and then round to e4m3: the same two roundings
+    assert torch.equal(scale, (x.abs().amax(1).double() / 448).to(F32))          # (in fp32 torch multiplies by the inverse of a number)
+    assert torch.equal(out.float(), (x / scale.unsqueeze(1)).clamp(-448, 448).to(E4M3).float())
