@@ -234,9 +234,10 @@ def quantized_layer(layer, weight_format: str):
     if layer.feed_forward is None or layer.feed_forward.kind != "gated_mlp":
         raise ValueError(f"weight format {weight_format!r}: feed-forward kind "
                          f"{None if layer.feed_forward is None else layer.feed_forward.kind!r} has no form for it (only 'gated_mlp')")
-    if layer.arrangement != "pre_norm" or layer.mixer_norm.kind != "rmsnorm" or layer.feed_forward_norm.kind != "rmsnorm" or layer.token_side_prefix is not None:
+    norms = tuple(None if n is None else n.kind for n in (layer.mixer_norm, layer.feed_forward_norm))      # some arrangements have one norm for both
+    if layer.arrangement != "pre_norm" or norms != ("rmsnorm", "rmsnorm") or layer.token_side_prefix is not None:
         raise ValueError(f"weight format {weight_format!r}: goes with the arrangement 'pre_norm' and RMS norms (found {layer.arrangement!r}, "
-                         f"{layer.mixer_norm.kind!r}, {layer.feed_forward_norm.kind!r})")
+                         f"{norms[0]!r}, {norms[1]!r})")
     with_format = lambda spec, kind: replace(spec, kind=kind, params={**spec.params, "weight_format": weight_format})
     return replace(layer, mixer=with_format(layer.mixer, "quantized_attention"), feed_forward=with_format(layer.feed_forward, "quantized_gated_mlp"),
                    arrangement="pre_norm_q8" if weight_format == "q8" else "pre_norm")

@@ -238,3 +238,15 @@ def test_aligned_cluster_barriers_are_met_by_whole_warps():
     body = found["tma_common.cuh"].split("void cluster_sync_all() {")[1].split("}")[0]
     assert found["tma_common.cuh"].count("barrier.cluster.arrive") == 1 and found["tma_common.cuh"].count("barrier.cluster.wait") == 1
     assert body.index("__syncwarp();") < body.index("barrier.cluster.arrive") < body.index("barrier.cluster.wait")
+
+
+@pytest.mark.parametrize("family", ["fevosun", "mivorax", "nufasun", "risizen", "samulorn", "vibunex"])
+@pytest.mark.parametrize("fmt", ["q8", "w4"])
+def test_models_without_a_form_for_the_formats_are_refused_by_name(family, fmt):
+    """Every configuration of the other architectures, layers with one norm for both sublayers among them."""
+    import importlib
+    from llm_steadyinfer_b200.config import config_from_dict
+    from llm_steadyinfer_b200.models import Model
+    for config in importlib.import_module(family + "_configs").CONFIGS.values():
+        with pytest.raises(ValueError, match="has no form for it|goes with the arrangement"):
+            Model(config_from_dict(config[0] if isinstance(config, tuple) else config), torch.bfloat16, "cpu", fmt)
