@@ -21,7 +21,7 @@ import torch
 
 from ..csrc import ops
 from .attention import Attention
-from .base import SummedDelta, register_feed_forward, register_mixer
+from .base import register_feed_forward, register_mixer
 from .block import register_arrangement
 from .mlp import GatedMLP
 from .norm import RMSNorm
@@ -205,11 +205,9 @@ register_feed_forward("quantized_gated_mlp", QuantizedGatedMLP)
 
 
 def norm_q8(norm: RMSNorm, resid, delta, out: Q8Rows, ahead=None) -> None:
-    """``resid += delta`` and the norm of it as 8-bit rows; ``delta`` as ``Norm.forward`` takes it, but for results with a norm of their own."""
-    second = None
-    if isinstance(delta, SummedDelta):
-        delta, second = delta.a, delta.b
-    ops.add_rmsnorm_q8(resid, delta, norm.weight, norm.eps, out.codes, out.scale, delta2=second, ahead=ahead)
+    """``resid += delta`` and the norm of it as 8-bit rows; ``delta``: the result of the sublayer before, or None. (Blocks of "pre_norm" hand on nothing
+    else, and a format's layers have no other arrangement.)"""
+    ops.add_rmsnorm_q8(resid, delta, norm.weight, norm.eps, out.codes, out.scale, ahead=ahead)
 
 
 def pre_norm_q8(block, resid, delta, ctx, cache):
