@@ -236,11 +236,12 @@ SI_EXPORT int si_gemm_quant_q8(const void* a, long long lda, const float* x_scal
 }
 
 // x [M, K] bf16; w [N, K / 8] int32 words, rows `ldw` words apart; scales bf16 [N, ceil(K / group)], zeros uint8 like them or null (8);
-// K a multiple of 8, group of 32.
+// K a multiple of 8, group of 32. (K up to 2^30 - 32: the end of a row's last step of 32 entries, in bytes, has to stay below 2^31, or the check of a load
+// against the row's end turns around.)
 SI_EXPORT int si_gemm_quant_w4(const void* x, long long ldx, const void* w, long long ldw, const void* scales, const void* zeros, int group,
                                void* out, long long ldo, int out_dtype, int M, int N, int K, cudaStream_t stream) {
   if (M <= 0 || N <= 0) return 0;
-  if (K <= 0 || K % 8 || K > 0x3fffffff || group <= 0 || group % 32) return -2;
+  if (K <= 0 || K % 8 || K > 0x3fffffe0 || group <= 0 || group % 32) return -2;
   QuantProduct p = {};
   p.x = x; p.ldx = ldx; p.w = w; p.ldw = ldw; p.scales = (const bf16*)scales; p.zeros = (const unsigned char*)zeros;
   p.group = group; p.groups = (K - 1) / group + 1; p.M = M; p.N = N; p.K = K;

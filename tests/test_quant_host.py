@@ -250,3 +250,16 @@ def test_models_without_a_form_for_the_formats_are_refused_by_name(family, fmt):
     for config in importlib.import_module(family + "_configs").CONFIGS.values():
         with pytest.raises(ValueError, match="has no form for it|goes with the arrangement"):
             Model(config_from_dict(config[0] if isinstance(config, tuple) else config), torch.bfloat16, "cpu", fmt)
+
+
+def test_rows_whose_last_step_ends_beyond_32_bits_are_refused():
+    """4-bit weights on no 16-byte boundary: 2^30 - 8 entries of x are 2^31 - 16 bytes, and the last of a step's four loads of 16 bytes would begin there: its
+    end passes 2^31 - 1 and compares as below the row's length. The entry returns before it launches anything (null pointers are not touched)."""
+    import ctypes
+    from llm_steadyinfer_b200.csrc import build
+    fn = build.load("gemm_quant").si_gemm_quant_w4
+    fn.argtypes, fn.restype = ops._GEMM_QUANT_W4_ARGS, ctypes.c_int
+    for K in (2 ** 30 - 8, 2 ** 30 - 16, 2 ** 30 - 24):
+        assert 2 * (32 * (-(-K // 32)) - 8) + 16 > 2 ** 31 - 1
+        assert fn(None, K, None, K // 8, None, None, 128, None, 1, 0, 1, 1, K, None) == -2
+    assert 2 * (2 ** 30 - 32 - 8) + 16 <= 2 ** 31 - 1          # the longest row that is taken
