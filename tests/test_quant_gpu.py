@@ -586,3 +586,105 @@ def test_codes_are_the_nearest_to_the_quotient(dtype, shift):
     # both sides divide in fp32 and then round to e4m3: the same two roundings
     assert torch.equal(scale, (x.abs().amax(1).double() / 448).to(F32))          # (in fp32 torch multiplies by the inverse of a number)
     assert torch.equal(out.float(), (x / scale.unsqueeze(1)).clamp(-448, 448).to(E4M3).float())
+
+
+@pytest.mark.parametrize("M,m", [(2, 1), (8, 3), (16, 9), (33, 20), (128, 127), (140, 128), (300, 257), (600, 1)])
+@pytest.mark.parametrize("K", [4096, 4088])
+def test_rows_of_a_product_stand_alone(M, m, K):
+    """A row's result does not change with what the rows behind it hold: NaN there, or other numbers."""
+    g = gen(M + K)
+    N = 520
+    a, w = torch.empty(M, K, dtype=E4M3, device=DEV), torch.empty(N, K, dtype=E4M3, device=DEV)
+    sa, sw = torch.empty(M, device=DEV), torch.empty(N, device=DEV)
+    ops().quantize_q8(torch.randn(M, K, generator=g, device=DEV), a, sa)
+    ops().quantize_q8(torch.randn(N, K, generator=g, device=DEV), w, sw)
+    words, s, z, _ = w4_weight(g, N, K, 128, True, whole=False)
+    x = torch.randn(M, K, generator=g, device=DEV).to(BF16)
+    first = None
+    for behind in (None, 3.0, float("nan"), float("inf")):
+        if behind is not None:
+            a[m:], sa[m:], x[m:] = behind, behind, behind
+        out, out4, status = torch.empty(M, N, device=DEV), torch.empty(M, N, device=DEV), status_word()
+        ops().gemm_q8(a, sa, w, sw, out, status)
+        ops().gemm_w4(x, words, s, z, 128, out4, status)
+        assert status.item() == 0
+        if first is None:
+            first = (out, out4)
+        assert torch.equal(out[:m], first[0][:m]) and torch.equal(out4[:m], first[1][:m])
+
+
+@pytest.mark.parametrize("M", [1, 8, 40, 128, 300])
+@pytest.mark.parametrize("K,ld", [(250, 256), (257, 272), (1001, 1008), (4090, 4096), (8, 16)])
+def test_gemm_q8_rows_that_end_before_their_stride(M, K, ld):
+    """Rows on 16-byte boundaries whose length is no multiple of 16: the tcgen05 kernels' last box ends inside the row's padding, which holds NaN."""
+    g = gen(M + K)
+    N = 200
+
+    def laid(rows):
+        buf = torch.full((rows, ld), float("nan"), device=DEV).to(E4M3)
+        buf[:, :K] = whole_codes(g, rows, K)
+        return buf[:, :K]
+
+    a, w, sa, sw = laid(M), laid(N), powers(g, M), powers(g, N)
+    want = (torch.mm(a.double(), w.double().t()) * sa.double().unsqueeze(1) * sw.double()).to(F32)
+    out, status = torch.full((M, N), float("nan"), device=DEV), status_word()
+    ops().gemm_q8(a, sa, w, sw, out, status)
+    assert status.item() == 0 and torch.equal(out, want)
+
+
+@pytest.mark.parametrize("M", [1, 8, 40, 128, 300])
+@pytest.mark.parametrize("K,ldx,ldw", [(1056, 1064, 136), (288, 512, 64), (4000, 4008, 504), (512, 520, 68)])
+def test_gemm_w4_rows_that_end_before_their_stride(M, K, ldx, ldw):
+    g = gen(M + K)
+    N = 200
+    words, s, z, w = w4_weight(g, N, K, 32, True)
+    wbuf = torch.full((N, ldw), -1, dtype=torch.int32, device=DEV)
+    wbuf[:, :K // 8] = words
+    xbuf = torch.full((M, ldx), float("nan"), dtype=BF16, device=DEV)
+    xbuf[:, :K] = torch.randint(-4, 5, (M, K), generator=g, device=DEV).to(BF16)
+    want = torch.mm(xbuf[:, :K].double(), w.t()).to(F32)
+    out, status = torch.full((M, N), float("nan"), device=DEV), status_word()
+    ops().gemm_w4(xbuf[:, :K], wbuf[:, :K // 8], s, z, 32, out, status)
+    assert status.item() == 0 and torch.equal(out, want)
+
+
+@pytest.mark.parametrize("M", [1, 2, 5, 8])
+@pytest.mark.parametrize("N,K,group,zeros", [(2048, 4096, 128, True), (512, 512, 256, False), (1000, 2816, 128, False), (256, 14336, 256, True), (96, 256, 1024, True)])
+def test_gemm_w4_few_rows_round_no_weight(M, N, K, group, zeros):
+    """Up to eight rows, groups of 128 and more, K a multiple of 256: a weight times its scale is never rounded. The products of x and q - z are exact; a
+    product then passes at most 8 instructions of 16 products and a sum (17 additions each), the sum of two chunks of 128, of 16 warps and of 8 blocks, and a
+    multiplication by the scale: 162 steps, each off by at most 2^-23 of the products' sizes. One rounding of each weight to bf16 would be off by some
+    2^-9 / sqrt(K) of them, ten times as much and more over so many results."""
+    g = gen(M + K)
+    words, s, z, w = w4_weight(g, N, K, group, zeros, whole=False)
+    x = torch.randn(M, K, generator=g, device=DEV).to(BF16)
+    want, sizes = torch.mm(x.double(), w.t()), torch.mm(x.double().abs(), w.abs().t())
+    out, status = torch.empty(M, N, device=DEV), status_word()
+    ops().gemm_w4(x, words, s, z, group, out, status)
+    assert status.item() == 0 and ((out.double() - want).abs() <= 162 * 2.0 ** -23 * sizes).all()
+    rounded = torch.mm(x.double(), w.to(BF16).double().t())
+    assert ((rounded - want).abs() > 162 * 2.0 ** -23 * sizes).any()          # the bound tells the two apart
+
+
+@pytest.mark.parametrize("captured", [False, True])
+def test_norm_takes_a_weight_that_was_just_written(captured):
+    o, n = ops(), 4096
+    resid, weight = torch.ones(8, n, device=DEV), torch.ones(n, device=DEV, dtype=BF16)
+    out, scale = torch.empty(8, n, dtype=E4M3, device=DEV), torch.empty(60, 8, device=DEV)
+
+    def run():
+        for i in range(60):
+            weight.fill_(2.0 ** (i % 7))
+            o.add_rmsnorm_q8(resid, None, weight, 0.0, out, scale[i])
+
+    run()
+    if captured:
+        graph = torch.cuda.CUDAGraph()
+        torch.cuda.synchronize()
+        with torch.cuda.graph(graph):
+            run()
+    want = torch.exp2((torch.arange(60, device=DEV) % 7).float()).unsqueeze(1) / 448
+    for _ in range(20):
+        scale.zero_()
+        graph.replay() if captured else run()
+        assert ((scale - want).abs() <= 2.0 ** -20 * want).all()
