@@ -302,6 +302,7 @@ gemm_q8_rows_kernel(const __grid_constant__ CUtensorMap amap, const __grid_const
   __syncthreads();
   tc05_fence_after_sync();
   const unsigned tmem = tmem_slot;
+  bool plain = true;                                       // the scales' products are normal numbers
   // Stages and phases are counted along: a division a step, in the one thread that feeds a pipeline, cost 80 clocks a step.
   if (warp < 2) {                                          // warp 0 fetches w, warp 1 a: each boxes of its own
     if (lane == 0) {
@@ -358,14 +359,15 @@ gemm_q8_rows_kernel(const __grid_constant__ CUtensorMap amap, const __grid_const
       if (++s == STAGES) { s = 0; wd = wd0; ad = ad0; phase ^= 1u; }
     }
     if (!ok && lane == 0) set_status(status, SI_WAIT_LIMIT);
-  } else if (warp - 3 < 4 * halves) {                       // four warps an accumulator, 32 of its lanes each
+  } else {
     pdl_wait();
+    const float2 rows = q8_range(sa, 0, M), cols = q8_range(sw, n0, min(n0 + h, N));      // while the product runs
+    plain = q8_normal(rows.x * cols.x) && q8_normal(rows.y * cols.y);
+  }
+  if (warp >= 3 && warp - 3 < 4 * halves) {                 // four warps an accumulator, 32 of its lanes each
     const int acc = (warp - 3) >> 2, c = acc * 128 + (warp & 3) * 32 + lane, n = n0 + c;
     const bool in = c < h && n < N;
     const float cs = in ? sw[n] : 0.f;
-    float2 rows = make_float2(1.f, 1.f);
-    if (parts == 1) rows = q8_range(sa, 0, M);              // alike for the block: all lanes take part
-    const bool plain = !in || q8_plain(cs, rows);
     const bool ok = mbar_wait_warp(&acc_full, 0);         // every part has a step at least
     if (!ok && lane == 0) set_status(status, SI_WAIT_LIMIT);
     tc05_fence_after_sync();
@@ -376,13 +378,15 @@ gemm_q8_rows_kernel(const __grid_constant__ CUtensorMap amap, const __grid_const
       __syncwarp();                                        // an aligned load: not every lane stored in the turn before
       tmem_ld_32x32(src + m0, v);
       if (parts == 1) {
-        if (!plain) {
+        if (plain) {
 #pragma unroll
-          for (int j = 0; j < 32; ++j) if (m0 + j < M) v[j] = q8_scaled_wide(v[j], sa[m0 + j], cs);
+          for (int j = 0; j < 32; ++j)
+            if (m0 + j < M && in) out[(size_t)(m0 + j) * ldo + n] = from_f32<TO>(v[j] * (sa[m0 + j] * cs));
+        } else {
+#pragma unroll
+          for (int j = 0; j < 32; ++j)
+            if (m0 + j < M && in) out[(size_t)(m0 + j) * ldo + n] = from_f32<TO>(q8_scaled(v[j], sa[m0 + j], cs));
         }
-#pragma unroll
-        for (int j = 0; j < 32; ++j)
-          if (m0 + j < M && in) out[(size_t)(m0 + j) * ldo + n] = from_f32<TO>(plain ? v[j] * (sa[m0 + j] * cs) : v[j]);
       } else {
 #pragma unroll
         for (int j = 0; j < 32; ++j)
@@ -407,17 +411,10 @@ gemm_q8_rows_kernel(const __grid_constant__ CUtensorMap amap, const __grid_const
         const float rs = sa[m];
         const float r[4] = {v[0].x, v[0].y, v[0].z, v[0].w};
         TO* dst = out + (size_t)m * ldo + n;
-        if (vec && n + 4 <= N) {
+        if (plain && vec && n + 4 <= N) {
           float y[4];
 #pragma unroll
-          for (int j = 0; j < 4; ++j) y[j] = rs * sw[n + j];
-          if (q8_normal(y[0]) && q8_normal(y[1]) && q8_normal(y[2]) && q8_normal(y[3])) {
-#pragma unroll
-            for (int j = 0; j < 4; ++j) y[j] *= r[j];
-          } else {
-#pragma unroll
-            for (int j = 0; j < 4; ++j) y[j] = q8_scaled_wide(r[j], rs, sw[n + j]);
-          }
+          for (int j = 0; j < 4; ++j) y[j] = r[j] * (rs * sw[n + j]);
           if constexpr (sizeof(TO) == 4) {
             *reinterpret_cast<float4*>(dst) = make_float4(y[0], y[1], y[2], y[3]);
           } else {
