@@ -1,9 +1,9 @@
 // Product of 8-bit rows with 8-bit weights: out[m, n] = sa[m] * sw[n] * sum_k a[m, k] * w[n, k], a [M, K] and w [N, K] in e4m3, scales fp32,
 // sums fp32, bf16 or fp32 output. Both operands go to the tensor cores as they lie in memory; the scales, one a row and one a column, are
 // applied to the finished sums. Three kernels by the number of rows:
-//   up to 16 rows    a stream of the weights through the fragments of mma.sync (no shared memory on the way)
-//   17 to 128        tcgen05 the other way round, 128 rows of w a tile, its k range cut over a cluster
-//   more             tcgen05, pairs of CTAs on tiles of 256 rows by 256, 128 or 64 columns
+//   up to 8 rows, and up to 16 where the matrix is small    a stream of the weights through the fragments of mma.sync (no shared memory on the way)
+//   up to 256        tcgen05 the other way round, up to 256 rows of w a tile, its k range cut over a cluster
+//   more, and from a few rows on where an estimate says it is sooner done    tcgen05, pairs of CTAs on tiles of 256 rows by 256, 128 or 64 columns
 // Rows that do not start on 16-byte boundaries go to gemm_quant.cu instead. The bf16 siblings are gemm_skinny.cu, gemm_rows.cu and gemm_tc05.cu;
 // the reference sends every product to cuBLAS (src/source/op/kernels/cuda/matmul_kernel.cu:128-150) and has no 8-bit form.
 //
@@ -212,8 +212,8 @@ gemm_q8_pair_kernel(const __grid_constant__ CUtensorMap amap, const __grid_const
 }
 
 // Columns of a pair's tile: those for which the busiest pair is done first. In clocks: 256 entries of k take 1,120, 750 or 630 with tiles of 256, 128 and
-// 64 columns, what comes before and after them 15,800, 10,560 and 9,300 once. us with 64, 128, 256: 512 x 4,096 x 14,336 41, 28, 42; 512 x 2,048 x
-// 2,048 7.7, 8.1, 12.6; 1,024 x 6,144 x 4,096 36, 24, 28; 1,024 x 4,096 x 14,336 78, 50, 46; 2,048 x 6,144 x 4,096 70, 52, 39.
+// 64 columns, what comes before and after them 15,800, 10,560 and 9,300 once. us with 64, 128, 256: 512 x 4,096 x 14,336 42, 28, 41; 512 x 2,048 x
+// 2,048 7.3, 8.1, 12.4; 1,024 x 6,144 x 4,096 37, 24, 28; 1,024 x 4,096 x 14,336 79, 50, 44; 2,048 x 6,144 x 4,096 65, 43, 40.
 static int q8_pair_columns(int M, int N, int K, long long* cost) {
   const long long slots = si_sm_count() / 2, m_tiles = (M + 255) / 256, nk = (K + 255) / 256;
   int best = 256;
@@ -257,8 +257,8 @@ static int q8_pair(const Q8Call& c) {
 // instructions and a commit cost the issuing thread some 430 clocks a step whatever the step's bytes (steps of 128 took 520 in all, so 256 are
 // taken), and a block some 3 us to begin, to meet the others and to end. The height h, any multiple of 8 up to 256, is chosen with the cut of k so that the
 // SMs share the bytes evenly (q8_rows_shape). The k range of a tile may be cut over the blocks of a cluster: each leaves its sums in its shared
-// memory, and block r adds the r-th part of the rows up over all blocks, in their order. us (TB/s of the weights): 61 x 28,672 x 4,096 24.3 (4.8),
-// 61 x 4,096 x 14,336 14.2 (4.1), 61 x 6,144 x 4,096 9.8, 128 x 4,096 x 14,336 16.5.
+// memory, and block r adds the r-th part of the rows up over all blocks, in their order. us (TB/s of the weights): 61 x 28,672 x 4,096 24.5 (4.8),
+// 61 x 4,096 x 14,336 14.2 (4.1), 61 x 6,144 x 4,096 10.0, 128 x 4,096 x 14,336 16.7.
 #define Q8_ROWS_MAX 256
 #define Q8_ROWS_SMEM (208 * 1024)
 #define Q8_ROWS_MAX_STAGES 8
@@ -608,10 +608,10 @@ gemm_q8_skinny_kernel(const u8* a, long long lda, const float* sa, const u8* w, 
 }
 
 // How many blocks and warps, us (a launch behind a launch, eight rows). Blocks go through the tiles in turn wherever tiles are more than run at
-// once: 28,672 x 4,096 24.6 a block a tile, 18.2 so. Four warps a block where K fills no more or all tiles then run at once: 2,048 x 2,048 3.3 with
+// once: 28,672 x 4,096 24.6 a block a tile, 18.4 so. Four warps a block where K fills no more or all tiles then run at once: 2,048 x 2,048 3.3 with
 // eight, 2.9; 6,144 x 4,096 7.0, 6.6. Sixteen where tiles are fewer than SMs and K is more than a round of eight: 2,048 x 8,192 8.8 and 7.0 (16 rows).
-// Nine to sixteen rows hold half as many weights in flight; a matrix of more than this goes to the tcgen05 kernel: 4,096 x 4,096 5.8 here, 6.6
-// there; 11,264 x 2,048 7.9, 8.0; 6,144 x 4,096 9.3, 8.1; 28,672 x 4,096 25.2, 21.6.
+// Nine to sixteen rows hold half as many weights in flight; a matrix of more than this goes to the tcgen05 kernel: 4,096 x 4,096 5.9 here, 6.6
+// there; 11,264 x 2,048 8.0, 8.0; 6,144 x 4,096 9.3, 8.4; 28,672 x 4,096 25.2, 21.7.
 #define Q8_SKINNY_16_MOST (22LL << 20)
 template <typename TO>
 static int q8_skinny(const Q8Call& c) {
@@ -632,8 +632,8 @@ static int q8_skinny(const Q8Call& c) {
   return si_last_error();
 }
 
-// Up to 256 rows the two tcgen05 kernels' costs are compared. us (one CTA and k cut, pairs): 112 x 2,048 x 2,048 8.5, 6.8; 112 x 4,096 x 4,096 9.3, 10.4;
-// 136 x 4,096 x 14,336 17.0, 23.5; 136 x 28,672 x 4,096 32.5, 31.6; 176 x 2,048 x 8,192 14.3, 14.9; 256 x 4,096 x 4,096 13.7, 10.5.
+// Up to 256 rows the two tcgen05 kernels' costs are compared. us (one CTA and k cut, pairs): 112 x 2,048 x 2,048 9.0, 6.6; 112 x 4,096 x 4,096 9.6, 9.9;
+// 136 x 4,096 x 14,336 17.2, 23.5; 136 x 28,672 x 4,096 32.6, 30.2; 176 x 2,048 x 8,192 14.6, 14.8; 256 x 4,096 x 4,096 13.9, 10.1.
 template <typename TO>
 static int q8_any(const Q8Call& c) {
   if (c.K % 16 == 0 && (c.M <= 8 || (c.M <= 16 && (long long)c.N * c.K <= Q8_SKINNY_16_MOST))) return q8_skinny<TO>(c);

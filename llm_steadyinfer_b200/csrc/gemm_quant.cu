@@ -6,12 +6,12 @@
 // Tiles of 64 rows of x by 128 output columns, eight warps as 2 x 4, 32-wide k steps through two buffers of shared memory; the next step's
 // operands are on their way to registers while mma.sync runs on this one's. The operands are widened on the way to shared memory to a type that
 // holds every value exactly: e4m3 to fp16 (its range and its three mantissa bits fit), bf16 stays. A 4-bit weight times its scale is rounded
-// to bf16 there (off by at most 2^-8 of its value), as gemm_w4.cu does for many rows. Sums are fp32. Rows of 32 entries lie 80 bytes apart:
+// to bf16 there (off by at most 2^-8 of its value) whatever the number of rows, as gemm_w4.cu does for many. Sums are fp32. Rows of 32 entries lie 80 bytes apart:
 // ldmatrix's eight rows then fall into different banks.
 //
 // Where tiles are fewer than blocks that run at once, the k steps of one are shared by the blocks of a cluster; each leaves its sums in its shared memory
 // and adds a part of the rows up over all blocks, in their order (us with one block a tile and so: 8 bits 8 x 4,000 x 4,088 137, 25; 61 x 500 x 7,000 236, 35;
-// 4 bits 212, 37 and 303, 45).
+// 4 bits 212, 37 and 303, 45; the first of them with rows of w on no 8-byte boundary, whose bytes come one by one, 45 to 55).
 #include "tma_common.cuh"
 #include "quant_common.cuh"
 

@@ -1,9 +1,9 @@
 // Product of bf16 rows with 4-bit weights: out[m, n] = sum_k x[m, k] * s[n, k / group] * (q[n, k] - z[n, k / group]), sums fp32, bf16 or fp32
 // output. q lies in int32 words of eight entries (quant_common.cuh); the weights are widened in registers on their way to the tensor cores and
 // never written anywhere in between. Two kernels by the number of rows:
-//   up to 8 rows     a stream of the weights through the fragments of mma.sync; q - z is exact in bf16, and with groups of 128 and more the scale is
-//                    applied to the fp32 sum of a group, so that no weight is rounded
-//   more             tcgen05 the other way round: 128 rows of the weight matrix are the M of the instruction and come to it through tensor memory,
+//   up to 8 rows, K a multiple of 256 up to 32,768    a stream of the weights through the fragments of mma.sync; q - z is exact in bf16, and with groups
+//                    of 128 and more the scale is applied to the fp32 sum of a group, so that no weight is rounded
+//   else             tcgen05 the other way round: 128 rows of the weight matrix are the M of the instruction and come to it through tensor memory,
 //                    widened and scaled by the warps that own their lanes; a weight times its scale is rounded to bf16 once (2^-8 of it at
 //                    most: a scale has eight bits and q - z five, and the instruction takes eight)
 // Rows that do not start on 16-byte boundaries go to gemm_quant.cu instead. The reference has no 4-bit form.
@@ -30,15 +30,17 @@ struct W4Call {
 // no weight is rounded. SMALL (groups of 64 and 32): a lane's entries lie in one group, and a weight times its scale is rounded to bf16 (by 2^-8 of
 // it at most), as with more rows.
 //
-// What bounds it is arithmetic: all but fp32 instructions issue every second clock, and eight weights cost three shifts, four masks and four
-// subtractions. Eight rows of 28,672 x 4,096 take 16.8 us (3.5 TB/s), 17.5 with zero points, 18.4 and 20.1 with groups of 64 or 32. Other forms, us: words
+// Eight rows of 28,672 x 4,096 take 16.8 us (3.5 TB/s), 17.5 with zero points, 18.3 and 20.1 with groups of 64 or 32. What bounds it is not told apart.
+// Not memory (34 % of its rate) and not the tensor pipe (15 %); taking entries apart costs three shifts, four masks and four subtractions for eight weights,
+// all but fp32 instructions issue every second clock (ALU 51 %), but without the subtractions it was no faster (below). A unit's full wait and exchange of
+// sums, and 13 units for the busiest SM where 12.1 would be its share, are the rest. Other forms, us: words
 // and x by loads of the lanes, the next words on their way to registers 27.9 and, with all arithmetic taken out, still 23 (a register that a load is to fill
 // cannot be moved); words by a TMA load of every warp's own, scales by its lanes 28.3, 240 instructions a chunk, 130 of them not the product's; by one TMA
 // load a unit and warps for the scales, x in shared memory, the sums added by the same warps behind a barrier 21.9, 203 instructions. Sums that start at
 // -(128 + z) times those of x, without the subtractions: 16.6, but 3.6 for 3.4 at 2,048 x 2,048, and an infinity in x gives NaN. Scales asked for three
 // units ahead: 16.7.
 //
-// More than 4,096 entries a row, or fewer units than SMs: a cluster shares the units, each block with its slice of k; the sums of all units wait in
+// More than 4,096 entries a row: a cluster shares the units, each block with its slice of k; the sums of all units wait in
 // shared memory until the cluster meets, and each block adds up and stores every parts-th unit, in the order of the blocks.
 #define W4_FEW_ROWS 8
 #define W4_FEW_WARPS 16
@@ -673,8 +675,10 @@ gemm_w4_tc_kernel(const __grid_constant__ CUtensorMap xmap, const __grid_constan
         __syncwarp();
         if (lane == 0) {
           if (PAIR) w4_arrive_leader(&ready[slot]); else mbar_arrive(&ready[slot]);
-          mbar_arrive(&w_empty[stage]);                    // not before the words are used: reads of shared memory were seen to end up behind the wait for
-        }                                                  // the slot, after the stage's next words had come
+          // Not before the words are used: given back as soon as they were in registers by the code's order, reads were seen to end up behind the wait
+          // for the slot, after the stage's next words had come. Here their values have gone through the stores to tensor memory, and those are waited for.
+          mbar_arrive(&w_empty[stage]);
+        }
         slot += 2;
         if (slot >= slots) { slot -= slots; ++uses; }
       }
@@ -789,9 +793,9 @@ static int w4_clusters(int size) {
 // The shape for which the busiest SM is done first, in clocks: a step of 256 is bn * 8 of the tensor cores (4,096 products a clock and SM) and 200 beside them,
 // 1,000 at least (widening, a wait, a commit), and for a CTA alone what taking in its bn rows of x lasts (60 bytes a clock). Where there is one accumulator its
 // stores come on top. More and narrower tiles have to save a sixteenth: they cost more power, at whose cap long products run. us, the rule's choice first
-// (P: two CTAs a tile, then columns and cuts of k): 16 x 4,096 x 4,096 16/4 8.1, 16/2 9.5, 16/1 13.8; 61 x 6,144 x 4,096 64/2 11.3, 64/1 15.4; 128 x
-// 28,672 x 4,096 P128 31.6, 128/1 33.3; 128 x 4,096 x 14,336 128/4 20.5, 64/2 25.4; 200 x 4,096 x 14,336 112/2 28.6, P64 43.3; 300 x 4,096 x 4,096 P80 18.0,
-// 80/1 17.5; 512 x 4,096 x 14,336 P128 52.5, 128/1 55.2, P176 57.6, P256 75.5; 937 x 4,096 x 14,336 P240 81, P112 100; 2,048 x 28,672 x 4,096 P256 363, P128
+// (P: two CTAs a tile, then columns and cuts of k): 16 x 4,096 x 4,096 16/4 8.2, 16/2 9.5, 16/1 13.8; 61 x 6,144 x 4,096 64/2 11.3, 64/1 15.4; 128 x
+// 28,672 x 4,096 P128 32.1, 128/1 33.3; 128 x 4,096 x 14,336 128/4 20.5, 64/2 25.4; 200 x 4,096 x 14,336 112/2 28.6, P64 43.3; 300 x 4,096 x 4,096 P80 18.3,
+// 80/1 17.5; 512 x 4,096 x 14,336 P128 53.1, 128/1 55.2, P176 57.6, P256 75.5; 937 x 4,096 x 14,336 P240 81, P112 100; 2,048 x 28,672 x 4,096 P256 363, P128
 // 357, P192 371.
 static W4Shape w4_shape(int M, int N, int K) {
   const int nk = (K + 255) / 256, fewest = (M + 255) / 256;

@@ -2493,8 +2493,9 @@ def gemm_w4(x, w, scales, zeros, group: int, out, status=None) -> None:
     """out[m, n] = sum_k x[m, k] * scales[n, k / group] * (q[n, k] - zeros[n, k / group]) with weights of four bits: x bf16 [M, K] (rows
     contiguous, K a multiple of 8), ``w`` int32 [N, K / 8], entry i of the eight in a word at bit ``W4_SHIFTS[i]`` (see ``pack_w4``); scales bf16
     [N, ceil(K / group)], zeros uint8 like them (0 .. 15) or None (8 everywhere), ``group`` 32, 64 or a multiple of 128; out bf16 or fp32 [M, N]; sums fp32.
-    A weight times its scale is rounded to bf16 before it is multiplied, except up to eight rows with groups of 128 and more. ``status``: as in
-    ``gemm_q8``."""
+    A weight times its scale is rounded to bf16 before it is multiplied, except up to eight rows where groups are of 128 and more, x and w start their rows
+    on 16-byte boundaries and K is a multiple of 256 up to 32,768 (beyond 4,096 up to some tens of thousands of columns): there a group's fp32 sum is
+    scaled. So a row's result may differ by that rounding between calls of eight rows and of more. ``status``: as in ``gemm_q8``."""
     stream = _here("gemm_w4", x, w, scales, zeros, out, status)
     if x.dtype is not _BF16 or w.dtype is not torch.int32:
         raise KernelError("gemm_w4: x must be bfloat16, w int32 words of eight entries")

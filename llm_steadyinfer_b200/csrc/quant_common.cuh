@@ -71,7 +71,7 @@ __device__ __forceinline__ uint2 q8_pack8(const Q8Row& to, float (&v)[8]) {
 __device__ __forceinline__ unsigned char q8_pack1(const Q8Row& to, float a) { return (unsigned char)__nv_cvt_float_to_fp8(to(a), __NV_SATFINITE, __NV_E4M3); }
 
 // Pair p (entries 2p, 2p + 1) of a word of eight 4-bit entries as two bf16 of value 128 + q: bf16 counts in ones from 128 to 255, so
-// the four bits go straight into the mantissa.
+// the four bits go straight into the mantissa (a widely known way of widening 4-bit entries; the constants follow from the two formats).
 // (Written as one instruction: the compiler makes two of the mask and the or, and such instructions are what bounds the kernels that widen.)
 __device__ __forceinline__ unsigned w4_pair_raw(unsigned word, int p) {
   unsigned v;
