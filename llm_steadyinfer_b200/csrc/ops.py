@@ -2425,7 +2425,7 @@ def add_rmsnorm_q8(resid, delta, weight, eps: float, out, scale, rows=None, ahea
 def swiglu_q8(gu, out, scale, group=None) -> None:
     """``swiglu`` with its output in 8 bits: y = silu(gate) * up (fp32) of the stacked projection gu [T, 2F] (fp32 or bf16, contiguous; gates
     and ups interleaved in groups of ``group`` columns, default F), scale[t] = max(max |y[t]|, 2^-100) / 448, out[t] = y[t] / scale[t] in
-    e4m3 [T, F]. silu of a gate below -87 is taken as zero."""
+    e4m3 [T, F]. silu of a gate below -88.7, where exp(-gate) passes fp32, is zero."""
     stream = _here("swiglu_q8", gu, out, scale)
     shape = out.shape
     if len(shape) != 2:

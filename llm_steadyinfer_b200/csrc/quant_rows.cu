@@ -232,13 +232,23 @@ __global__ void norm_q8_scalar_kernel(const NormArgs a, unsigned char* out, floa
 }
 
 // silu(g) * u with the hardware's exponential of base 2 and reciprocal: off by 2 + 1.2 |g| units where g is negative (and exp(-g) large), by four where it
-// is positive; zero where exp(-g) is beyond 2^126 (g below -87), a value below any code beside entries of ordinary size (subnormal intermediates are taken
-// as zero, which changes no other value). With the accurate functions arithmetic bounded the kernel: 84 us for 2,048 x 14,336, the accurate quotient alone 50 of them.
+// is positive. The reciprocal is that of a quarter of 1 + exp(-g), which it can take up to 2^126 without a subnormal result, and u the other quarter: so all
+// gates down to -88.7, where exp(-g) passes fp32's range and the result is zero, are as the formula has them. (ftz changes exp(-g) alone, where it is nothing
+// beside one.) Two entries at a time. With the accurate functions arithmetic bounded the kernel: 84 us for 2,048 x 14,336, the accurate quotient alone 50 of them.
+__device__ __forceinline__ void silu_mul_q8(float& g0, float& g1, float u0, float u1) {
+  asm("{\n.reg .f32 a, b;\n.reg .b64 g, e, c;\n"
+      "mov.b64 g, {%0, %1};\nmov.b64 c, {%4, %4};\nmul.rn.f32x2 e, g, c;\n"
+      "mov.b64 {a, b}, e;\nex2.approx.ftz.f32 a, a;\nex2.approx.ftz.f32 b, b;\nmov.b64 e, {a, b};\n"
+      "mov.b64 c, {%5, %5};\nfma.rn.f32x2 e, e, c, c;\n"
+      "mov.b64 {a, b}, e;\nrcp.approx.ftz.f32 a, a;\nrcp.approx.ftz.f32 b, b;\nmov.b64 e, {a, b};\n"
+      "mul.rn.f32x2 g, g, e;\nmov.b64 e, {%2, %3};\nmul.rn.f32x2 e, e, c;\nmul.rn.f32x2 g, g, e;\nmov.b64 {%0, %1}, g;\n}\n"
+      : "+f"(g0), "+f"(g1) : "f"(u0), "f"(u1), "f"(-1.4426950408889634f), "f"(0.25f));
+}
 __device__ __forceinline__ float silu_mul_q8(float g, float u) {
   float e, q;
   asm("ex2.approx.ftz.f32 %0, %1;" : "=f"(e) : "f"(g * -1.4426950408889634f));
-  asm("rcp.approx.ftz.f32 %0, %1;" : "=f"(q) : "f"(1.f + e));
-  return g * q * u;
+  asm("rcp.approx.ftz.f32 %0, %1;" : "=f"(q) : "f"(__fmaf_rn(e, 0.25f, 0.25f)));
+  return g * q * (u * 0.25f);
 }
 
 // x as it is: the loaded entries stay packed in registers and are widened twice, before and after the reduction. A block goes through rows, and asks for
@@ -316,9 +326,9 @@ __global__ void __launch_bounds__(512, CHUNKS <= 2 && sizeof(TX) == 2 ? 3 : 2) g
       gate[c].get(v[c]);
       up[c].get(u);
 #pragma unroll
-      for (int i = 0; i < 8; ++i) {
-        v[c][i] = silu_mul_q8(v[c][i], u[i]);
-        top = fmaxf(top, fabsf(v[c][i]));
+      for (int i = 0; i < 8; i += 2) {
+        silu_mul_q8(v[c][i], v[c][i + 1], u[i], u[i + 1]);
+        top = fmaxf(top, fmaxf(fabsf(v[c][i]), fabsf(v[c][i + 1])));
       }
     }
   top = block_sum_max(0.f, top, scratch).y;

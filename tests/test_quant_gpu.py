@@ -688,3 +688,22 @@ def test_norm_takes_a_weight_that_was_just_written(captured):
         scale.zero_()
         graph.replay() if captured else run()
         assert ((scale - want).abs() <= 2.0 ** -20 * want).all()
+
+
+@pytest.mark.parametrize("dtype", [BF16, F32])
+@pytest.mark.parametrize("F", [64, 4096, 4099, 16390])
+def test_swiglu_q8_rows_whose_gates_are_all_far_below_zero(dtype, F):
+    """Gates down to where exp(-gate) is fp32's largest (-88.72), with ups so large that the results are ordinary; one row beyond, all zeros."""
+    g = gen(F)
+    gu = torch.empty(4, 2 * F, device=DEV)
+    gu[:, :F] = -80 - 8.6 * torch.rand(4, F, generator=g, device=DEV)
+    gu[1, :F] = -88.5
+    gu[2, :F] = -87.5
+    gu[3, :F] = -89
+    gu[:, F:] = torch.randn(4, F, generator=g, device=DEV) * 2.0 ** 110
+    gu = gu.to(dtype)
+    out, scale = torch.empty(4, F, dtype=E4M3, device=DEV), torch.empty(4, device=DEV)
+    ops().swiglu_q8(gu, out, scale)
+    gate, up = gu[:3, :F].double(), gu[:3, F:].double()
+    check_rows(out[:3], scale[:3], gate / (1 + torch.exp(-gate)) * up, (6 + 1.173 * 89) * 2.0 ** -23)          # as for other gates
+    assert (out[3].float() == 0).all() and torch.isfinite(scale[3])
