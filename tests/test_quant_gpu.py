@@ -707,3 +707,14 @@ def test_swiglu_q8_rows_whose_gates_are_all_far_below_zero(dtype, F):
     gate, up = gu[:3, :F].double(), gu[:3, F:].double()
     check_rows(out[:3], scale[:3], gate / (1 + torch.exp(-gate)) * up, (6 + 1.173 * 89) * 2.0 ** -23)          # as for other gates
     assert (out[3].float() == 0).all() and torch.isfinite(scale[3])
+
+
+@pytest.mark.parametrize("n", [1000, 1003])
+def test_codes_follow_the_quotient_at_every_size_of_a_row(n):
+    """Rows from below the least maximum to fp32's largest: codes equal the quotient's to the bit, in every binade."""
+    e = torch.arange(-140, 128, device=DEV).double()
+    x = ((torch.rand(268, n, generator=gen(n), device=DEV).double() * 2 - 1) * torch.exp2(e).unsqueeze(1)).float()
+    out, scale = torch.empty(268, n, dtype=E4M3, device=DEV), torch.empty(268, device=DEV)
+    ops().quantize_q8(x, out, scale)
+    assert torch.equal(scale, (x.abs().amax(1).clamp_min(2.0 ** -100).double() / 448).float())
+    assert torch.equal(out.float(), (x / scale.unsqueeze(1)).clamp(-448, 448).to(E4M3).float())
